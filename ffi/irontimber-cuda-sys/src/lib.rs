@@ -62,6 +62,36 @@ pub struct it_mtp_backend_k {
     pub rollback: Option<unsafe extern "C" fn(user: *mut c_void, keep_rows: usize)>,
     pub reset_all: Option<unsafe extern "C" fn(user: *mut c_void)>,
 }
+/// Types, layouts and scalings of the attention block's operators.
+pub const IT_F32: c_int = 0; pub const IT_F16: c_int = 1; pub const IT_BF16: c_int = 2;
+pub const IT_ROPE_HALF: c_int = 0; pub const IT_ROPE_INTERLEAVED: c_int = 1;
+pub const IT_ROPE_SCALE_NONE: c_int = 0; pub const IT_ROPE_SCALE_LINEAR: c_int = 1; pub const IT_ROPE_SCALE_NTK: c_int = 2; pub const IT_ROPE_SCALE_YARN: c_int = 3;
+#[repr(C)] pub struct it_rope { _p: [u8; 0] }
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct it_rope_config { pub n_rot: i32, pub layout: i32, pub scaling: i32, pub base: f64, pub factor: f64, pub original_ctx: f64, pub beta_fast: f64, pub beta_slow: f64 }
+#[repr(C)]
+pub struct it_norm_rope_args {
+    pub type_: i32, pub cache_type: i32, pub rows: i32, pub heads: i32, pub kv_heads: i32, pub head_dim: i32,
+    pub rope: *const it_rope,
+    pub q: *const c_void, pub q_row: i64, pub q_head: i64, pub k: *const c_void, pub k_row: i64, pub k_head: i64, pub v: *const c_void, pub v_row: i64, pub v_head: i64,
+    pub q_out: *mut c_void, pub qo_row: i64, pub qo_head: i64, pub k_cache: *mut c_void, pub kc_slot: i64, pub kc_head: i64, pub v_cache: *mut c_void, pub vc_slot: i64, pub vc_head: i64,
+    pub slots: i64, pub slot0: i64, pub positions: *const i32, pub base: *const i32, pub q_norm: *const f32, pub k_norm: *const f32, pub pos0: i32, pub eps: f32,
+}
+#[repr(C)]
+pub struct it_tree_attention_args {
+    pub type_: i32, pub cache_type: i32, pub rows: i32, pub heads: i32, pub kv_heads: i32, pub head_dim: i32,
+    pub q: *const c_void, pub q_row: i64, pub q_head: i64, pub gate: *const c_void, pub g_row: i64, pub g_head: i64, pub out: *mut c_void, pub o_row: i64, pub o_head: i64,
+    pub k_cache: *const c_void, pub kc_slot: i64, pub kc_head: i64, pub v_cache: *const c_void, pub vc_slot: i64, pub vc_head: i64,
+    pub slots: i64, pub cached: i64, pub parents: *const i32, pub length: *const i32, pub weights: *mut f32, pub w_head: i64,
+    pub workspace: *mut c_void, pub workspace_bytes: usize, pub scale: f32,
+}
+#[repr(C)]
+pub struct it_cache_evict_args {
+    pub kv_heads: i32, pub head_dim: i32, pub k_cache: *mut c_void, pub kc_slot: i64, pub kc_head: i64, pub v_cache: *mut c_void, pub vc_slot: i64, pub vc_head: i64,
+    pub weights: *mut f32, pub w_head: i64, pub kept: *mut i32, pub kept_head: i64, pub slots: i64, pub n: i64, pub keep: i64, pub recent: i64,
+    pub workspace: *mut c_void, pub workspace_bytes: usize,
+}
 pub type it_tok_cb = Option<unsafe extern "C" fn(user: *mut c_void, tok: u32) -> c_int>;
 
 extern "C" {
@@ -171,6 +201,16 @@ extern "C" {
 
     /// Greedy pick on caller-owned device buffers without any allocation (see the header for its limits).
     pub fn it_argmax_static(stream: *mut c_void, logits_dev: *const f32, n: usize, index_dev: *mut u32) -> c_int;
+
+    // ---- the attention block of a host with its own schedule (norm / rope / kv-store / attention dispatches, src/vk/mod.rs:815-840)
+    pub fn it_rope_create(cfg: *const it_rope_config, out: *mut *mut it_rope) -> c_int;
+    pub fn it_rope_destroy(r: *mut it_rope);
+    pub fn it_rope_read(r: *const it_rope, freq: *mut f64, mscale: *mut f64) -> c_int;
+    pub fn it_norm_rope(stream: *mut c_void, a: *const it_norm_rope_args) -> c_int;
+    pub fn it_tree_attention(stream: *mut c_void, a: *const it_tree_attention_args) -> c_int;
+    pub fn it_tree_attention_workspace(a: *const it_tree_attention_args, nbytes: *mut usize) -> c_int;
+    pub fn it_cache_evict(stream: *mut c_void, a: *const it_cache_evict_args) -> c_int;
+    pub fn it_cache_evict_workspace(a: *const it_cache_evict_args, nbytes: *mut usize) -> c_int;
 }
 
 /// The message of the last failure on this thread.

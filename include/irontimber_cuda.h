@@ -325,6 +325,101 @@ int64_t it_engine_generate_mtp_k(it_engine* e, size_t k, const uint32_t* prompt,
  *    streams, no dependency) race on it and give wrong results.  Calls on one stream are safe back to back. */
 int it_argmax_static(void* stream, const float* logits_dev, size_t n, uint32_t* index_dev);
 
+/* ---- the attention block of a host with its own schedule ---------------------------------------------------------
+ * Three operators for hosts that call the products above one by one and keep their own KV cache: norms and rotation of q and k with
+ * the cache store, attention of one token, a chain or a tree of drafted tokens over that cache, and eviction from it.  They
+ * stand where VkEngine records its norm, rope, kv-store and attention dispatches (src/vk/mod.rs:815-840; CPU: src/cpu.rs:134-186), for any
+ * cache a caller owns and for contexts longer than the engine's attention takes; results are rounded, not the reference's bits.
+ *
+ * Conventions of all three: device pointers of the current device and a stream of it (NULL: the default stream), launched in stream
+ * order without waiting and without allocating; the arena and stream of a context (it_arena_ptr, it_ctx_stream) are such pointers and such a
+ * stream.  Strides count elements; the elements of a head are contiguous.  head_dim is a multiple of 8 up to 256, heads a multiple of kv_heads.  Types
+ * are pairs: f32 activations over an f16 cache (as in the engine), or f16 / bf16 for both.  Activation pointers and strides are
+ * aligned to 4 elements, cache pointers to 16 bytes and cache strides to 8 elements.  A cache is [slot][kv head][head_dim] or [kv head][slot][head_dim] or
+ * any other pair of strides; k and v may lie in one buffer.  All may be recorded in a CUDA graph once one call of that entry point on that device
+ * has been made outside of recording.  A call of no rows (keep 0) looks at no pointer and does nothing.  Sums, norms, softmax statistics and accumulators are f32 (angles: 64-bit fractions of a turn). */
+enum { IT_F32 = 0, IT_F16 = 1, IT_BF16 = 2 };
+enum { IT_ROPE_HALF = 0, IT_ROPE_INTERLEAVED = 1 };                                     /* pair i: elements (i, i + n_rot/2), or (2i, 2i + 1) */
+enum { IT_ROPE_SCALE_NONE = 0, IT_ROPE_SCALE_LINEAR = 1, IT_ROPE_SCALE_NTK = 2, IT_ROPE_SCALE_YARN = 3 };
+
+/* Frequencies of a rotation of the first n_rot elements (even, 2..256) of a head: f_i = base^(-2i/n_rot).  LINEAR divides them by factor; NTK replaces base
+ * by base * factor^(n_rot/(n_rot-2)); YARN keeps pairs that turn more than beta_fast times in original_ctx positions, divides those that
+ * turn less than beta_slow times by factor, interpolates between, and multiplies sine and cosine by 0.1 ln(factor) + 1.  factor >= 1.
+ * A host object without device memory: usable on every device, from any thread, until destroyed; calls copy it. */
+typedef struct it_rope it_rope;
+typedef struct it_rope_config {
+    int32_t n_rot, layout, scaling;
+    double base, factor, original_ctx, beta_fast, beta_slow;
+} it_rope_config;
+int it_rope_create(const it_rope_config* cfg, it_rope** out);
+void it_rope_destroy(it_rope* r);
+int it_rope_read(const it_rope* r, double* freq, double* mscale);   /* n_rot / 2 angles per position (radians), and the factor on sine and cosine */
+
+/* For rows t < rows: q head: q_out = rotate(norm(q)); k head: k_cache[slot] = rotate(norm(k)); v_cache[slot] = v, slot = slot0 + t (+ *base).
+ * norm(x) = x / sqrt(mean(x^2) + eps) * weight, per head, skipped where the weight pointer is NULL; rope NULL: no rotation.  The position of row t
+ * is positions[t] (device), or pos0 + t (+ *base) when positions is NULL.  base (device, may be NULL): one i32 added to slots and default
+ * positions, so that a recorded graph can be replayed at other lengths; rows whose slot then falls outside [0, slots) are not stored.
+ * q may be NULL (k and v only) and k, v may be NULL together (q only).  q_out is q itself (same strides) or does not overlap q, k or v.
+ * A head's positions beyond 2^31 do not exist; negative positions rotate backwards. */
+typedef struct it_norm_rope_args {
+    int32_t type, cache_type, rows, heads, kv_heads, head_dim;
+    const it_rope* rope;
+    const void* q; int64_t q_row, q_head;
+    const void* k; int64_t k_row, k_head;
+    const void* v; int64_t v_row, v_head;
+    void* q_out; int64_t qo_row, qo_head;
+    void* k_cache; int64_t kc_slot, kc_head;
+    void* v_cache; int64_t vc_slot, vc_head;
+    int64_t slots, slot0;
+    const int32_t* positions; const int32_t* base;
+    const float* q_norm; const float* k_norm;
+    int32_t pos0; float eps;
+} it_norm_rope_args;
+int it_norm_rope(void* stream, const it_norm_rope_args* a);
+
+/* Attention of `rows` rows (1..256) whose keys and values lie in slots cached .. cached + rows - 1, behind `cached` earlier ones that every row sees.
+ * Row t sees slot cached + j when j == t or j is an ancestor of t: parents[t] (device, i32) is the row it continues, or -1 for one that
+ * continues the cache; a parent that is not a smaller row counts as -1.  parents NULL: a chain, row t sees rows 0..t.
+ * out[t][h] = softmax(scale * q.k) v (* sigmoid(gate[t][h]) when gate is given); scale 0 means head_dim^-1/2.  What masked slots hold
+ * (NaN, infinities, slots behind the last) does not reach the result.  `length` (device i32, may be NULL): the number of cached slots, clamped to
+ * [0, cached], for recorded graphs.  weights (f32, [kv head][slot], slots contiguous, may be NULL): weights[g][slot] += the softmax weight
+ * that the slot received from all rows and all query heads of kv head g; slots that no row sees are left alone.
+ * slots: how many the cache has, >= cached + rows.  out may be q or gate itself (same strides).
+ * workspace: 256-byte aligned device memory of it_tree_attention_workspace() bytes (0: may be NULL), free for other use once the call's work is done;
+ * calls that may overlap need one each.  Results do not depend on it, on the stream, or on chance: the same inputs give the same bits. */
+typedef struct it_tree_attention_args {
+    int32_t type, cache_type, rows, heads, kv_heads, head_dim;
+    const void* q; int64_t q_row, q_head;
+    const void* gate; int64_t g_row, g_head;
+    void* out; int64_t o_row, o_head;
+    const void* k_cache; int64_t kc_slot, kc_head;
+    const void* v_cache; int64_t vc_slot, vc_head;
+    int64_t slots, cached;
+    const int32_t* parents; const int32_t* length;
+    float* weights; int64_t w_head;
+    void* workspace; size_t workspace_bytes;
+    float scale;
+} it_tree_attention_args;
+int it_tree_attention(void* stream, const it_tree_attention_args* a);
+int it_tree_attention_workspace(const it_tree_attention_args* a, size_t* nbytes);    /* looks at sizes only, not at pointers */
+
+/* Cuts a cache of n slots down to `keep` per kv head: the last `recent` slots stay, and of the others the keep - recent with the largest weight
+ * (equal weights: the lower slot; NaN ranks below everything; -0 equals 0).  What stays moves to slots 0..keep-1 in its old order, in place, in k_cache, v_cache
+ * and weights (each may be NULL except weights); kept[g][i] (i32, kept_head apart, may be NULL) is the slot that slot i of head g held before.  Slots from keep on are left
+ * as they were.  0 <= recent <= keep <= n <= slots, n <= 1,048,576.  Works on 16-bit caches of any head_dim that is a multiple of 8 up to 256.
+ * workspace as above, it_cache_evict_workspace() bytes. */
+typedef struct it_cache_evict_args {
+    int32_t kv_heads, head_dim;
+    void* k_cache; int64_t kc_slot, kc_head;
+    void* v_cache; int64_t vc_slot, vc_head;
+    float* weights; int64_t w_head;
+    int32_t* kept; int64_t kept_head;
+    int64_t slots, n, keep, recent;
+    void* workspace; size_t workspace_bytes;
+} it_cache_evict_args;
+int it_cache_evict(void* stream, const it_cache_evict_args* a);
+int it_cache_evict_workspace(const it_cache_evict_args* a, size_t* nbytes);
+
 #ifdef __cplusplus
 }
 #endif

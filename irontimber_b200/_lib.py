@@ -64,6 +64,14 @@ SIGNATURES = {
     "it_matvec_q8": (C.c_int, [P, P, c_size, c_size, c_size, c_size, c_size, C.c_int]),
     "it_argmax": (C.c_int, [P, c_size, c_size, c_size]),
     "it_argmax_static": (C.c_int, [P, P, c_size, P]),
+    "it_rope_create": (C.c_int, [P, C.POINTER(P)]),
+    "it_rope_destroy": (None, [P]),
+    "it_rope_read": (C.c_int, [P, P, P]),
+    "it_norm_rope": (C.c_int, [P, P]),
+    "it_tree_attention": (C.c_int, [P, P]),
+    "it_tree_attention_workspace": (C.c_int, [P, P]),
+    "it_cache_evict": (C.c_int, [P, P]),
+    "it_cache_evict_workspace": (C.c_int, [P, P]),
     "it_engine_create_synth": (C.c_int, [C.c_int, P, C.c_uint64, C.c_int, C.POINTER(P)]),
     "it_engine_create_synth_sharded": (C.c_int, [C.c_int, P, C.c_uint64, C.c_int, C.c_int, C.c_int, C.POINTER(P)]),
     "it_qmatrix_upload_q6_k": (C.c_int, [P, P, c_size, c_size, C.POINTER(P)]),

@@ -82,6 +82,13 @@ class Q8Rows:
             self.handle = None
 
 
+class _Floats:
+    """Device memory for torch.as_tensor to see without a copy."""
+
+    def __init__(self, ptr, shape):
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<f4", "data": (ptr, False), "version": 3}
+
+
 class CudaBackend:
     def __init__(self, device=0, arena_floats=1 << 22):
         self.L = _lib.load()
@@ -90,9 +97,13 @@ class CudaBackend:
         self.ctx = h
         self.arena_floats = arena_floats
         self.device = device
+        self._torch_stream, self._workspaces = None, []
 
     def close(self):
         if self.ctx:
+            if self._workspaces:               # torch's allocator hands them on without waiting for this stream
+                self.sync()
+                self._workspaces = []
             self.L.it_ctx_destroy(self.ctx)
             self.ctx = None
 
@@ -239,6 +250,49 @@ class CudaBackend:
     def argmax(self, off, n, dst):
         """argmax dispatch (src/vk/mod.rs:866): stores the u32 index bit-cast into arena[dst]."""
         _lib.check(self.L.it_argmax(self.ctx, off, n, dst))
+
+    # ---- the attention block (attention.py) on this backend's stream ----------------------------------------------------
+    def view(self, off, *shape):
+        """Arena elements off .. as a torch tensor of this shape (f32), without a copy; valid until close()."""
+        import torch
+        if off % 4 or off + int(np.prod(shape)) > self.arena_floats:
+            raise ValueError(f"elements {off} .. of a shape {shape} in an arena of {self.arena_floats}; offsets are multiples of 4")
+        return torch.as_tensor(_Floats(self.arena_ptr + 4 * off, shape), device=f"cuda:{self.device}")
+
+    @property
+    def torch_stream(self):
+        """The stream as torch sees it (`with torch.cuda.stream(be.torch_stream)` puts torch's work in order with the ops)."""
+        import torch
+        if self._torch_stream is None:
+            self._torch_stream = torch.cuda.ExternalStream(self.stream, device=f"cuda:{self.device}")
+        return self._torch_stream
+
+    def norm_rope(self, rope, q, k, v, q_out, k_cache, v_cache, slot0, positions, **options):
+        """attention.norm_rope on this backend's stream (norm, rope and kv-store dispatches, src/vk/mod.rs:815-832)."""
+        from . import attention
+        attention.norm_rope(rope, q, k, v, q_out, k_cache, v_cache, slot0, positions, stream=self.torch_stream, **options)
+
+    def tree_attention(self, q, k_cache, v_cache, cached, out, **options):
+        """attention.tree_attention on this backend's stream (attention dispatch, src/vk/mod.rs:833-840).  The workspace is the backend's own: one stream
+        orders its uses, those of recorded graphs too, and a larger one does not replace one that a recorded graph knows."""
+        from . import attention
+        if options.get("workspace") is None:
+            options["workspace"] = self._workspace(attention.tree_attention_workspace(q.shape[0], q.shape[1], k_cache.shape[1], q.shape[2], cached, q.dtype))
+        attention.tree_attention(q, k_cache, v_cache, cached, out, stream=self.torch_stream, **options)
+
+    def cache_evict(self, k_cache, v_cache, weights, n, keep, recent, kept=None, **options):
+        """attention.cache_evict on this backend's stream."""
+        from . import attention
+        if kept is None and options.get("workspace") is None:
+            options["workspace"] = self._workspace(4 * k_cache.shape[1] * keep + 256)
+        attention.cache_evict(k_cache, v_cache, weights, n, keep, recent, kept, stream=self.torch_stream, **options)
+
+    def _workspace(self, nbytes):
+        import torch
+        if not self._workspaces or self._workspaces[-1].numel() < nbytes:
+            had = self._workspaces[-1].numel() if self._workspaces else 0
+            self._workspaces.append(torch.empty(max(nbytes, 2 * had, 256), dtype=torch.uint8, device=f"cuda:{self.device}"))
+        return self._workspaces[-1]
 
     def read_u32(self, off):
         return int(self.download(off, 1, np.uint32)[0])

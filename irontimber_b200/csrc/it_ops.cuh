@@ -1,0 +1,54 @@
+// What the operators of the attention block (it_norm_rope.cu, it_tree_attention.cu, it_cache_evict.cu) share: they take raw device pointers
+// and a stream instead of a context, so the device's facts and the word in which a kernel says that a wait ran out live here.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "it_internal.h"
+
+// The current device's SM count and status word (mapped host memory, made by the first call on the device: not while `stream` is recorded).
+struct it_ops_device { int device, sm_count; int *status_host, *status_dev; };
+int it_ops_current(void* stream, const char* who, it_ops_device* out);
+
+static inline bool it_aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+static inline size_t it_type_size(int type) { return type == IT_F32 ? 4 : 2; }
+// Activations over a cache: f32 over f16, or one 16-bit type for both.
+static inline bool it_type_pair(int act, int cache) { return (act == IT_F32 && cache == IT_F16) || (act == IT_F16 && cache == IT_F16) || (act == IT_BF16 && cache == IT_BF16); }
+// Whether [a, a + an) and [b, b + bn) share a byte.
+static inline bool it_overlap(const void* a, size_t an, const void* b, size_t bn) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + bn && y < x + an;
+}
+// Bytes from the first to behind the last element of a [n0][n1][d] array with these strides.
+static inline size_t it_span(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t d, size_t size) {
+    return n0 > 0 && n1 > 0 ? ((size_t)((n0 - 1) * s0 + (n1 - 1) * s1) + (size_t)d) * size : 0;
+}
+// Strides of a [n0][n1][d] array that nothing overlaps itself with: the smaller one holds a head, the larger one all of the other axis.
+static inline bool it_strides_ok(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t d, int64_t unit) {
+    const int64_t most = (int64_t)1 << 38;                     // below the 2^40 bytes of a tensor map's stride
+    if ((n0 > 1 && (s0 < d || s0 % unit || s0 >= most)) || (n1 > 1 && (s1 < d || s1 % unit || s1 >= most))) return false;
+    return n0 <= 1 || n1 <= 1 || (s0 <= s1 ? s1 >= (n0 - 1) * s0 + d : s0 >= (n1 - 1) * s1 + d);
+}
+
+namespace {
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// Four neighbouring elements as one access.
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) { const float4 a = *reinterpret_cast<const float4*>(p); v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; }
+template <class T> __device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
+    union { uint2 u; T e[4]; } a; a.u = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = to_f32(a.e[i]);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+template <class T> __device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
+    union { uint2 u; T e[4]; } a;
+#pragma unroll
+    for (int i = 0; i < 4; i++) a.e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<uint2*>(p) = a.u;
+}
+}  // namespace
