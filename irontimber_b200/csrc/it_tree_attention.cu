@@ -13,98 +13,10 @@
 // done twice; the f16 cache is exact.  16-bit activations: p is rounded to the cache's type like the output itself, q is exact.
 // Masks: only tiles that reach behind the cached slots look at them.  A masked score is replaced, whatever it was; there a non-finite V element is
 // taken out of the product and added to the rows that do see it (0 * inf would be NaN in those that do not).
-#include "it_ops.cuh"
-#include "it_pipe.cuh"
+#include "it_tree_attention.cuh"
 #include <mutex>
 
 namespace {
-
-constexpr int TA_KEYS = 64, TA_MAXROWS = 256, TA_WORDS = TA_MAXROWS / 32, TA_UNIT_MAX = 8;
-constexpr int TA_SMEM_MAX = 226 * 1024;
-constexpr float TA_LOG2E = 1.4426950408889634f;
-constexpr float TA_SHIFT = 14.f;         // p is 2^14 at the maximum: small ones keep their bits in f16
-
-struct TaParams {
-    const void *q, *gate; void* out; const int *parents, *length; float* weights;
-    float* part_o; float2* part_ml; float2* stats; int* status;
-    long long q_row, q_head, g_row, g_head, o_row, o_head, w_head;
-    int rows, heads, group, kv_heads, dim, cached, splits, prows, pad_rows, units; float scale;
-};
-
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-template <class T> struct Ta16;
-template <> struct Ta16<__half> {
-    static constexpr unsigned EXP = 0x7c00u;
-    static __device__ __forceinline__ unsigned pack(float lo, float hi) { const __half2 h = __floats2half2_rn(lo, hi); return *reinterpret_cast<const unsigned*>(&h); }
-    static __device__ __forceinline__ float2 unpack(unsigned u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-    static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-template <> struct Ta16<__nv_bfloat16> {
-    static constexpr unsigned EXP = 0x7f80u;
-    static __device__ __forceinline__ unsigned pack(float lo, float hi) { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const unsigned*>(&h); }
-    static __device__ __forceinline__ float2 unpack(unsigned u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
-    static __device__ __forceinline__ void mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-// The two values of a register with non-finite ones replaced by zero; `seen` collects whether there were any.
-template <class T> __device__ __forceinline__ unsigned finite_only(unsigned u, bool& seen) {
-    const bool lo = (u & Ta16<T>::EXP) == Ta16<T>::EXP, hi = ((u >> 16) & Ta16<T>::EXP) == Ta16<T>::EXP;
-    seen = seen || lo || hi;
-    return u & ((lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u));
-}
-__device__ __forceinline__ void ldsm4(unsigned (&r)[4], unsigned a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(unsigned (&r)[4], unsigned a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(unsigned dst, const void* map, int x, int y, int z, unsigned bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
-}
-// Place of 16-byte piece c (0..7) of row r in a box of 128-byte rows with the 128-byte swizzle.
-__device__ __forceinline__ unsigned swz(int r, int c) { return (unsigned)(r * 128 + ((c ^ (r & 7)) << 4)); }
-
-// Cached slots of this call, and all its slots.
-__device__ __forceinline__ int ta_cached(const TaParams& p) { return p.length ? min(max(*p.length, 0), p.cached) : p.cached; }
-
-// Which rows each row sees, as bits: its parent's set and itself, by following pointers twice as far in every round.  Ends after the rounds it takes
-// for `rows` rows whatever the pointers are; a parent that is not a smaller row counts as none.
-__device__ void ta_ancestors(unsigned (*anc)[TA_WORDS], int* jump, const int* parents, int rows) {
-    const int tid = threadIdx.x, n = blockDim.x;
-    for (int t = tid; t < rows; t += n) {
-        const int q = parents[t];
-        jump[t] = q >= 0 && q < t ? q : -1;
-#pragma unroll
-        for (int w = 0; w < TA_WORDS; w++) anc[t][w] = w == t >> 5 ? 1u << (t & 31) : 0u;
-    }
-    __syncthreads();
-    for (int far = 1; far < rows; far <<= 1) {
-        unsigned add[2][TA_WORDS]; int next[2];
-#pragma unroll
-        for (int k = 0; k < 2; k++) {                       // at least 128 threads: two rows each at most
-            const int t = tid + k * n, j = t < rows ? jump[t] : -1;
-            next[k] = j >= 0 ? jump[j] : -1;
-#pragma unroll
-            for (int w = 0; w < TA_WORDS; w++) add[k][w] = j >= 0 ? anc[j][w] : 0u;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int t = tid + k * n;
-            if (t >= rows) continue;
-            jump[t] = next[k];
-#pragma unroll
-            for (int w = 0; w < TA_WORDS; w++) anc[t][w] |= add[k][w];
-        }
-        __syncthreads();
-    }
-}
 
 // Shared memory: q (twice for f32 activations), then the ring of units (64 slots of K or of V), then the small things.
 template <bool SPLIT, int NB, int R> struct TaSmem {
@@ -129,36 +41,7 @@ __device__ void ta_load_q(const TaParams& p, unsigned char* smem, int g, int r0)
         const int r = r0 + i, t = r / p.group, h = g * p.group + r % p.group;
         const bool live = r < p.prows && 8 * lane < p.dim;
         unsigned hi[4] = {}, lo[4] = {};
-        float f = p.scale * TA_LOG2E;
-        if constexpr (SPLIT) {
-            float v[8] = {};
-            if (live) {
-                const float* x = (const float*)p.q + t * p.q_row + h * p.q_head + 8 * lane;
-                float a[4], b[4]; load4(x, a); load4(x + 4, b);
-#pragma unroll
-                for (int j = 0; j < 4; j++) { v[j] = a[j]; v[4 + j] = b[j]; }
-            }
-            float m = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[j]));
-#pragma unroll
-            for (int s = 16; s; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-            // 2^e brings the largest element to [2^14, 2^15)
-            const int e = min(max(14 - ((int)(__float_as_uint(m) >> 23) - 127), -110), 110);
-            const float up = __uint_as_float((unsigned)(127 + e) << 23);
-            f *= __uint_as_float((unsigned)(127 - e) << 23);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float a = v[2 * j] * up, b = v[2 * j + 1] * up;
-                hi[j] = Ta16<T>::pack(a, b);
-                const float2 h2 = Ta16<T>::unpack(hi[j]);
-                lo[j] = Ta16<T>::pack(a - h2.x, b - h2.y);
-            }
-        } else if (live) {
-            const uint2* x = reinterpret_cast<const uint2*>((const T*)p.q + t * p.q_row + h * p.q_head + 8 * lane);
-            const uint2 a = x[0], b = x[1];
-            hi[0] = a.x; hi[1] = a.y; hi[2] = b.x; hi[3] = b.y;
-        }
+        const float f = ta_q_row<T, SPLIT>(p, live, t, h, lane, hi, lo);
         if (lane < NB * 8) {
             const unsigned at = (unsigned)((lane >> 3) * R * 128) + swz(i, lane & 7);
             *reinterpret_cast<uint4*>(smem + L::Q + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -201,14 +84,6 @@ __device__ __forceinline__ void ta_scores(float (&s)[KT / 8][4], unsigned q0, un
     for (int n = 0; n < KT / 8; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) s[n][i] += s2[n][i];
-}
-
-// Whether row t sees slot j.
-__device__ __forceinline__ bool ta_sees(const TaParams& p, const unsigned (*anc)[TA_WORDS], int t, int j, int cached) {
-    const int i = j - cached;
-    if (i < 0) return true;
-    if (i >= p.rows) return false;
-    return p.parents ? (anc[t][i >> 5] >> (i & 31)) & 1u : i <= t;
 }
 
 template <class T, bool SPLIT, int NB, int WR, int WK>
@@ -581,18 +456,26 @@ k_tree_weights(const __grid_constant__ CUtensorMap kmap, const __grid_constant__
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
 // How a call is cut: rows of a CTA's product tile, tiles of product rows, runs of the cache.
-struct TaPlan { int nb, wr, pad_rows, row_tiles, splits; size_t part_o, part_ml, stats, total; };
+struct TaPlan { bool tc; int nb, wr, nr, pad_rows, row_tiles, splits; size_t part_o, part_ml, stats, total; };
+
+// Which kernel: see the figures at the rule.  IT_TREE=mma|tc forces one (for tests and measurements).
+bool ta_takes_tc(int prows, long slots) {
+    if (const char* v = getenv("IT_TREE")) return v[0] == 't';
+    return true;
+}
 
 TaPlan ta_plan(const it_tree_attention_args* a, int sm_count) {
     TaPlan pl;
     const int group = a->heads / a->kv_heads, prows = a->rows * group;
-    pl.nb = a->head_dim <= 64 ? 1 : a->head_dim <= 128 ? 2 : 4;
-    // four consumer warps (with the producer five: two on one sub-core, which leaves a thread 255 registers; nine warps leave it 168 and spill): 16 product rows each
+    pl.tc = ta_takes_tc(prows, (long)a->cached + a->rows);
+    pl.nb = a->head_dim <= 64 && !pl.tc ? 1 : a->head_dim <= 128 ? 2 : 4;
+    // mma.sync: four consumer warps (with the producer five: two on one sub-core, which leaves a thread 255 registers; nine warps leave it 168 and spill): 16 product rows each
     // share the rows and split a tile's slots, 32: two by two, 64: a warp for 16 rows
     pl.wr = prows <= 16 ? 1 : prows <= 32 ? 2 : 4;
-    pl.row_tiles = (prows + 16 * pl.wr - 1) / (16 * pl.wr);
-    pl.pad_rows = pl.row_tiles * 16 * pl.wr;
-    const long tiles = ((long)a->cached + a->rows + TA_KEYS - 1) / TA_KEYS, ctas = (long)a->kv_heads * pl.row_tiles;
+    pl.nr = 16 * pl.wr;
+    pl.row_tiles = (prows + pl.nr - 1) / pl.nr;
+    pl.pad_rows = pl.row_tiles * pl.nr;
+    const long keys = pl.tc ? 128 : TA_KEYS, tiles = ((long)a->cached + a->rows + keys - 1) / keys, ctas = (long)a->kv_heads * pl.row_tiles;
     long splits = sm_count / ctas;             // one wave of CTAs
     if (splits > tiles) splits = tiles;
     if (splits < 1) splits = 1;
@@ -608,7 +491,7 @@ TaPlan ta_plan(const it_tree_attention_args* a, int sm_count) {
 
 typedef CUresult (*ta_encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-int ta_map(CUtensorMap* map, const void* cache, int type, int dim, int64_t slots, int64_t slot, int heads, int64_t head) {
+int ta_map(CUtensorMap* map, const void* cache, int type, int dim, int64_t slots, int64_t slot, int heads, int64_t head, int keys) {
     static ta_encode_fn encode = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
@@ -620,7 +503,7 @@ int ta_map(CUtensorMap* map, const void* cache, int type, int dim, int64_t slots
     if (heads == 1) head = dim;
     const cuuint64_t dims[3] = { (cuuint64_t)dim, (cuuint64_t)slots, (cuuint64_t)heads };
     const cuuint64_t strides[2] = { (cuuint64_t)slot * 2, (cuuint64_t)head * 2 };
-    const cuuint32_t box[3] = { 64, TA_KEYS, 1 }, estr[3] = { 1, 1, 1 };
+    const cuuint32_t box[3] = { 64, (cuuint32_t)keys, 1 }, estr[3] = { 1, 1, 1 };
     const CUresult r = encode(map, type == IT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(cache), dims, strides, box, estr,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? IT_OK : it_fail(IT_ECUDA, "it_tree_attention: cuTensorMapEncodeTiled failed with code %d", (int)r);
@@ -653,18 +536,17 @@ int ta_prepare(int device) {
     if (const int r = ta_prepare_type<__half, true>()) return r;
     if (const int r = ta_prepare_type<__half, false>()) return r;
     if (const int r = ta_prepare_type<__nv_bfloat16, false>()) return r;
+    if (const int r = it_tree_tc_prepare()) return r;
     done[device] = true;
     return IT_OK;
 }
 
-// A launch that may begin while the kernel before it in the stream still runs; it waits for that kernel itself.
-template <typename... KArgs, typename... Args> cudaError_t ta_launch(bool early, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = early ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, args...);
+int ta_join(const TaParams& p, int type, int nb, cudaStream_t st) {
+    const dim3 grid(p.prows, p.kv_heads), block(64 * nb);
+    auto go = [&](auto kern) -> int { IT_CUDA(ta_launch(true, kern, grid, block, 0, st, p)); return IT_OK; };
+    if (type == IT_F32) return nb == 1 ? go(k_tree_join<float, 1>) : nb == 2 ? go(k_tree_join<float, 2>) : go(k_tree_join<float, 4>);
+    if (type == IT_F16) return nb == 1 ? go(k_tree_join<__half, 1>) : nb == 2 ? go(k_tree_join<__half, 2>) : go(k_tree_join<__half, 4>);
+    return nb == 1 ? go(k_tree_join<__nv_bfloat16, 1>) : nb == 2 ? go(k_tree_join<__nv_bfloat16, 2>) : go(k_tree_join<__nv_bfloat16, 4>);
 }
 template <class T, bool SPLIT, int NB, int WR, int WK>
 int ta_run(const TaParams& p, const TaPlan& pl, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
@@ -729,16 +611,21 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     const TaPlan pl = ta_plan(a, 148);
     IT_CHECK_ARG(a->workspace && it_aligned(a->workspace, 256) && a->workspace_bytes >= pl.total, "%s: a workspace of %zu bytes, 256-byte aligned, is needed", who, pl.total);
     CUtensorMap km, vm;
-    if (const int r = ta_map(&km, a->k_cache, a->cache_type, a->head_dim, a->cached + T, a->kc_slot, a->kv_heads, a->kc_head)) return r;
-    if (const int r = ta_map(&vm, a->v_cache, a->cache_type, a->head_dim, a->cached + T, a->vc_slot, a->kv_heads, a->vc_head)) return r;
+    if (const int r = ta_map(&km, a->k_cache, a->cache_type, a->head_dim, a->cached + T, a->kc_slot, a->kv_heads, a->kc_head, pl.tc ? 128 : TA_KEYS)) return r;
+    if (const int r = ta_map(&vm, a->v_cache, a->cache_type, a->head_dim, a->cached + T, a->vc_slot, a->kv_heads, a->vc_head, pl.tc ? 128 : TA_KEYS)) return r;
     TaParams p;
     char* ws = (char*)a->workspace;
     p.q = a->q; p.gate = a->gate; p.out = a->out; p.parents = a->parents; p.length = a->length; p.weights = a->weights;
     p.part_o = (float*)(ws + pl.part_o); p.part_ml = (float2*)(ws + pl.part_ml); p.stats = a->weights ? (float2*)(ws + pl.stats) : nullptr; p.status = dev.status_dev;
     p.q_row = a->q_row; p.q_head = a->q_head; p.g_row = a->g_row; p.g_head = a->g_head; p.o_row = a->o_row; p.o_head = a->o_head; p.w_head = a->w_head;
     p.rows = a->rows; p.heads = a->heads; p.group = a->heads / a->kv_heads; p.kv_heads = a->kv_heads; p.dim = a->head_dim; p.cached = (int)a->cached; p.splits = pl.splits;
-    p.prows = a->rows * p.group; p.pad_rows = pl.pad_rows; p.units = 0; p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale;
+    p.prows = a->rows * p.group; p.pad_rows = pl.pad_rows; p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale;
     const cudaStream_t st = (cudaStream_t)stream;
+    if (pl.tc) {
+        if (const int r = it_tree_tc_run(p, a->type, pl.nb, pl.nr, pl.row_tiles, km, vm, st)) return r;
+        if (p.splits > 1) if (const int r = ta_join(p, a->type, pl.nb, st)) return r;
+        return p.weights ? it_tree_tc_weigh(p, a->type, pl.nb, pl.nr, km, st) : IT_OK;
+    }
     if (a->type == IT_F32) return ta_run_type<__half, true>(p, pl, km, vm, st);
     if (a->type == IT_F16) return ta_run_type<__half, false>(p, pl, km, vm, st);
     return ta_run_type<__nv_bfloat16, false>(p, pl, km, vm, st);

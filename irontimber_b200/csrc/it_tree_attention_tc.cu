@@ -1,0 +1,584 @@
+// Tree attention on the 5th-generation tensor cores (tcgen05.mma kind::f16, accumulators in tensor memory): the same function as the mma.sync kernel of
+// it_tree_attention.cu, for any number of product rows.
+//
+// Both products are formed with the cache as the first operand, whose 128 rows are always full, and the product rows (row t * group + head) as columns, of which there are
+// as few as 16:   S^T [128 slots x columns] = K [slots x d] . Q^T,    O^T [d x columns] = V^T [d x slots] . P^T
+// so that a decoded token's six rows cost 32 columns and not 128 rows, and everything comes in the layout that it has:
+//   K and V tiles   128 slots as boxes of 64 elements of a tensor map, 128-byte swizzle: K is read K-major, V (as V^T) MN-major
+//   Q               rows of 128-byte pieces, K-major; f32 activations as two sets of columns, high and low halves, added in f32 when they are read
+//   P               [slot][column], MN-major: a thread has one slot (a lane of tensor memory) and stores its columns as 16-byte pieces
+// Warps 0-7 (two groups of four; a group has half of the columns): scores out of tensor memory, running maximum (redux over the slots of a warp, an ordered atomicMax over the four warps),
+// exponentials, P; then the tile before: O^T out of tensor memory into f32 accumulators in registers.  Every tile's product starts from zero and is
+// added with a rounded f32 addition: chained over a long run in tensor memory the hardware's truncating accumulation loses f32's last bits (1.3e-5 of the result after 120 tiles
+// with the mma.sync kernel).  Warp 8: copies.  Warp 9: issues whichever product has its inputs, the next tile's scores or this tile's O.
+// What bounds it: 64 columns of f32 activations (128 with the low halves) 2 x 1024 tensor cycles a tile of 128 slots at head dimension 256; few columns: HBM.
+#include "it_tree_attention.cuh"
+
+namespace {
+
+constexpr int TC_KEYS = 128, TC_THREADS = 384, TC_SOFT = 256;
+constexpr int TC_SMEM_LIMIT = 227 * 1024, TC_SMALL = 3072, TC_SLOTS_MAX = 6;
+constexpr int TC_SOFT_REGS = 216, TC_OTHER_REGS = 72;       // 216 x 256 + 72 x 128 = 64,512 = 168 x 384
+
+template <bool SPLIT, int NB, int NR> struct TcTree {
+    static constexpr int NC = NR * (SPLIT ? 2 : 1), NCB = NC > 64 ? 2 : 1, RW = NR / 2;       // columns of a product, 64-column blocks of P, product rows of a warp group
+    static constexpr int HD = 64 * NB, MT = NB / 2;                                           // M tiles of O^T
+    static constexpr int OR = MT == 2 ? NR : RW;                                              // accumulators of a thread: one element of d, this many product rows
+    static constexpr int QB = NB * NC * 128, PB = NCB * TC_KEYS * 128, SLOT = NB * TC_KEYS * 128, BOX = TC_KEYS * 128;
+    static constexpr int FIT = (TC_SMEM_LIMIT - TC_SMALL - QB - PB) / SLOT, SLOTS = FIT < TC_SLOTS_MAX ? FIT : TC_SLOTS_MAX;
+    static constexpr int KS = (SLOTS + 1) / 2, VS = SLOTS - KS;
+    static constexpr int Q = 0, P = QB, KR = P + PB, VR = KR + KS * SLOT, SMALL = VR + VS * SLOT, TOTAL = SMALL + TC_SMALL;
+    // offsets from SMALL
+    static constexpr int BARS = 0, TMEM = 256, FLAG = 272, MAXES = 512, BASE = 1024, CORR = 1280, FAC = 2048;
+    static constexpr int TCOLS = 2 * NC + MT * NC, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
+    static_assert(VS >= 1 && NR % 16 == 0 && NC <= 128 && NR <= 64 && NC % 16 == 0, "");
+    static_assert(PB >= TA_MAXROWS * TA_WORDS * 4 + TA_MAXROWS * 4, "the ancestors are worked out in P's place");
+};
+
+// Shared-memory descriptors, 128-byte swizzle, version 1.  K-major: 8-row groups 1024 bytes apart.  MN-major: blocks of 64 elements `block` bytes apart, groups of 8 along K 1024 bytes apart.
+__device__ __forceinline__ unsigned long long desc_k(unsigned addr) {
+    return (unsigned long long)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ unsigned long long desc_mn(unsigned addr, unsigned block) {
+    return (unsigned long long)((addr & 0x3FFFFu) >> 4) | ((unsigned long long)(block >> 4) << 16) | ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16 instruction descriptor: D f32, A and B f16 or bf16, M 128, N columns; bits 15 and 16: A and B MN-major
+template <class T> __host__ __device__ constexpr unsigned idesc(int n, bool mn) {
+    constexpr unsigned ty = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (ty << 7) | (ty << 10) | (mn ? (1u << 15) | (1u << 16) : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16(unsigned d, unsigned long long a, unsigned long long b, unsigned id, bool acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void commit_to(unsigned bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory"); }
+__device__ __forceinline__ bool elect_one() {
+    unsigned e;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+// Neighbouring columns of this thread's lane.
+__device__ __forceinline__ void tm_ld(float (&v)[8], unsigned a) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void tm_ld(float (&v)[16], unsigned a) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void tm_ld(float (&v)[32], unsigned a) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+                   "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]) : "r"(a) : "memory");
+}
+// Waits for the loads; the values pass through it so that nothing that uses them moves in front.
+template <int N> __device__ __forceinline__ void tm_wait(float (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
+}
+// Maximum over a warp (NaN left out, as by fmaxf).
+__device__ __forceinline__ float warp_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+// Integers in the order of the floats.
+__device__ __forceinline__ int ordered(float v) { const int i = __float_as_int(v); return i ^ ((i >> 31) & 0x7fffffff); }
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+template <int N> __device__ __forceinline__ void warp_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N> __device__ __forceinline__ void warp_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
+// Barriers of one group of four warps (wg 0 or 1), and of both.
+__device__ __forceinline__ void group_sync(int wg) {
+    if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
+}
+__device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
+
+// Product rows [r0, r0 + NR) of KV head g as columns of Q^T, and for each the factor from the product to log2 of its exponential.
+template <class T, bool SPLIT, int NB, int NR>
+__device__ void tc_load_q(const TaParams& p, unsigned char* q, float* fac, int g, int r0, int warp, int nw, int lane) {
+    using L = TcTree<SPLIT, NB, NR>;
+    for (int i = warp; i < NR; i += nw) {
+        const int r = r0 + i, t = r / p.group, h = g * p.group + r % p.group;
+        const bool live = r < p.prows && 8 * lane < p.dim;
+        unsigned hi[4] = {}, lo[4] = {};
+        const float f = ta_q_row<T, SPLIT>(p, live, t, h, lane, hi, lo);
+        if (lane < NB * 8) {
+            const unsigned at = (unsigned)((lane >> 3) * L::NC * 128) + swz(i, lane & 7);
+            *reinterpret_cast<uint4*>(q + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (SPLIT) *reinterpret_cast<uint4*>(q + at + NR * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        if (lane == 0) fac[i] = f;
+    }
+}
+
+// Whether row t sees tree slot i, by walking up; for the rare case only.
+__device__ __noinline__ bool tc_walk(const int* parents, int t, int i) {
+    if (i > t) return false;
+    if (!parents) return true;
+    while (t > i) { const int q = parents[t]; if (q < 0 || q >= t) return false; t = q; }
+    return t == i;
+}
+
+template <class T, bool SPLIT, int NB, int NR>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TaParams p) {
+    using L = TcTree<SPLIT, NB, NR>;
+    using TA = typename std::conditional<SPLIT, float, T>::type;
+    constexpr int NC = L::NC, RW = L::RW, OR = L::OR, HD = L::HD, KS = L::KS, VS = L::VS;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x, g = blockIdx.y, r0 = blockIdx.z * NR;
+    unsigned char* const small = smem + L::SMALL;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(small + L::FLAG);
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(small + L::TMEM);
+    int* maxes = reinterpret_cast<int*>(small + L::MAXES);              // [2][2][32]
+    float* base_s = reinterpret_cast<float*>(small + L::BASE);          // [NR]
+    float* corr_s = reinterpret_cast<float*>(small + L::CORR);          // [3][NR]
+    float* fac = reinterpret_cast<float*>(small + L::FAC);              // [NR]
+    const unsigned bars = smem_u32(small + L::BARS);
+    const unsigned kfull = bars, kempty = kfull + 8 * KS, vfull = kempty + 8 * KS, vempty = vfull + 8 * VS, sfull = vempty + 8 * VS, sfree = sfull + 16, pfull = sfree + 16, ofull = pfull + 8;
+    const unsigned kring = smem_u32(smem + L::KR), vring = smem_u32(smem + L::VR);
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TC_KEYS - 1) / TC_KEYS;
+    const int tile0 = (int)((long long)split * tiles / p.splits), n = (int)((long long)(split + 1) * tiles / p.splits) - tile0;
+    if (tid == 0) {
+        *abort_flag = (smem_u32(smem) & 1023u) != 0;                 // the swizzle counts on it; never seen
+        for (int s = 0; s < KS; s++) { mbar_init(kfull + 8 * s, 1); mbar_init(kempty + 8 * s, 1); }
+        for (int s = 0; s < VS; s++) { mbar_init(vfull + 8 * s, 1); mbar_init(vempty + 8 * s, 1); }
+        for (int s = 0; s < 2; s++) { mbar_init(sfull + 8 * s, 1); mbar_init(sfree + 8 * s, 8); }
+        mbar_init(pfull, 8); mbar_init(ofull, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (tid >= 128 && tid < 256) maxes[tid - 128] = ordered(-INFINITY);
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)L::ALLOC) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const unsigned tmem = *tmem_slot, otm = tmem + 2 * NC;
+    auto load = [&](bool v, int i) {                // tile i of K or V; the slot is free
+        const int s = v ? i % VS : i % KS;
+        const unsigned dst = (v ? vring : kring) + s * L::SLOT, bar = (v ? vfull : kfull) + 8 * s;
+        mbar_expect_tx(bar, L::SLOT);
+#pragma unroll
+        for (int b = 0; b < NB; b++) tma_load_3d(dst + b * L::BOX, v ? &vmap : &kmap, 64 * b, (tile0 + i) * TC_KEYS, g, bar);
+    };
+    if (warp == 8 && lane == 0) {                   // the first tiles before anything else
+        for (int i = 0; i < n && i < KS; i++) { load(false, i); if (i < VS) load(true, i); }
+    }
+    __syncwarp();
+    tc_load_q<T, SPLIT, NB, NR>(p, smem + L::Q, fac, g, r0, warp, TC_THREADS / 32, lane);
+    const int first_masked = cached / TC_KEYS - tile0;             // tiles from here on reach behind the cached slots
+    unsigned vis[3] = { 0, 0, 0 };                                 // which of the group's product rows see this thread's slot of the first, second, third such tile
+    if (n > first_masked && n > 0) {
+        unsigned (*anc)[TA_WORDS] = reinterpret_cast<unsigned (*)[TA_WORDS]>(smem + L::P);
+        if (p.parents) ta_ancestors(anc, reinterpret_cast<int*>(smem + L::P + TA_MAXROWS * TA_WORDS * 4), p.parents, p.rows);
+        __syncthreads();
+        if (warp < 8) {
+            const int wg = warp >> 2, key = tid & 127;
+            for (int k = 0; k < 3; k++) {
+                unsigned m = 0;
+                const int j = (tile0 + first_masked + k) * TC_KEYS + key;
+                for (int r = 0; r < RW; r++) {
+                    const int t = min((r0 + wg * RW + r) / p.group, p.rows - 1);
+                    if (ta_sees(p, anc, t, j, cached)) m |= 1u << r;
+                }
+                if (k == 0) vis[0] = m; else if (k == 1) vis[1] = m; else vis[2] = m;
+            }
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // Q before the products read it
+    __syncthreads();
+
+    if (warp < 8) {
+        warp_regs_inc<TC_SOFT_REGS>();
+        const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
+        const unsigned lanes = (unsigned)(quad * 32) << 16;
+        const int orow = L::MT == 2 ? 0 : wg * RW, d = (L::MT == 2 ? wg * 128 : 0) + key;        // first product row of the accumulators, their element of the head
+        const unsigned oaddr = otm + lanes + (L::MT == 2 ? wg * NC : 0) + orow;
+        float acc[OR], l[RW], mrun = -INFINITY;                     // mrun: the running maximum of row `lane` of the group
+#pragma unroll
+        for (int r = 0; r < OR; r++) acc[r] = 0.f;
+#pragma unroll
+        for (int r = 0; r < RW; r++) l[r] = 0.f;
+        bool ok = true;
+        auto collect = [&](int i) {                                 // O^T of tile i
+            ok = ok && mbar_wait_warp(ofull, (unsigned)i & 1u, abort_flag, p.status, 52);
+            ok = ok && mbar_wait_warp(pfull, (unsigned)i & 1u, abort_flag, p.status, 53);      // met long ago: the other group's factors are seen through it
+            fence_after();
+            const float* c = corr_s + (i % 3) * NR + orow;
+            constexpr int CH = OR < 16 ? OR : 16;
+#pragma unroll
+            for (int r = 0; r < OR; r += CH) {
+                float a[CH], b[CH];
+                tm_ld(a, oaddr + r);
+                if constexpr (SPLIT) tm_ld(b, oaddr + NR + r);
+                tm_wait(a);
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int x = 0; x < CH; x++) { asm volatile("" : "+f"(b[x])); a[x] += b[x]; }
+                }
+#pragma unroll
+                for (int x = 0; x < CH; x++) acc[r + x] = fmaf(acc[r + x], c[r + x], a[x]);
+            }
+            fence_before();
+        };
+        for (int i = 0; i < n; i++) {
+            const int buf = i & 1;
+            ok = ok && mbar_wait_warp(sfull + 8 * buf, (unsigned)(i >> 1) & 1u, abort_flag, p.status, 51);
+            fence_after();
+            float x[RW];
+            {
+                const unsigned sa = tmem + lanes + buf * NC + wg * RW;
+                tm_ld(x, sa);
+                if constexpr (SPLIT) {
+                    float y[RW];
+                    tm_ld(y, sa + NR);
+                    tm_wait(x);
+#pragma unroll
+                    for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
+                } else tm_wait(x);
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(sfree + 8 * buf);
+            const bool masked = i >= first_masked;
+            const unsigned see = masked ? (i == first_masked ? vis[0] : i == first_masked + 1 ? vis[1] : vis[2]) : 0xffffffffu;
+            float mine = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < RW; r++) {
+                x[r] *= fac[wg * RW + r];
+                if (masked && !((see >> r) & 1u)) x[r] = -INFINITY;
+                const float m = warp_max(x[r]);
+                if (lane == r) mine = m;
+            }
+            int* const top = maxes + (buf * 2 + wg) * 32;
+            if (lane < RW) atomicMax(top + lane, ordered(fmaxf(mrun, mine)));
+            group_sync(wg);
+            if (lane < RW) {
+                const float m = unordered(top[lane]), ref = m == -INFINITY ? 0.f : m;
+                corr_s[(i % 3) * NR + wg * RW + lane] = ex2(mrun - ref);       // the four warps write the same values
+                base_s[wg * RW + lane] = ref - TA_SHIFT;
+                mrun = m;
+            }
+            __syncwarp();
+            unsigned hi[RW / 2], lo[SPLIT ? RW / 2 : 1];
+            const float* c = corr_s + (i % 3) * NR + wg * RW;
+#pragma unroll
+            for (int r = 0; r < RW; r += 2) {
+                const float a = ex2(x[r] - base_s[wg * RW + r]), b = ex2(x[r + 1] - base_s[wg * RW + r + 1]);
+                l[r] = fmaf(l[r], c[r], a); l[r + 1] = fmaf(l[r + 1], c[r + 1], b);
+                hi[r / 2] = Ta16<T>::pack(a, b);
+                if constexpr (SPLIT) { const float2 h = Ta16<T>::unpack(hi[r / 2]); lo[r / 2] = Ta16<T>::pack(a - h.x, b - h.y); }
+            }
+            if (i > 0) collect(i - 1);                               // frees O^T and P
+            unsigned char* const prow = smem + L::P + key * 128;
+#pragma unroll
+            for (int k = 0; k < RW / 8; k++) {
+                const int ch = wg * (RW / 8) + k, cl = ch + NR / 8;       // 16-byte pieces of the high and the low columns
+                *reinterpret_cast<uint4*>(prow + ((ch ^ (key & 7)) << 4)) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+                if constexpr (SPLIT)
+                    *reinterpret_cast<uint4*>(prow + (cl >> 3) * L::BOX + (((cl & 7) ^ (key & 7)) << 4)) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+            }
+            if (masked) {
+                // V elements that are not finite leave the product and go to the rows that see their slot
+                const int j0 = (tile0 + i) * TC_KEYS, from = max(cached - j0, 0), to = min(TC_KEYS, p.cached + p.rows - j0);
+                ok = ok && mbar_wait_warp(vfull + 8 * (i % VS), (unsigned)(i / VS) & 1u, abort_flag, p.status, 54);
+                unsigned char* const v = smem + L::VR + (i % VS) * L::SLOT + (d >> 6) * L::BOX + (d & 7) * 2;
+                bool any = false;
+                for (int k = from; k < to; k++) {
+                    const unsigned short raw = *reinterpret_cast<const unsigned short*>(v + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4));
+                    if ((raw & Ta16<T>::EXP) != Ta16<T>::EXP) continue;
+                    any = true;
+                    unsigned long long rows = 0;
+                    for (int r = 0; r < OR; r++) {
+                        const int pr = r0 + orow + r;
+                        if (pr < p.prows && j0 + k - cached < p.rows && tc_walk(p.parents, pr / p.group, j0 + k - cached)) rows |= 1ull << r;
+                    }
+                    const float bad = Ta16<T>::unpack(raw).x;
+#pragma unroll
+                    for (int r = 0; r < OR; r++) if ((rows >> r) & 1ull) acc[r] += bad;
+                }
+                if (L::MT == 1) groups_sync();              // both groups have looked at the elements that one of them clears
+                if (any && (L::MT == 2 || wg == 0))
+                    for (int k = from; k < to; k++) {
+                        unsigned short* e = reinterpret_cast<unsigned short*>(v + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4));
+                        if ((*e & Ta16<T>::EXP) == Ta16<T>::EXP) *e = 0;
+                    }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && ok) mbar_arrive(pfull);
+        }
+        if (n > 0) collect(n - 1);
+        // ---- the sums of the slots' threads, and the rows' maxima
+        float* const sums = reinterpret_cast<float*>(smem + L::P);             // [8][RW]; every product is done
+        float2* const ml = reinterpret_cast<float2*>(smem + L::P + 4096);      // [NR]
+#pragma unroll
+        for (int r = 0; r < RW; r++) {
+            float s = l[r];
+#pragma unroll
+            for (int k = 16; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+            if (lane == r) sums[warp * RW + r] = s;
+        }
+        group_sync(wg);
+        if (quad == 0 && lane < RW) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) s += sums[(wg * 4 + k) * RW + lane];
+            ml[wg * RW + lane] = make_float2(mrun, ok && !*abort_flag ? s : NAN);
+        }
+        groups_sync();
+        const bool bad = *abort_flag != 0;
+#pragma unroll
+        for (int r = 0; r < OR; r++) {
+            const int row = r0 + orow + r;
+            if (row >= p.prows) continue;
+            const float2 e = ml[orow + r];
+            const float sum = bad ? NAN : e.y;
+            if (p.splits > 1) {
+                const size_t at = ((size_t)split * p.kv_heads + g) * p.pad_rows + row;
+                if (d == 0) p.part_ml[at] = make_float2(e.x == -INFINITY ? -INFINITY : e.x - TA_SHIFT, sum);
+                if (e.x == -INFINITY && sum == 0.f) continue;          // nothing seen: not read either
+                __stcg(p.part_o + at * HD + d, acc[r]);
+            } else {
+                const int t = row / p.group, h = g * p.group + row % p.group;
+                if (p.stats && d == 0) p.stats[(size_t)g * p.pad_rows + row] = make_float2(e.x == -INFINITY ? 0.f : e.x - TA_SHIFT, sum);
+                if (d >= p.dim) continue;
+                float v = acc[r] * (sum == 0.f ? 0.f : 1.f / sum);
+                if (p.gate) v /= 1.f + __expf(-to_f32(((const TA*)p.gate)[t * p.g_row + h * p.g_head + d]));
+                ((TA*)p.out)[t * p.o_row + h * p.o_head + d] = from_f32<TA>(v);
+            }
+        }
+    } else {
+        warp_regs_dec<TC_OTHER_REGS>();
+        if (warp == 8) {
+            // ---------------- copies
+            if (lane == 0) {
+                int kn = min(n, KS), vn = min(n, min(KS, VS)); bool ok = true;        // tiles asked for so far
+                for (int i = 0; ok && i < n; i++) {
+                    if (i >= kn) {
+                        ok = mbar_wait(kempty + 8 * (i % KS), ((unsigned)(i / KS) & 1u) ^ 1u, abort_flag, p.status, 55);
+                        if (!ok) break;
+                        load(false, i); kn = i + 1;
+                    }
+                    if (i >= vn) {
+                        ok = mbar_wait(vempty + 8 * (i % VS), ((unsigned)(i / VS) & 1u) ^ 1u, abort_flag, p.status, 56);
+                        if (!ok) break;
+                        load(true, i); vn = i + 1;
+                    }
+                }
+                if (*abort_flag) {                  // leave only after every copy has landed (bounded)
+                    for (int i = kn > KS ? kn - KS : 0; i < kn; i++) { const long long t0 = clock64(); while (!mbar_test(kfull + 8 * (i % KS), (unsigned)(i / KS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
+                    for (int i = vn > VS ? vn - VS : 0; i < vn; i++) { const long long t0 = clock64(); while (!mbar_test(vfull + 8 * (i % VS), (unsigned)(i / VS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
+                }
+            }
+        } else if (warp == 9) {
+            // ---------------- products: the scores of tile si, O^T of tile oi, whichever has its inputs
+            if (elect_one()) {
+                const unsigned long long qd = desc_k(smem_u32(smem + L::Q)), pd = desc_mn(smem_u32(smem + L::P), L::BOX);
+                int si = 0, oi = 0; long long since = clock64();
+                while (oi < n) {
+                    if (si < n && mbar_poll(kfull + 8 * (si % KS), (unsigned)(si / KS) & 1u) && mbar_poll(sfree + 8 * (si & 1), ((unsigned)(si >> 1) & 1u) ^ 1u)) {
+                        fence_after();
+                        const unsigned long long kd = desc_k(kring + (si % KS) * L::SLOT);
+#pragma unroll
+                        for (int k = 0; k < 4 * NB; k++)             // 16 elements of the head a step
+                            mma_f16(tmem + (si & 1) * NC, kd + (unsigned)(((k >> 2) * L::BOX + (k & 3) * 32) >> 4), qd + (unsigned)(((k >> 2) * NC * 128 + (k & 3) * 32) >> 4), idesc<T>(NC, false), k > 0);
+                        commit_to(sfull + 8 * (si & 1)); commit_to(kempty + 8 * (si % KS));
+                        si++; since = clock64();
+                    } else if (oi < si && mbar_poll(pfull, (unsigned)oi & 1u) && mbar_poll(vfull + 8 * (oi % VS), (unsigned)(oi / VS) & 1u)) {
+                        fence_after();
+#pragma unroll
+                        for (int m = 0; m < L::MT; m++) {
+                            const unsigned long long vd = desc_mn(vring + (oi % VS) * L::SLOT + m * 2 * L::BOX, L::BOX);
+#pragma unroll
+                            for (int k = 0; k < TC_KEYS / 16; k++)   // 16 slots a step
+                                mma_f16(otm + m * NC, vd + (unsigned)(k * 2048 >> 4), pd + (unsigned)(k * 2048 >> 4), idesc<T>(NC, true), k > 0);
+                        }
+                        commit_to(ofull); commit_to(vempty + 8 * (oi % VS));
+                        oi++; since = clock64();
+                    } else if (*abort_flag) break;
+                    else if (clock64() - since > WAIT_CLOCKS) { if (!*abort_flag) atomicExch(p.status, 57); *abort_flag = 1; break; }
+                }
+                // the last commits must find the CTA's shared memory still its own (bounded)
+                if (si > 0) { const long long t0 = clock64(); while (!mbar_test(kempty + 8 * ((si - 1) % KS), (unsigned)((si - 1) / KS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
+                if (oi > 0) { const long long t0 = clock64(); while (!mbar_test(vempty + 8 * ((oi - 1) % VS), (unsigned)((oi - 1) / VS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
+            }
+        }
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((unsigned)L::ALLOC) : "memory");
+    }
+}
+
+// ---- received weight --------------------------------------------------------------------------------------------------------
+// The scores of a 128-slot tile once more, against the finished maximum and sum of every product row: a thread has a slot and adds up its columns, so that nothing crosses
+// threads but the two groups' halves.  The CTA walks the product rows, NR at a time; the next ones are brought in while the last ones' exponentials are formed.
+template <bool SPLIT, int NB, int NR> struct TcWeights {
+    using A = TcTree<SPLIT, NB, NR>;
+    static constexpr int Q = 0, K = A::QB, ANC = K + A::SLOT, JUMP = ANC + TA_MAXROWS * TA_WORDS * 4, ROW = JUMP + TA_MAXROWS * 4, HALF = ROW + 3 * 3 * NR * 4, BARS = HALF + TC_KEYS * 4, TMEM = BARS + 32, FLAG = TMEM + 16,
+                         TOTAL = FLAG + 16;
+    static constexpr int ALLOC = 2 * A::NC < 32 ? 32 : 2 * A::NC;
+};
+template <class T, bool SPLIT, int NB, int NR>
+__global__ void __launch_bounds__(TC_SOFT)
+k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ TaParams p) {
+    using L = TcTree<SPLIT, NB, NR>;
+    using W = TcWeights<SPLIT, NB, NR>;
+    constexpr int NC = L::NC, RW = L::RW;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tile = blockIdx.x, g = blockIdx.y;
+    const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
+    const int cached = ta_cached(p), total = cached + p.rows;
+    if (tile * TC_KEYS >= total) { asm volatile("griddepcontrol.wait;" ::: "memory"); return; }
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + W::FLAG);
+    unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + W::TMEM);
+    const unsigned kfull = smem_u32(smem + W::BARS), sfull = kfull + 8;
+    unsigned (*anc)[TA_WORDS] = reinterpret_cast<unsigned (*)[TA_WORDS]>(smem + W::ANC);
+    float* const row = reinterpret_cast<float*>(smem + W::ROW);       // [3][factor, base, 1 / sum][NR]: a slow warp may still read step i - 1 while a fast one brings i + 1
+    if (tid == 0) {
+        *abort_flag = 0; mbar_init(kfull, 1); mbar_init(sfull, 1); mbar_init(sfull + 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        mbar_expect_tx(kfull, L::SLOT);
+#pragma unroll
+        for (int b = 0; b < NB; b++) tma_load_3d(smem_u32(smem + W::K) + b * L::BOX, &kmap, 64 * b, tile * TC_KEYS, g, kfull);
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)W::ALLOC) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    const bool masked = (tile + 1) * TC_KEYS > cached;
+    if (masked && p.parents) ta_ancestors(anc, reinterpret_cast<int*>(smem + W::JUMP), p.parents, p.rows);
+    asm volatile("griddepcontrol.wait;" ::: "memory");                // the statistics come from the kernel before
+    const int steps = (p.prows + NR - 1) / NR;
+    auto bring = [&](int i) {                                         // product rows of step i, and their statistics
+        float* const rw = row + (i % 3) * 3 * NR;
+        tc_load_q<T, SPLIT, NB, NR>(p, smem + W::Q, rw, g, i * NR, warp, TC_SOFT / 32, lane);
+        if (tid < NR) {
+            const int r = i * NR + tid;
+            const float2 st = r < p.prows ? __ldcg(&p.stats[(size_t)g * p.pad_rows + r]) : make_float2(0.f, 0.f);
+            rw[NR + tid] = st.x; rw[2 * NR + tid] = st.y == 0.f ? 0.f : 1.f / st.y;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    };
+    bring(0);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const unsigned tmem = *tmem_slot;
+    const unsigned long long qd = desc_k(smem_u32(smem + W::Q)), kd = desc_k(smem_u32(smem + W::K));
+    auto issue = [&](int i) {
+        if (warp == 0 && elect_one()) {
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < 4 * NB; k++)
+                mma_f16(tmem + (i & 1) * NC, kd + (unsigned)(((k >> 2) * L::BOX + (k & 3) * 32) >> 4), qd + (unsigned)(((k >> 2) * NC * 128 + (k & 3) * 32) >> 4), idesc<T>(NC, false), k > 0);
+            commit_to(sfull + 8 * (i & 1));
+        }
+        __syncwarp();
+    };
+    bool ok = mbar_wait_warp(kfull, 0, abort_flag, p.status, 61);
+    issue(0);
+    float sum = 0.f;
+    for (int i = 0; i < steps; i++) {
+        ok = ok && mbar_wait_warp(sfull + 8 * (i & 1), (unsigned)(i >> 1) & 1u, abort_flag, p.status, 62);
+        fence_after();
+        if (i + 1 < steps) {                                          // the products of step i are done with Q
+            bring(i + 1);
+            fence_before();
+            __syncthreads();
+            issue(i + 1);
+        }
+        float x[RW];
+        const unsigned sa = tmem + ((unsigned)(quad * 32) << 16) + (i & 1) * NC + wg * RW;
+        tm_ld(x, sa);
+        if constexpr (SPLIT) {
+            float y[RW];
+            tm_ld(y, sa + NR);
+            tm_wait(x);
+#pragma unroll
+            for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
+        } else tm_wait(x);
+        fence_before();
+        const float* const rw = row + (i % 3) * 3 * NR + wg * RW;
+#pragma unroll
+        for (int r = 0; r < RW; r++) {
+            const int pr = i * NR + wg * RW + r;
+            if (pr >= p.prows || (masked && !ta_sees(p, anc, pr / p.group, tile * TC_KEYS + key, cached))) continue;
+            sum += ex2(fmaf(x[r], rw[r], -rw[NR + r])) * rw[2 * NR + r];
+        }
+    }
+    float* const half = reinterpret_cast<float*>(smem + W::HALF);
+    if (wg == 1) half[key] = sum;
+    fence_before();
+    __syncthreads();
+    if (wg == 0 && tile * TC_KEYS + key < total) {
+        float* w = p.weights + (long long)g * p.w_head + tile * TC_KEYS + key;
+        *w = ok && !*abort_flag ? *w + (sum + half[key]) : NAN;
+    }
+    if (warp == 0) {
+        if (!ok && lane == 0) {                                       // leave only after the copy has landed (bounded)
+            const long long t0 = clock64();
+            while (!mbar_test(kfull, 0) && clock64() - t0 < WAIT_CLOCKS) { }
+        }
+        __syncwarp();
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((unsigned)W::ALLOC) : "memory");
+    }
+}
+
+template <class T, bool SPLIT, int NB, int NR> int prepare_shape() {
+    IT_CUDA(cudaFuncSetAttribute(k_tree_attention_tc<T, SPLIT, NB, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcTree<SPLIT, NB, NR>::TOTAL));
+    // setmaxnreg deals out the registers of the launch: a kernel compiled to fewer would wait for ever
+    cudaFuncAttributes at;
+    IT_CUDA(cudaFuncGetAttributes(&at, k_tree_attention_tc<T, SPLIT, NB, NR>));
+    if (at.numRegs * TC_THREADS < TC_SOFT_REGS * TC_SOFT + TC_OTHER_REGS * (TC_THREADS - TC_SOFT)) return it_fail(IT_ESTATE, "it_tree_attention: built with %d registers a thread", at.numRegs);
+    IT_CUDA(cudaFuncSetAttribute(k_tree_weights_tc<T, SPLIT, NB, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcWeights<SPLIT, NB, NR>::TOTAL));
+    return IT_OK;
+}
+template <class T, bool SPLIT, int NB> int prepare_dim() {
+    if (const int r = prepare_shape<T, SPLIT, NB, 16>()) return r;
+    if (const int r = prepare_shape<T, SPLIT, NB, 32>()) return r;
+    return prepare_shape<T, SPLIT, NB, 64>();
+}
+template <class T, bool SPLIT> int prepare_type() { const int r = prepare_dim<T, SPLIT, 2>(); return r ? r : prepare_dim<T, SPLIT, 4>(); }
+
+template <class T, bool SPLIT, int NB, int NR> int run_shape(const TaParams& p, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+    IT_CUDA(ta_launch(false, k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TC_THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, km, vm, p));
+    return IT_OK;
+}
+template <class T, bool SPLIT, int NB, int NR> int weigh_shape(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
+    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((p.cached + p.rows + TC_KEYS - 1) / TC_KEYS, p.kv_heads), dim3(TC_SOFT), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
+    return IT_OK;
+}
+template <class T, bool SPLIT, int NB> int run_dim(const TaParams& p, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+    return nr == 16 ? run_shape<T, SPLIT, NB, 16>(p, row_tiles, km, vm, st) : nr == 32 ? run_shape<T, SPLIT, NB, 32>(p, row_tiles, km, vm, st) : run_shape<T, SPLIT, NB, 64>(p, row_tiles, km, vm, st);
+}
+template <class T, bool SPLIT, int NB> int weigh_dim(const TaParams& p, int nr, const CUtensorMap& km, cudaStream_t st) {
+    return nr == 16 ? weigh_shape<T, SPLIT, NB, 16>(p, km, st) : nr == 32 ? weigh_shape<T, SPLIT, NB, 32>(p, km, st) : weigh_shape<T, SPLIT, NB, 64>(p, km, st);
+}
+
+}  // namespace
+
+int it_tree_tc_prepare() {
+    if (const int r = prepare_type<__half, true>()) return r;
+    if (const int r = prepare_type<__half, false>()) return r;
+    return prepare_type<__nv_bfloat16, false>();
+}
+int it_tree_tc_run(const TaParams& p, int type, int nb, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+    if (type == IT_F32) return nb <= 2 ? run_dim<__half, true, 2>(p, nr, row_tiles, km, vm, st) : run_dim<__half, true, 4>(p, nr, row_tiles, km, vm, st);
+    if (type == IT_F16) return nb <= 2 ? run_dim<__half, false, 2>(p, nr, row_tiles, km, vm, st) : run_dim<__half, false, 4>(p, nr, row_tiles, km, vm, st);
+    return nb <= 2 ? run_dim<__nv_bfloat16, false, 2>(p, nr, row_tiles, km, vm, st) : run_dim<__nv_bfloat16, false, 4>(p, nr, row_tiles, km, vm, st);
+}
+int it_tree_tc_weigh(const TaParams& p, int type, int nb, int nr, const CUtensorMap& km, cudaStream_t st) {
+    if (type == IT_F32) return nb <= 2 ? weigh_dim<__half, true, 2>(p, nr, km, st) : weigh_dim<__half, true, 4>(p, nr, km, st);
+    if (type == IT_F16) return nb <= 2 ? weigh_dim<__half, false, 2>(p, nr, km, st) : weigh_dim<__half, false, 4>(p, nr, km, st);
+    return nb <= 2 ? weigh_dim<__nv_bfloat16, false, 2>(p, nr, km, st) : weigh_dim<__nv_bfloat16, false, 4>(p, nr, km, st);
+}
