@@ -1,5 +1,4 @@
-// Tree attention on the 5th-generation tensor cores (tcgen05.mma kind::f16, accumulators in tensor memory): the same function as the mma.sync kernel of
-// it_tree_attention.cu, for any number of product rows.
+// The products of tree attention (it_tree_attention.cu) on the 5th-generation tensor cores: tcgen05.mma kind::f16, accumulators in tensor memory.
 //
 // Both products are formed with the cache as the first operand, whose 128 rows are always full, and the product rows (row t * group + head) as columns, of which there are
 // as few as 16:   S^T [128 slots x columns] = K [slots x d] . Q^T,    O^T [d x columns] = V^T [d x slots] . P^T
@@ -7,29 +6,30 @@
 //   K and V tiles   128 slots as boxes of 64 elements of a tensor map, 128-byte swizzle: K is read K-major, V (as V^T) MN-major
 //   Q               rows of 128-byte pieces, K-major; f32 activations as two sets of columns, high and low halves, added in f32 when they are read
 //   P               [slot][column], MN-major: a thread has one slot (a lane of tensor memory) and stores its columns as 16-byte pieces
-// Warps 0-7 (two groups of four; a group has half of the columns): scores out of tensor memory, running maximum (redux over the slots of a warp, an ordered atomicMax over the four warps),
-// exponentials, P; then the tile before: O^T out of tensor memory into f32 accumulators in registers.  Every tile's product starts from zero and is
-// added with a rounded f32 addition: chained over a long run in tensor memory the hardware's truncating accumulation loses f32's last bits (1.3e-5 of the result after 120 tiles
-// with the mma.sync kernel).  Warp 8: copies.  Warp 9: issues whichever product has its inputs, the next tile's scores or this tile's O.
+// Warps 0-7 (two groups of four; a group has half of the columns): scores out of tensor memory, exponentials against a reference that moves only when
+// it has to (redux over the slots of a warp, an ordered atomicMax over the four), P; then the tile before: O^T out of tensor memory into f32 accumulators in registers.  Every tile's product starts from zero and is
+// added with a rounded f32 addition: chained over a long run in tensor memory the hardware's truncating accumulation loses f32's last bits (1.3e-5 of the result after 240 tiles of 64
+// slots chained in mma.sync accumulators).  Warps 8 and 10: copies.  Warp 9: issues whichever product has its inputs, the next tile's scores or this tile's O.
 // What bounds it: 64 columns of f32 activations (128 with the low halves) 2 x 1024 tensor cycles a tile of 128 slots at head dimension 256; few columns: HBM.
 #include "it_tree_attention.cuh"
 
 namespace {
 
-constexpr int TC_KEYS = 128, TC_THREADS = 384, TC_SOFT = 256;
+constexpr int TC_THREADS = 384, TC_SOFT = 256;
 constexpr int TC_SMEM_LIMIT = 227 * 1024, TC_SMALL = 3072, TC_SLOTS_MAX = 6;
 constexpr int TC_SOFT_REGS = 216, TC_OTHER_REGS = 72;       // 216 x 256 + 72 x 128 = 64,512 = 168 x 384
+constexpr float TC_SHIFT = 6.f, TC_TOP = 15.f;              // p is 2^6 at the reference and may grow to 2^15 before the reference moves
 
 template <bool SPLIT, int NB, int NR> struct TcTree {
     static constexpr int NC = NR * (SPLIT ? 2 : 1), NCB = NC > 64 ? 2 : 1, RW = NR / 2;       // columns of a product, 64-column blocks of P, product rows of a warp group
     static constexpr int HD = 64 * NB, MT = NB / 2;                                           // M tiles of O^T
     static constexpr int OR = MT == 2 ? NR : RW;                                              // accumulators of a thread: one element of d, this many product rows
-    static constexpr int QB = NB * NC * 128, PB = NCB * TC_KEYS * 128, SLOT = NB * TC_KEYS * 128, BOX = TC_KEYS * 128;
+    static constexpr int QB = NB * NC * 128, PB = NCB * TA_KEYS * 128, SLOT = NB * TA_KEYS * 128, BOX = TA_KEYS * 128;
     static constexpr int FIT = (TC_SMEM_LIMIT - TC_SMALL - QB - PB) / SLOT, SLOTS = FIT < TC_SLOTS_MAX ? FIT : TC_SLOTS_MAX;
     static constexpr int KS = (SLOTS + 1) / 2, VS = SLOTS - KS;
     static constexpr int Q = 0, P = QB, KR = P + PB, VR = KR + KS * SLOT, SMALL = VR + VS * SLOT, TOTAL = SMALL + TC_SMALL;
     // offsets from SMALL
-    static constexpr int BARS = 0, TMEM = 256, FLAG = 272, MAXES = 512, BASE = 1024, CORR = 1280, FAC = 2048;
+    static constexpr int BARS = 0, TMEM = 256, FLAG = 272, MAXES = 512, BASE = 1024, CORR = 1280, FAC = 2048, TROW = 2304;
     static constexpr int TCOLS = 2 * NC + MT * NC, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
     static_assert(VS >= 1 && NR % 16 == 0 && NC <= 128 && NR <= 64 && NC % 16 == 0, "");
     static_assert(PB >= TA_MAXROWS * TA_WORDS * 4 + TA_MAXROWS * 4, "the ancestors are worked out in P's place");
@@ -90,23 +90,43 @@ template <int N> __device__ __forceinline__ void warp_regs_dec() { asm volatile(
 __device__ __forceinline__ void group_sync(int wg) {
     if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
 }
+// Whether any thread of a group says so, with a barrier of the group.
+__device__ __forceinline__ bool group_any(int wg, bool q) {
+    unsigned r;
+    if (wg == 0) asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbarrier.cta.red.or.pred p, 1, 128, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r) : "r"(q ? 1u : 0u) : "memory");
+    else asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbarrier.cta.red.or.pred p, 2, 128, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r) : "r"(q ? 1u : 0u) : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
 
-// Product rows [r0, r0 + NR) of KV head g as columns of Q^T, and for each the factor from the product to log2 of its exponential.
-template <class T, bool SPLIT, int NB, int NR>
-__device__ void tc_load_q(const TaParams& p, unsigned char* q, float* fac, int g, int r0, int warp, int nw, int lane) {
+// Product rows [r0, r0 + NR) of KV head g as columns of Q^T; for each the factor from the product to log2 of its exponential, and its row t (rows behind the last: the
+// last one's).  A warp has all of its rows' loads under way at once: one after the other they were 7 us of a 64-row tile.
+template <class T, bool SPLIT, int NB, int NR, int NW>
+__device__ void tc_load_q(const TaParams& p, unsigned char* q, float* fac, int* trow, int g, int r0, int warp, int lane) {
     using L = TcTree<SPLIT, NB, NR>;
-    for (int i = warp; i < NR; i += nw) {
-        const int r = r0 + i, t = r / p.group, h = g * p.group + r % p.group;
-        const bool live = r < p.prows && 8 * lane < p.dim;
-        unsigned hi[4] = {}, lo[4] = {};
-        const float f = ta_q_row<T, SPLIT>(p, live, t, h, lane, hi, lo);
+    constexpr int N = NR < 3 * NW ? (NR + NW - 1) / NW : 3;
+    TaRow<T, SPLIT> x[N];
+#pragma unroll 1
+    for (int i0 = warp; i0 < NR; i0 += N * NW) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int i = i0 + k * NW, r = r0 + i, t = min(ta_row(p, r), p.rows - 1), h = g * p.group + r - t * p.group;
+        if (i < NR && lane == 0) trow[i] = t;
+        x[k].load(p, i < NR && r < p.prows && 8 * lane < p.dim, t, h, lane);
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int i = i0 + k * NW;
+        if (i >= NR) break;
+        unsigned hi[4], lo[4];
+        const float f = x[k].halves(p, hi, lo);
         if (lane < NB * 8) {
             const unsigned at = (unsigned)((lane >> 3) * L::NC * 128) + swz(i, lane & 7);
             *reinterpret_cast<uint4*>(q + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             if constexpr (SPLIT) *reinterpret_cast<uint4*>(q + at + NR * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         if (lane == 0) fac[i] = f;
+    }
     }
 }
 
@@ -134,63 +154,44 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     float* base_s = reinterpret_cast<float*>(small + L::BASE);          // [NR]
     float* corr_s = reinterpret_cast<float*>(small + L::CORR);          // [3][NR]
     float* fac = reinterpret_cast<float*>(small + L::FAC);              // [NR]
+    int* trow = reinterpret_cast<int*>(small + L::TROW);                // [NR]
     const unsigned bars = smem_u32(small + L::BARS);
     const unsigned kfull = bars, kempty = kfull + 8 * KS, vfull = kempty + 8 * KS, vempty = vfull + 8 * VS, sfull = vempty + 8 * VS, sfree = sfull + 16, pfull = sfree + 16, ofull = pfull + 8;
     const unsigned kring = smem_u32(smem + L::KR), vring = smem_u32(smem + L::VR);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TC_KEYS - 1) / TC_KEYS;
+    const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TA_KEYS - 1) / TA_KEYS;
     const int tile0 = (int)((long long)split * tiles / p.splits), n = (int)((long long)(split + 1) * tiles / p.splits) - tile0;
-    if (tid == 0) {
+    // Tile i of K (v = 0) or V, when its slot is free; copies of K and V have a warp each, since they wait for different products.
+    auto load = [&](int v, int i) {
+        const int s = i % (v ? VS : KS);
+        const unsigned dst = (v ? vring : kring) + s * L::SLOT, bar = (v ? vfull : kfull) + 8 * s;
+        mbar_expect_tx(bar, L::SLOT);
+#pragma unroll
+        for (int b = 0; b < NB; b++) tma_load_3d(dst + b * L::BOX, v ? &vmap : &kmap, 64 * b, (tile0 + i) * TA_KEYS, g, bar);
+    };
+    if (warp == 8 && lane == 0) {
         *abort_flag = (smem_u32(smem) & 1023u) != 0;                 // the swizzle counts on it; never seen
         for (int s = 0; s < KS; s++) { mbar_init(kfull + 8 * s, 1); mbar_init(kempty + 8 * s, 1); }
         for (int s = 0; s < VS; s++) { mbar_init(vfull + 8 * s, 1); mbar_init(vempty + 8 * s, 1); }
         for (int s = 0; s < 2; s++) { mbar_init(sfull + 8 * s, 1); mbar_init(sfree + 8 * s, 8); }
         mbar_init(pfull, 8); mbar_init(ofull, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+#pragma unroll 1
+        for (int i = 0; i < 2 * min(n, KS); i++) if (!(i & 1) || i / 2 < VS) load(i & 1, i >> 1);        // the first tiles before anything else
     }
-    if (tid >= 128 && tid < 256) maxes[tid - 128] = ordered(-INFINITY);
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)L::ALLOC) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (tid < 128) maxes[tid] = ordered(-INFINITY);
+    __syncwarp();
+    tc_load_q<T, SPLIT, NB, NR, TC_THREADS / 32>(p, smem + L::Q, fac, trow, g, r0, warp, lane);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // Q before the products read it
     fence_before();
     __syncthreads();
     fence_after();
     const unsigned tmem = *tmem_slot, otm = tmem + 2 * NC;
-    auto load = [&](bool v, int i) {                // tile i of K or V; the slot is free
-        const int s = v ? i % VS : i % KS;
-        const unsigned dst = (v ? vring : kring) + s * L::SLOT, bar = (v ? vfull : kfull) + 8 * s;
-        mbar_expect_tx(bar, L::SLOT);
-#pragma unroll
-        for (int b = 0; b < NB; b++) tma_load_3d(dst + b * L::BOX, v ? &vmap : &kmap, 64 * b, (tile0 + i) * TC_KEYS, g, bar);
-    };
-    if (warp == 8 && lane == 0) {                   // the first tiles before anything else
-        for (int i = 0; i < n && i < KS; i++) { load(false, i); if (i < VS) load(true, i); }
-    }
-    __syncwarp();
-    tc_load_q<T, SPLIT, NB, NR>(p, smem + L::Q, fac, g, r0, warp, TC_THREADS / 32, lane);
-    const int first_masked = cached / TC_KEYS - tile0;             // tiles from here on reach behind the cached slots
-    unsigned vis[3] = { 0, 0, 0 };                                 // which of the group's product rows see this thread's slot of the first, second, third such tile
-    if (n > first_masked && n > 0) {
-        unsigned (*anc)[TA_WORDS] = reinterpret_cast<unsigned (*)[TA_WORDS]>(smem + L::P);
-        if (p.parents) ta_ancestors(anc, reinterpret_cast<int*>(smem + L::P + TA_MAXROWS * TA_WORDS * 4), p.parents, p.rows);
-        __syncthreads();
-        if (warp < 8) {
-            const int wg = warp >> 2, key = tid & 127;
-            for (int k = 0; k < 3; k++) {
-                unsigned m = 0;
-                const int j = (tile0 + first_masked + k) * TC_KEYS + key;
-                for (int r = 0; r < RW; r++) {
-                    const int t = min((r0 + wg * RW + r) / p.group, p.rows - 1);
-                    if (ta_sees(p, anc, t, j, cached)) m |= 1u << r;
-                }
-                if (k == 0) vis[0] = m; else if (k == 1) vis[1] = m; else vis[2] = m;
-            }
-        }
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // Q before the products read it
-    __syncthreads();
 
     if (warp < 8) {
         warp_regs_inc<TC_SOFT_REGS>();
@@ -204,33 +205,38 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
         for (int r = 0; r < RW; r++) l[r] = 0.f;
         bool ok = true;
-        auto collect = [&](int i) {                                 // O^T of tile i
-            ok = ok && mbar_wait_warp(ofull, (unsigned)i & 1u, abort_flag, p.status, 52);
-            ok = ok && mbar_wait_warp(pfull, (unsigned)i & 1u, abort_flag, p.status, 53);      // met long ago: the other group's factors are seen through it
-            fence_after();
-            const float* c = corr_s + (i % 3) * NR + orow;
-            constexpr int CH = OR < 16 ? OR : 16;
+        // Which of the group's product rows see this thread's slot, for the tiles that reach behind the cached slots; while the first scores are formed.
+        const int first_masked = cached / TA_KEYS - tile0;
+        unsigned vis[3] = { 0, 0, 0 };
+        if (n > first_masked && n > 0) {
+            unsigned (*anc)[TA_WORDS] = reinterpret_cast<unsigned (*)[TA_WORDS]>(smem + L::P);
+            if (p.parents) ta_ancestors<TC_SOFT>(anc, reinterpret_cast<int*>(smem + L::P + TA_MAXROWS * TA_WORDS * 4), p.parents, p.rows, tid, [] { groups_sync(); });
 #pragma unroll
-            for (int r = 0; r < OR; r += CH) {
-                float a[CH], b[CH];
-                tm_ld(a, oaddr + r);
-                if constexpr (SPLIT) tm_ld(b, oaddr + NR + r);
-                tm_wait(a);
-                if constexpr (SPLIT) {
-#pragma unroll
-                    for (int x = 0; x < CH; x++) { asm volatile("" : "+f"(b[x])); a[x] += b[x]; }
+            for (int k = 0; k < 3; k++) {
+                if (first_masked + k >= n) break;
+                const int i = (tile0 + first_masked + k) * TA_KEYS + key - cached;           // the slot among the rows' own
+                unsigned m = i < 0 ? 0xffffffffu : 0u;
+                if (i >= 0 && i < p.rows) {
+#pragma unroll 4
+                    for (int r = 0; r < RW; r++) {
+                        const int t = trow[wg * RW + r];
+                        if (p.parents ? (anc[t][i >> 5] >> (i & 31)) & 1u : i <= t) m |= 1u << r;
+                    }
                 }
-#pragma unroll
-                for (int x = 0; x < CH; x++) acc[r + x] = fmaf(acc[r + x], c[r + x], a[x]);
+                vis[k] = m;
             }
-            fence_before();
-        };
-        for (int i = 0; i < n; i++) {
-            const int buf = i & 1;
-            ok = ok && mbar_wait_warp(sfull + 8 * buf, (unsigned)(i >> 1) & 1u, abort_flag, p.status, 51);
-            fence_after();
-            float x[RW];
-            {
+            groups_sync();                                          // before P takes the place of the ancestors
+        }
+        int exact = 0;                                              // references moved so far
+#pragma unroll 1
+        for (int i = 0; i <= n; i++) {                              // softmax of tile i, O^T of tile i - 1, P of tile i
+            unsigned hi[RW / 2], lo[SPLIT ? RW / 2 : 1];
+            const bool masked = i >= first_masked;
+            if (i < n) {
+                const int buf = i & 1;
+                ok = ok && mbar_wait_warp(sfull + 8 * buf, (unsigned)(i >> 1) & 1u, abort_flag, p.status, 51);
+                fence_after();
+                float x[RW];
                 const unsigned sa = tmem + lanes + buf * NC + wg * RW;
                 tm_ld(x, sa);
                 if constexpr (SPLIT) {
@@ -240,40 +246,79 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
                     for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
                 } else tm_wait(x);
-            }
-            fence_before();
-            __syncwarp();
-            if (lane == 0 && ok) mbar_arrive(sfree + 8 * buf);
-            const bool masked = i >= first_masked;
-            const unsigned see = masked ? (i == first_masked ? vis[0] : i == first_masked + 1 ? vis[1] : vis[2]) : 0xffffffffu;
-            float mine = -INFINITY;
+                fence_before();
+                __syncwarp();
+                if (lane == 0 && ok) mbar_arrive(sfree + 8 * buf);
+                // Exponents against the rows' references.  A reference need not be the maximum: it moves when an exponent would pass f16's range, in the first tile, and in
+                // masked tiles (a row may have seen nothing before), which spares all other tiles the maximum over slots.
+                const float *const f = fac + wg * RW, *const bs = base_s + wg * RW;
+                float* const c = corr_s + (i % 3) * NR + wg * RW;
+                bool move = i == 0 || masked;
+                float y[RW], top = -INFINITY;
+                if (!move) {
 #pragma unroll
-            for (int r = 0; r < RW; r++) {
-                x[r] *= fac[wg * RW + r];
-                if (masked && !((see >> r) & 1u)) x[r] = -INFINITY;
-                const float m = warp_max(x[r]);
-                if (lane == r) mine = m;
-            }
-            int* const top = maxes + (buf * 2 + wg) * 32;
-            if (lane < RW) atomicMax(top + lane, ordered(fmaxf(mrun, mine)));
-            group_sync(wg);
-            if (lane < RW) {
-                const float m = unordered(top[lane]), ref = m == -INFINITY ? 0.f : m;
-                corr_s[(i % 3) * NR + wg * RW + lane] = ex2(mrun - ref);       // the four warps write the same values
-                base_s[wg * RW + lane] = ref - TA_SHIFT;
-                mrun = m;
-            }
-            __syncwarp();
-            unsigned hi[RW / 2], lo[SPLIT ? RW / 2 : 1];
-            const float* c = corr_s + (i % 3) * NR + wg * RW;
+                    for (int r = 0; r < RW; r++) { y[r] = fmaf(x[r], f[r], -bs[r]); top = fmaxf(top, y[r]); }
+                    move = group_any(wg, top > TC_TOP);             // the same answer in all four warps
+                }
+                if (move) {
+                    const unsigned see = masked ? (i == first_masked ? vis[0] : i == first_masked + 1 ? vis[1] : vis[2]) : 0xffffffffu;
+                    float mine = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < RW; r += 2) {
-                const float a = ex2(x[r] - base_s[wg * RW + r]), b = ex2(x[r + 1] - base_s[wg * RW + r + 1]);
-                l[r] = fmaf(l[r], c[r], a); l[r + 1] = fmaf(l[r + 1], c[r + 1], b);
-                hi[r / 2] = Ta16<T>::pack(a, b);
-                if constexpr (SPLIT) { const float2 h = Ta16<T>::unpack(hi[r / 2]); lo[r / 2] = Ta16<T>::pack(a - h.x, b - h.y); }
+                    for (int r = 0; r < RW; r++) {
+                        x[r] *= f[r];
+                        if (!((see >> r) & 1u)) x[r] = -INFINITY;
+                        const float m = warp_max(x[r]);
+                        if (lane == r) mine = m;
+                    }
+                    int* const best = maxes + ((exact & 1) * 2 + wg) * 32;
+                    exact++;
+                    if (lane < RW) atomicMax(best + lane, ordered(fmaxf(mrun, mine)));
+                    group_sync(wg);
+                    if (lane < RW) {                                // the four warps write the same values
+                        const float m = unordered(best[lane]), ref = m == -INFINITY ? 0.f : m;
+                        c[lane] = ex2(mrun - ref);
+                        base_s[wg * RW + lane] = ref - TC_SHIFT;
+                        mrun = m;
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int r = 0; r < RW; r++) { y[r] = x[r] - bs[r]; l[r] *= c[r]; }
+                } else if (lane < RW) c[lane] = 1.f;
+#pragma unroll
+                for (int r = 0; r < RW; r += 2) {
+                    const float a = ex2(y[r]), b = ex2(y[r + 1]);
+                    l[r] += a; l[r + 1] += b;
+                    hi[r / 2] = Ta16<T>::pack(a, b);
+                    if constexpr (SPLIT) { const float2 h = Ta16<T>::unpack(hi[r / 2]); lo[r / 2] = Ta16<T>::pack(a - h.x, b - h.y); }
+                }
             }
-            if (i > 0) collect(i - 1);                               // frees O^T and P
+            if (i > 0) {                                            // O^T of tile i - 1: frees it and P
+                ok = ok && mbar_wait_warp(ofull, (unsigned)(i - 1) & 1u, abort_flag, p.status, 52);
+                ok = ok && mbar_wait_warp(pfull, (unsigned)(i - 1) & 1u, abort_flag, p.status, 53);      // met long ago: the other group's factors are seen through it
+                fence_after();
+                const float* const c = corr_s + ((i - 1) % 3) * NR + orow;
+                constexpr int CH = 8, NCH = OR / CH;
+                float a[2][CH], b[2][CH];
+                tm_ld(a[0], oaddr);
+                if constexpr (SPLIT) tm_ld(b[0], oaddr + NR);
+#pragma unroll
+                for (int k = 0; k < NCH; k++) {                     // the next columns are on their way while these are added
+                    float (&u)[CH] = a[k & 1], (&v)[CH] = b[k & 1];
+                    tm_wait(u);
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int e = 0; e < CH; e++) asm volatile("" : "+f"(v[e]));
+                    }
+                    if (k + 1 < NCH) {
+                        tm_ld(a[(k + 1) & 1], oaddr + (k + 1) * CH);
+                        if constexpr (SPLIT) tm_ld(b[(k + 1) & 1], oaddr + NR + (k + 1) * CH);
+                    }
+#pragma unroll
+                    for (int e = 0; e < CH; e++) acc[k * CH + e] = fmaf(acc[k * CH + e], c[k * CH + e], SPLIT ? u[e] + v[e] : u[e]);
+                }
+                fence_before();
+            }
+            if (i == n) break;
             unsigned char* const prow = smem + L::P + key * 128;
 #pragma unroll
             for (int k = 0; k < RW / 8; k++) {
@@ -284,25 +329,26 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
             if (masked) {
                 // V elements that are not finite leave the product and go to the rows that see their slot
-                const int j0 = (tile0 + i) * TC_KEYS, from = max(cached - j0, 0), to = min(TC_KEYS, p.cached + p.rows - j0);
+                const int j0 = (tile0 + i) * TA_KEYS, from = max(cached - j0, 0), to = min(TA_KEYS, p.cached + p.rows - j0);
                 ok = ok && mbar_wait_warp(vfull + 8 * (i % VS), (unsigned)(i / VS) & 1u, abort_flag, p.status, 54);
                 unsigned char* const v = smem + L::VR + (i % VS) * L::SLOT + (d >> 6) * L::BOX + (d & 7) * 2;
                 bool any = false;
+#pragma unroll 1
                 for (int k = from; k < to; k++) {
                     const unsigned short raw = *reinterpret_cast<const unsigned short*>(v + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4));
                     if ((raw & Ta16<T>::EXP) != Ta16<T>::EXP) continue;
                     any = true;
                     unsigned long long rows = 0;
-                    for (int r = 0; r < OR; r++) {
-                        const int pr = r0 + orow + r;
-                        if (pr < p.prows && j0 + k - cached < p.rows && tc_walk(p.parents, pr / p.group, j0 + k - cached)) rows |= 1ull << r;
-                    }
+#pragma unroll 1
+                    for (int r = 0; r < OR; r++)
+                        if (j0 + k - cached < p.rows && tc_walk(p.parents, trow[orow + r], j0 + k - cached)) rows |= 1ull << r;
                     const float bad = Ta16<T>::unpack(raw).x;
 #pragma unroll
                     for (int r = 0; r < OR; r++) if ((rows >> r) & 1ull) acc[r] += bad;
                 }
                 if (L::MT == 1) groups_sync();              // both groups have looked at the elements that one of them clears
                 if (any && (L::MT == 2 || wg == 0))
+#pragma unroll 1
                     for (int k = from; k < to; k++) {
                         unsigned short* e = reinterpret_cast<unsigned short*>(v + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4));
                         if ((*e & Ta16<T>::EXP) == Ta16<T>::EXP) *e = 0;
@@ -312,68 +358,79 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             __syncwarp();
             if (lane == 0 && ok) mbar_arrive(pfull);
         }
-        if (n > 0) collect(n - 1);
-        // ---- the sums of the slots' threads, and the rows' maxima
-        float* const sums = reinterpret_cast<float*>(smem + L::P);             // [8][RW]; every product is done
-        float2* const ml = reinterpret_cast<float2*>(smem + L::P + 4096);      // [NR]
+        // ---- every product is done: the rings are free.  The rows' sums are those of the slots' threads.
+        float* const sums = reinterpret_cast<float*>(smem + L::KR);            // [NR][128]
+        float2* const ml = reinterpret_cast<float2*>(smem + L::P);             // [NR]
 #pragma unroll
-        for (int r = 0; r < RW; r++) {
-            float s = l[r];
-#pragma unroll
-            for (int k = 16; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-            if (lane == r) sums[warp * RW + r] = s;
-        }
+        for (int r = 0; r < RW; r++) sums[(wg * RW + r) * TA_KEYS + key] = l[r];
         group_sync(wg);
-        if (quad == 0 && lane < RW) {
-            float s = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) s += sums[(wg * 4 + k) * RW + lane];
-            ml[wg * RW + lane] = make_float2(mrun, ok && !*abort_flag ? s : NAN);
-        }
-        groups_sync();
         const bool bad = *abort_flag != 0;
 #pragma unroll
-        for (int r = 0; r < OR; r++) {
-            const int row = r0 + orow + r;
-            if (row >= p.prows) continue;
-            const float2 e = ml[orow + r];
-            const float sum = bad ? NAN : e.y;
-            if (p.splits > 1) {
-                const size_t at = ((size_t)split * p.kv_heads + g) * p.pad_rows + row;
-                if (d == 0) p.part_ml[at] = make_float2(e.x == -INFINITY ? -INFINITY : e.x - TA_SHIFT, sum);
-                if (e.x == -INFINITY && sum == 0.f) continue;          // nothing seen: not read either
-                __stcg(p.part_o + at * HD + d, acc[r]);
-            } else {
-                const int t = row / p.group, h = g * p.group + row % p.group;
-                if (p.stats && d == 0) p.stats[(size_t)g * p.pad_rows + row] = make_float2(e.x == -INFINITY ? 0.f : e.x - TA_SHIFT, sum);
-                if (d >= p.dim) continue;
-                float v = acc[r] * (sum == 0.f ? 0.f : 1.f / sum);
-                if (p.gate) v /= 1.f + __expf(-to_f32(((const TA*)p.gate)[t * p.g_row + h * p.g_head + d]));
-                ((TA*)p.out)[t * p.o_row + h * p.o_head + d] = from_f32<TA>(v);
+        for (int r = 0; r < RW / 4; r++) {
+            const int row = wg * RW + quad + 4 * r;
+            const float4 e = *reinterpret_cast<const float4*>(sums + row * TA_KEYS + 4 * lane);
+            float v = (e.x + e.y) + (e.z + e.w);
+#pragma unroll
+            for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(0xffffffffu, v, k);
+            if (lane == 0) ml[row].y = bad ? NAN : v;
+        }
+        if (quad == 0 && lane < RW) ml[wg * RW + lane].x = mrun == -INFINITY ? mrun : base_s[wg * RW + lane];
+        if (p.splits > 1) {
+            // rows behind the last one are written too: the workspace has room for them
+            const size_t at = ((size_t)split * p.kv_heads + g) * p.pad_rows + r0;
+            float* const o = p.part_o + (at + orow) * HD + d;
+#pragma unroll
+            for (int r = 0; r < OR; r++) __stcg(o + r * HD, acc[r]);
+            groups_sync();
+            if (tid < NR) p.part_ml[at + tid] = ml[tid];
+        } else {
+            // through shared memory, so that a loop can write whole rows, four elements a thread
+            float* const os = reinterpret_cast<float*>(smem + L::KR);          // [NR][HD], where the sums were
+            groups_sync();
+#pragma unroll
+            for (int r = 0; r < OR; r++) os[(orow + r) * HD + d] = acc[r];
+            groups_sync();
+            if (p.stats && tid < NR) p.stats[(size_t)g * p.pad_rows + r0 + tid] = make_float2(ml[tid].x == -INFINITY ? 0.f : ml[tid].x, ml[tid].y);
+            constexpr int LN = HD / 4, STEP = TC_SOFT / LN, U = 4;              // threads of a row, rows at once, rows of a thread whose gates are on their way together
+            const int c = tid % LN * 4;
+#pragma unroll 1
+            for (int q = tid / LN; q < NR && c < p.dim; q += U * STEP) {
+                float z[U][4];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int r = q + u * STEP, row = r0 + r;
+                    if (p.gate && r < NR && row < p.prows) { const int t = trow[r]; load4((const TA*)p.gate + t * p.g_row + (g * p.group + row - t * p.group) * p.g_head + c, z[u]); }
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int r = q + u * STEP, row = r0 + r;
+                    if (r >= NR || row >= p.prows) break;
+                    const int t = trow[r], h = g * p.group + row - t * p.group;
+                    const float sum = ml[r].y, inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const float4 v = *reinterpret_cast<const float4*>(os + r * HD + c);
+                    float o[4] = { v.x * inv, v.y * inv, v.z * inv, v.w * inv };
+                    if (p.gate) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[e] /= 1.f + __expf(-z[u][e]);
+                    }
+                    store4((TA*)p.out + t * p.o_row + h * p.o_head + c, o);
+                }
             }
         }
     } else {
         warp_regs_dec<TC_OTHER_REGS>();
-        if (warp == 8) {
-            // ---------------- copies
+        if (warp == 8 || warp == 10) {
+            // ---------------- copies of K, and of V
             if (lane == 0) {
-                int kn = min(n, KS), vn = min(n, min(KS, VS)); bool ok = true;        // tiles asked for so far
-                for (int i = 0; ok && i < n; i++) {
-                    if (i >= kn) {
-                        ok = mbar_wait(kempty + 8 * (i % KS), ((unsigned)(i / KS) & 1u) ^ 1u, abort_flag, p.status, 55);
-                        if (!ok) break;
-                        load(false, i); kn = i + 1;
-                    }
-                    if (i >= vn) {
-                        ok = mbar_wait(vempty + 8 * (i % VS), ((unsigned)(i / VS) & 1u) ^ 1u, abort_flag, p.status, 56);
-                        if (!ok) break;
-                        load(true, i); vn = i + 1;
-                    }
+                const int v = warp == 10, ring = v ? VS : KS;
+                const unsigned full = v ? vfull : kfull, empty = v ? vempty : kempty;
+                int i = min(n, min(KS, ring));          // asked for already
+                for (; i < n; i++) {
+                    if (i >= ring && !mbar_wait(empty + 8 * (i % ring), ((unsigned)(i / ring) & 1u) ^ 1u, abort_flag, p.status, 55)) break;
+                    load(v, i);
                 }
-                if (*abort_flag) {                  // leave only after every copy has landed (bounded)
-                    for (int i = kn > KS ? kn - KS : 0; i < kn; i++) { const long long t0 = clock64(); while (!mbar_test(kfull + 8 * (i % KS), (unsigned)(i / KS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
-                    for (int i = vn > VS ? vn - VS : 0; i < vn; i++) { const long long t0 = clock64(); while (!mbar_test(vfull + 8 * (i % VS), (unsigned)(i / VS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
-                }
+                if (*abort_flag)                        // leave only after every copy has landed (bounded)
+                    for (int k = i > ring ? i - ring : 0; k < i; k++) { const long long t0 = clock64(); while (!mbar_test(full + 8 * (k % ring), (unsigned)(k / ring) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
             }
         } else if (warp == 9) {
             // ---------------- products: the scores of tile si, O^T of tile oi, whichever has its inputs
@@ -395,7 +452,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                         for (int m = 0; m < L::MT; m++) {
                             const unsigned long long vd = desc_mn(vring + (oi % VS) * L::SLOT + m * 2 * L::BOX, L::BOX);
 #pragma unroll
-                            for (int k = 0; k < TC_KEYS / 16; k++)   // 16 slots a step
+                            for (int k = 0; k < TA_KEYS / 16; k++)   // 16 slots a step
                                 mma_f16(otm + m * NC, vd + (unsigned)(k * 2048 >> 4), pd + (unsigned)(k * 2048 >> 4), idesc<T>(NC, true), k > 0);
                         }
                         commit_to(ofull); commit_to(vempty + 8 * (oi % VS));
@@ -423,7 +480,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 // threads but the two groups' halves.  The CTA walks the product rows, NR at a time; the next ones are brought in while the last ones' exponentials are formed.
 template <bool SPLIT, int NB, int NR> struct TcWeights {
     using A = TcTree<SPLIT, NB, NR>;
-    static constexpr int Q = 0, K = A::QB, ANC = K + A::SLOT, JUMP = ANC + TA_MAXROWS * TA_WORDS * 4, ROW = JUMP + TA_MAXROWS * 4, HALF = ROW + 3 * 3 * NR * 4, BARS = HALF + TC_KEYS * 4, TMEM = BARS + 32, FLAG = TMEM + 16,
+    static constexpr int Q = 0, K = A::QB, ANC = K + A::SLOT, JUMP = ANC + TA_MAXROWS * TA_WORDS * 4, ROW = JUMP + TA_MAXROWS * 4, HALF = ROW + 3 * 4 * NR * 4, BARS = HALF + TA_KEYS * 4, TMEM = BARS + 32, FLAG = TMEM + 16,
                          TOTAL = FLAG + 16;
     static constexpr int ALLOC = 2 * A::NC < 32 ? 32 : 2 * A::NC;
 };
@@ -437,30 +494,30 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tile = blockIdx.x, g = blockIdx.y;
     const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
     const int cached = ta_cached(p), total = cached + p.rows;
-    if (tile * TC_KEYS >= total) { asm volatile("griddepcontrol.wait;" ::: "memory"); return; }
+    if (tile * TA_KEYS >= total) { asm volatile("griddepcontrol.wait;" ::: "memory"); return; }
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + W::FLAG);
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + W::TMEM);
     const unsigned kfull = smem_u32(smem + W::BARS), sfull = kfull + 8;
     unsigned (*anc)[TA_WORDS] = reinterpret_cast<unsigned (*)[TA_WORDS]>(smem + W::ANC);
-    float* const row = reinterpret_cast<float*>(smem + W::ROW);       // [3][factor, base, 1 / sum][NR]: a slow warp may still read step i - 1 while a fast one brings i + 1
+    float* const row = reinterpret_cast<float*>(smem + W::ROW);       // [3][factor, base, 1 / sum, row t][NR]: a slow warp may still read step i - 1 while a fast one brings i + 1
     if (tid == 0) {
         *abort_flag = 0; mbar_init(kfull, 1); mbar_init(sfull, 1); mbar_init(sfull + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         mbar_expect_tx(kfull, L::SLOT);
 #pragma unroll
-        for (int b = 0; b < NB; b++) tma_load_3d(smem_u32(smem + W::K) + b * L::BOX, &kmap, 64 * b, tile * TC_KEYS, g, kfull);
+        for (int b = 0; b < NB; b++) tma_load_3d(smem_u32(smem + W::K) + b * L::BOX, &kmap, 64 * b, tile * TA_KEYS, g, kfull);
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)W::ALLOC) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const bool masked = (tile + 1) * TC_KEYS > cached;
-    if (masked && p.parents) ta_ancestors(anc, reinterpret_cast<int*>(smem + W::JUMP), p.parents, p.rows);
+    const bool masked = (tile + 1) * TA_KEYS > cached;
+    if (masked && p.parents) ta_ancestors<TC_SOFT>(anc, reinterpret_cast<int*>(smem + W::JUMP), p.parents, p.rows, tid, [] { __syncthreads(); });
     asm volatile("griddepcontrol.wait;" ::: "memory");                // the statistics come from the kernel before
     const int steps = (p.prows + NR - 1) / NR;
     auto bring = [&](int i) {                                         // product rows of step i, and their statistics
-        float* const rw = row + (i % 3) * 3 * NR;
-        tc_load_q<T, SPLIT, NB, NR>(p, smem + W::Q, rw, g, i * NR, warp, TC_SOFT / 32, lane);
+        float* const rw = row + (i % 3) * 4 * NR;
+        tc_load_q<T, SPLIT, NB, NR, TC_SOFT / 32>(p, smem + W::Q, rw, reinterpret_cast<int*>(rw + 3 * NR), g, i * NR, warp, lane);
         if (tid < NR) {
             const int r = i * NR + tid;
             const float2 st = r < p.prows ? __ldcg(&p.stats[(size_t)g * p.pad_rows + r]) : make_float2(0.f, 0.f);
@@ -507,11 +564,11 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
             for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
         } else tm_wait(x);
         fence_before();
-        const float* const rw = row + (i % 3) * 3 * NR + wg * RW;
+        const float* const rw = row + (i % 3) * 4 * NR + wg * RW;
 #pragma unroll
         for (int r = 0; r < RW; r++) {
             const int pr = i * NR + wg * RW + r;
-            if (pr >= p.prows || (masked && !ta_sees(p, anc, pr / p.group, tile * TC_KEYS + key, cached))) continue;
+            if (pr >= p.prows || (masked && !ta_sees(p, anc, reinterpret_cast<const int*>(rw)[3 * NR + r], tile * TA_KEYS + key, cached))) continue;
             sum += ex2(fmaf(x[r], rw[r], -rw[NR + r])) * rw[2 * NR + r];
         }
     }
@@ -519,8 +576,8 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     if (wg == 1) half[key] = sum;
     fence_before();
     __syncthreads();
-    if (wg == 0 && tile * TC_KEYS + key < total) {
-        float* w = p.weights + (long long)g * p.w_head + tile * TC_KEYS + key;
+    if (wg == 0 && tile * TA_KEYS + key < total) {
+        float* w = p.weights + (long long)g * p.w_head + tile * TA_KEYS + key;
         *w = ok && !*abort_flag ? *w + (sum + half[key]) : NAN;
     }
     if (warp == 0) {
@@ -555,7 +612,7 @@ template <class T, bool SPLIT, int NB, int NR> int run_shape(const TaParams& p, 
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB, int NR> int weigh_shape(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
-    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((p.cached + p.rows + TC_KEYS - 1) / TC_KEYS, p.kv_heads), dim3(TC_SOFT), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
+    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, p.kv_heads), dim3(TC_SOFT), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB> int run_dim(const TaParams& p, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
