@@ -7,6 +7,8 @@ Activations are f32 over an f16 cache, or f16 / bf16 for both.  Heads are contig
 stream.  All arithmetic runs in libirontimber_cuda.so; this file only marshals arguments.
 """
 import ctypes as C
+import functools
+import struct
 
 import torch
 
@@ -81,43 +83,67 @@ def _word(table, word, what):
     return table[word]
 
 
-def _three(x, name, shape, dtype, device):
-    """A [a, b, element] tensor of this shape with contiguous elements."""
-    if x.dim() != 3 or (shape is not None and tuple(x.shape) != shape):
-        raise ValueError(f"{name} has the shape {tuple(x.shape)}" + (f", not {shape}" if shape else ", not three dimensions"))
-    if x.dtype != dtype:
+# A call of a few microseconds is half arguments: tensors are asked for each fact once, the argument structure is packed in one go, and the device and stream
+# are looked up without building objects.
+_NORM_ROPE, _TREE, _EVICT = struct.Struct("@6iP" + "Pqq" * 6 + "qqPPPPif"), struct.Struct("@6i" + "Pqq" * 5 + "qqPPPqPNf0q"), struct.Struct("@2i" + "Pqq" * 2 + "PqPqqqqqPN")
+assert (_NORM_ROPE.size, _TREE.size, _EVICT.size) == (C.sizeof(NormRopeArgs), C.sizeof(TreeAttentionArgs), C.sizeof(CacheEvictArgs))
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_NONE3 = (0, 0, 0)
+
+
+def _three(x, name, shape, dtype, index):
+    """Address and outer strides of a [a, b, element] tensor of this shape with contiguous elements."""
+    st = x.stride()
+    if len(st) != 3 or x.shape != shape:
+        raise ValueError(f"{name} has the shape {tuple(x.shape)}, not {tuple(shape)}")
+    if x.dtype is not dtype:
         raise TypeError(f"{name} is {x.dtype}, not {dtype}")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, not {device}")
-    if x.shape[2] > 1 and x.stride(2) != 1:
+    if x.get_device() != index:
+        raise ValueError(f"{name} is on {x.device}, not on the device of the others")
+    if st[2] != 1 and shape[2] > 1:
         raise ValueError(f"the elements of a head of {name} are not contiguous")
+    return x.data_ptr(), st[0], st[1]
+
+
+def _flat(x, name, n, dtype, index):
+    """Address of a contiguous vector of at least n elements; 0 for None."""
+    if x is None:
+        return 0
+    if x.dim() != 1 or x.shape[0] < n or x.dtype is not dtype or x.get_device() != index or (n > 1 and x.stride(0) != 1):
+        raise ValueError(f"{name} is {tuple(x.shape)} {x.dtype} on {x.device}: a contiguous vector of {n} {dtype} on the device of the others is wanted")
     return x.data_ptr()
 
 
-def _flat(x, name, n, dtype, device):
-    if x.dim() != 1 or x.shape[0] < n or x.dtype != dtype or x.device != device or (n > 1 and x.stride(0) != 1):
-        raise ValueError(f"{name} is {tuple(x.shape)} {x.dtype} on {x.device}: a contiguous vector of {n} {dtype} on {device} is wanted")
-    return x.data_ptr()
+def _caches(k, v, index):
+    """Shape, type and the addresses and strides of a pair of caches."""
+    shape, dtype = k.shape, k.dtype
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise TypeError(f"a cache is float16 or bfloat16, not {dtype}")
+    if len(shape) != 3:
+        raise ValueError(f"k_cache has the shape {tuple(shape)}, not three dimensions")
+    return shape, TYPES[dtype], _three(k, "k_cache", shape, dtype, index), _three(v, "v_cache", shape, dtype, index)
 
 
-def _caches(k, v, device):
-    """Pointers and shape of a pair of caches."""
-    _three(k, "k_cache", None, k.dtype, device)
-    _three(v, "v_cache", tuple(k.shape), k.dtype, device)
-    if k.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"a cache is float16 or bfloat16, not {k.dtype}")
-    return k.shape
+def _rows(x, name):
+    if x.dim() != 3:
+        raise ValueError(f"{name} has the shape {tuple(x.shape)}, not three dimensions")
+    return x.shape
 
 
-def _launch(call, args, device, stream):
-    if not device.type == "cuda":
-        raise ValueError(f"tensors are on {device}, not on a CUDA device")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _launch(call, args, device, stream)
+def _launch(call, args, index, stream):
+    if index < 0:
+        raise ValueError("tensors are not on a CUDA device")
+    if index != (_current_device() if _current_device else torch.cuda.current_device()):
+        with torch.cuda.device(index):
+            return _launch(call, args, index, stream)
     if stream is None:
-        stream = torch.cuda.current_stream(device)
-    _lib.check(call(getattr(stream, "cuda_stream", stream), C.byref(args)))
+        stream = _current_stream(index) if _current_stream else torch.cuda.current_stream(index).cuda_stream
+    elif not isinstance(stream, int):
+        stream = stream.cuda_stream
+    code = call(stream, args)
+    if code:
+        _lib.check(code)
 
 
 def norm_rope(rope, q, k, v, q_out, k_cache, v_cache, slot0, positions, q_norm=None, k_norm=None, eps=1e-6, base=None, stream=None):
@@ -126,37 +152,29 @@ def norm_rope(rope, q, k, v, q_out, k_cache, v_cache, slot0, positions, q_norm=N
     q, q_out: [row, head, element] (q_out may be q); k, v: [row, kv head, element]; q_norm, k_norm: f32 weights of a head, or None for no norm; rope None: no
     rotation.  positions: int32 tensor [row], or the position of row 0.  base: int32 tensor whose value is added to slots (and to positions that
     are a number), read on the device.  q and q_out, or k, v and the caches, may be None."""
-    some = q if q is not None else k
-    device, act, rows, dim = some.device, some.dtype, some.shape[0], some.shape[2]
-    a = NormRopeArgs(type=TYPES.get(act, -1), rows=rows, head_dim=dim, rope=rope.handle if rope is not None else None, slot0=slot0, eps=eps)
-    a.heads = a.kv_heads = 1
-    a.cache_type = 1 if act == torch.float32 else a.type
+    some, name = (q, "q") if q is not None else (k, "k")
+    rows, heads, dim = _rows(some, name)
+    act, index = some.dtype, some.get_device()
+    t = ct = TYPES.get(act, -1)
+    kv, slots, qp, qo, kp, vp, kc, vc = 1, 0, _NONE3, _NONE3, _NONE3, _NONE3, _NONE3, _NONE3
+    if t == 0:
+        ct = 1
     if q is not None:
-        a.q, a.q_out = _three(q, "q", None, act, device), _three(q_out, "q_out", tuple(q.shape), act, device)
-        (a.q_row, a.q_head, _), (a.qo_row, a.qo_head, _) = q.stride(), q_out.stride()
-        a.heads = q.shape[1]
+        qp, qo = _three(q, "q", q.shape, act, index), _three(q_out, "q_out", q.shape, act, index)
     if k is not None:
-        a.k, a.v = _three(k, "k", (rows, k.shape[1], dim), act, device), _three(v, "v", tuple(k.shape), act, device)
-        slots, kv, d = _caches(k_cache, v_cache, device)
-        if kv != k.shape[1] or d != dim:
-            raise ValueError(f"caches of {kv} heads of {d} for {k.shape[1]} heads of {dim}")
-        (a.k_row, a.k_head, _), (a.v_row, a.v_head, _) = k.stride(), v.stride()
-        a.k_cache, a.v_cache, a.slots, a.cache_type = k_cache.data_ptr(), v_cache.data_ptr(), slots, TYPES[k_cache.dtype]
-        (a.kc_slot, a.kc_head, _), (a.vc_slot, a.vc_head, _) = k_cache.stride(), v_cache.stride()
-        a.kv_heads = kv
-        if q is None:
-            a.heads = kv
+        (slots, kv, d), ct, kc, vc = _caches(k_cache, v_cache, index)
+        want = (rows, kv, dim)
+        if d != dim or k.shape != want:
+            raise ValueError(f"caches of {kv} heads of {d} for k of {tuple(k.shape)} behind q of {rows} rows of {dim}")
+        kp, vp = _three(k, "k", want, act, index), _three(v, "v", want, act, index)
+    pos0 = 0
     if isinstance(positions, torch.Tensor):
-        a.positions = _flat(positions, "positions", rows, torch.int32, device)
+        positions = _flat(positions, "positions", rows, torch.int32, index)
     else:
-        a.pos0 = positions
-    if base is not None:
-        a.base = _flat(base, "base", 1, torch.int32, device)
-    if q_norm is not None:
-        a.q_norm = _flat(q_norm, "q_norm", dim, torch.float32, device)
-    if k_norm is not None:
-        a.k_norm = _flat(k_norm, "k_norm", dim, torch.float32, device)
-    _launch(_lib.load().it_norm_rope, a, device, stream)
+        pos0, positions = positions, 0
+    args = _NORM_ROPE.pack(t, ct, rows, heads, kv, dim, rope.handle.value if rope is not None else 0, *qp, *kp, *vp, *qo, *kc, *vc, slots, slot0, positions, _flat(base, "base", 1, torch.int32, index),
+                           _flat(q_norm, "q_norm", dim, torch.float32, index), _flat(k_norm, "k_norm", dim, torch.float32, index), pos0, eps)
+    _launch(_load().it_norm_rope, args, index, stream)
 
 
 def tree_attention(q, k_cache, v_cache, cached, out, parents=None, gate=None, scale=0.0, length=None, weights=None, workspace=None, stream=None):
@@ -165,73 +183,75 @@ def tree_attention(q, k_cache, v_cache, cached, out, parents=None, gate=None, sc
     parents: int32 [row], the row that a row continues or -1 for the cache; None: a chain.  scale 0: head_dim^-1/2.  length: int32 tensor, the number of cached
     slots (at most `cached`), read on the device.  weights: f32 [kv head, slot], to which the softmax weight that every slot received is added.
     workspace: a uint8 tensor of tree_attention_workspace() bytes; None: one from torch's allocator."""
-    device, act = q.device, q.dtype
-    rows, heads, dim = q.shape
-    slots, kv, d = _caches(k_cache, v_cache, device)
+    shape = rows, heads, dim = _rows(q, "q")
+    act, index = q.dtype, q.get_device()
+    (slots, kv, d), ct, kc, vc = _caches(k_cache, v_cache, index)
     if d != dim:
         raise ValueError(f"caches of heads of {d} for heads of {dim}")
-    a = TreeAttentionArgs(TYPES.get(act, -1), TYPES[k_cache.dtype], rows, heads, kv, dim)
-    a.q, a.out = _three(q, "q", None, act, device), _three(out, "out", (rows, heads, dim), act, device)
-    (a.q_row, a.q_head, _), (a.o_row, a.o_head, _) = q.stride(), out.stride()
-    if gate is not None:
-        a.gate = _three(gate, "gate", (rows, heads, dim), act, device)
-        a.g_row, a.g_head, _ = gate.stride()
-    a.k_cache, a.v_cache, a.slots, a.cached, a.scale = k_cache.data_ptr(), v_cache.data_ptr(), slots, cached, scale
-    (a.kc_slot, a.kc_head, _), (a.vc_slot, a.vc_head, _) = k_cache.stride(), v_cache.stride()
-    if parents is not None:
-        a.parents = _flat(parents, "parents", rows, torch.int32, device)
-    if length is not None:
-        a.length = _flat(length, "length", 1, torch.int32, device)
-    if weights is not None:
-        a.weights, a.w_head = _weights(weights, kv, cached + rows, device)
-    L = _lib.load()
-    need = C.c_size_t()
-    _lib.check(L.it_tree_attention_workspace(C.byref(a), C.byref(need)))
-    _workspace(a, workspace, need.value, device, stream)
-    _launch(L.it_tree_attention, a, device, stream)
+    t = TYPES.get(act, -1)
+    qp, op = _three(q, "q", shape, act, index), _three(out, "out", shape, act, index)
+    gp = _three(gate, "gate", shape, act, index) if gate is not None else _NONE3
+    wp, wh = _weights(weights, kv, cached + rows, index) if weights is not None else (0, 0)
+    parents, length = _flat(parents, "parents", rows, torch.int32, index), _flat(length, "length", 1, torch.int32, index)
+    if workspace is None:
+        workspace = _workspace(_tree_bytes(t, ct, rows, heads, kv, dim), index, stream)
+    else:
+        _check_workspace(workspace, index)
+    args = _TREE.pack(t, ct, rows, heads, kv, dim, *qp, *gp, *op, *kc, *vc, slots, cached, parents, length, wp, wh, workspace.data_ptr(), workspace.numel(), scale)
+    _launch(_load().it_tree_attention, args, index, stream)
 
 
 def cache_evict(k_cache, v_cache, weights, n, keep, recent, kept=None, workspace=None, stream=None):
     """Cuts a cache of n slots to `keep` a KV head: the last `recent`, and of the others those with the largest weight (f32 [kv head, slot]; ties: the
     lower slot).  They move to the front in their order, in place, in both caches and the weights; kept (int32 [kv head, keep]) gets the slots they had."""
-    device = weights.device
-    slots, kv, dim = _caches(k_cache, v_cache, device)
-    a = CacheEvictArgs(kv, dim, k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1))
-    a.slots, a.n, a.keep, a.recent = slots, n, keep, recent
-    a.weights, a.w_head = _weights(weights, kv, n, device)
+    index = weights.get_device()
+    (slots, kv, dim), _, kc, vc = _caches(k_cache, v_cache, index)
+    wp, wh = _weights(weights, kv, n, index)
+    ws, nbytes, kp, kh = 0, 0, 0, 0
     if kept is not None:
-        if tuple(kept.shape) != (kv, keep) or kept.dtype != torch.int32 or kept.device != device or (keep > 1 and kept.stride(1) != 1):
+        if kept.shape != (kv, keep) or kept.dtype is not torch.int32 or kept.get_device() != index or (keep > 1 and kept.stride(1) != 1):
             raise ValueError(f"kept is {tuple(kept.shape)} {kept.dtype}: int32 {(kv, keep)} with contiguous rows is wanted")
-        a.kept, a.kept_head = kept.data_ptr(), kept.stride(0)
-    L = _lib.load()
-    if kept is None or workspace is not None:
-        need = C.c_size_t()
-        _lib.check(L.it_cache_evict_workspace(C.byref(a), C.byref(need)))
-        _workspace(a, workspace, need.value, device, stream)
-    _launch(L.it_cache_evict, a, device, stream)
+        kp, kh = kept.data_ptr(), kept.stride(0)
+    else:
+        workspace = _workspace(4 * kv * keep + 256, index, stream) if workspace is None else _check_workspace(workspace, index)
+        ws, nbytes = workspace.data_ptr(), workspace.numel()
+    args = _EVICT.pack(kv, dim, *kc, *vc, wp, wh, kp, kh, slots, n, keep, recent, ws, nbytes)
+    _launch(_load().it_cache_evict, args, index, stream)
 
 
-def _weights(w, kv, n, device):
-    if w.dim() != 2 or w.shape[0] != kv or w.shape[1] < n or w.dtype != torch.float32 or w.device != device or (n > 1 and w.stride(1) != 1):
-        raise ValueError(f"weights are {tuple(w.shape)} {w.dtype} on {w.device}: f32 [{kv}, {n} or more] with contiguous rows on {device} are wanted")
+_load = _lib.load
+
+
+def _weights(w, kv, n, index):
+    if w.dim() != 2 or w.shape[0] != kv or w.shape[1] < n or w.dtype is not torch.float32 or w.get_device() != index or (n > 1 and w.stride(1) != 1):
+        raise ValueError(f"weights are {tuple(w.shape)} {w.dtype} on {w.device}: f32 [{kv}, {n} or more] with contiguous rows on the device of the others are wanted")
     return w.data_ptr(), w.stride(0)
 
 
-def _workspace(a, workspace, need, device, stream):
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        if stream is not None:               # torch hands the memory out again in the order of the current stream
-            workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream, device=device))
-    elif workspace.dtype != torch.uint8 or workspace.device != device or not workspace.is_contiguous():
+def _workspace(nbytes, index, stream):
+    if index < 0:
+        raise ValueError("tensors are not on a CUDA device")
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=index)
+    if stream is not None:                   # torch hands the memory out again in the order of the current stream
+        workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream, device=index))
+    return workspace
+
+
+def _check_workspace(w, index):
+    if w.dtype is not torch.uint8 or w.get_device() != index or not w.is_contiguous():
         raise ValueError("a workspace is a contiguous uint8 tensor on the tensors' device")
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    return w
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_bytes(t, ct, rows, heads, kv, dim, cached=(1 << 30) - 1):
+    """Bytes of workspace; by default for any number of cached slots, which is what a call that allocates asks for (it depends on them only while they are few)."""
+    need = C.c_size_t()
+    _lib.check(_lib.load().it_tree_attention_workspace(C.byref(TreeAttentionArgs(t, ct, rows, heads, kv, dim, cached=cached)), C.byref(need)))
+    return need.value
 
 
 def tree_attention_workspace(rows, heads, kv_heads, head_dim, cached, dtype=torch.float32):
     """Bytes of workspace for a call of these sizes."""
     t = TYPES.get(dtype, -1)
-    a = TreeAttentionArgs(t, 1 if t == 0 else t, rows, heads, kv_heads, head_dim)
-    a.cached = cached
-    need = C.c_size_t()
-    _lib.check(_lib.load().it_tree_attention_workspace(C.byref(a), C.byref(need)))
-    return need.value
+    return _tree_bytes(t, 1 if t == 0 else t, rows, heads, kv_heads, head_dim, cached)

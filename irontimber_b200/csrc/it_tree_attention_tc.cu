@@ -104,19 +104,17 @@ __device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 3, 256;" 
 template <class T, bool SPLIT, int NB, int NR, int NW>
 __device__ void tc_load_q(const TaParams& p, unsigned char* q, float* fac, int* trow, int g, int r0, int warp, int lane) {
     using L = TcTree<SPLIT, NB, NR>;
-    constexpr int N = NR < 3 * NW ? (NR + NW - 1) / NW : 3;
+    constexpr int N = (NR + NW - 1) / NW;
     TaRow<T, SPLIT> x[N];
-#pragma unroll 1
-    for (int i0 = warp; i0 < NR; i0 += N * NW) {
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        const int i = i0 + k * NW, r = r0 + i, t = min(ta_row(p, r), p.rows - 1), h = g * p.group + r - t * p.group;
+        const int i = warp + k * NW, r = r0 + i, t = min(ta_row(p, r), p.rows - 1), h = g * p.group + r - t * p.group;
         if (i < NR && lane == 0) trow[i] = t;
         x[k].load(p, i < NR && r < p.prows && 8 * lane < p.dim, t, h, lane);
     }
 #pragma unroll
     for (int k = 0; k < N; k++) {
-        const int i = i0 + k * NW;
+        const int i = warp + k * NW;
         if (i >= NR) break;
         unsigned hi[4], lo[4];
         const float f = x[k].halves(p, hi, lo);
@@ -126,7 +124,6 @@ __device__ void tc_load_q(const TaParams& p, unsigned char* q, float* fac, int* 
             if constexpr (SPLIT) *reinterpret_cast<uint4*>(q + at + NR * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         if (lane == 0) fac[i] = f;
-    }
     }
 }
 
@@ -161,7 +158,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TA_KEYS - 1) / TA_KEYS;
-    const int tile0 = (int)((long long)split * tiles / p.splits), n = (int)((long long)(split + 1) * tiles / p.splits) - tile0;
+    // this run's tiles: the first `tiles % splits` runs have one more
+    const int per = (int)((unsigned)tiles / (unsigned)p.splits), more = tiles - per * p.splits, tile0 = split * per + min(split, more), n = per + (split < more ? 1 : 0);
     // Tile i of K (v = 0) or V, when its slot is free; copies of K and V have a warp each, since they wait for different products.
     auto load = [&](int v, int i) {
         const int s = i % (v ? VS : KS);
@@ -376,11 +374,10 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
         }
         if (quad == 0 && lane < RW) ml[wg * RW + lane].x = mrun == -INFINITY ? mrun : base_s[wg * RW + lane];
         if (p.splits > 1) {
-            // rows behind the last one are written too: the workspace has room for them
             const size_t at = ((size_t)split * p.kv_heads + g) * p.pad_rows + r0;
             float* const o = p.part_o + (at + orow) * HD + d;
 #pragma unroll
-            for (int r = 0; r < OR; r++) __stcg(o + r * HD, acc[r]);
+            for (int r = 0; r < OR; r++) if (r0 + orow + r < p.prows) __stcg(o + r * HD, acc[r]);
             groups_sync();
             if (tid < NR) p.part_ml[at + tid] = ml[tid];
         } else {
