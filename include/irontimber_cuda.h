@@ -406,7 +406,7 @@ int it_tree_attention_workspace(const it_tree_attention_args* a, size_t* nbytes)
 /* Cuts a cache of n slots down to `keep` per kv head: the last `recent` slots stay, and of the others the keep - recent with the largest weight
  * (equal weights: the lower slot; NaN ranks below everything; -0 equals 0).  What stays moves to slots 0..keep-1 in its old order, in place, in k_cache, v_cache
  * and weights (each may be NULL except weights); kept[g][i] (i32, kept_head apart, may be NULL) is the slot that slot i of head g held before.  Slots from keep on are left
- * as they were.  0 <= recent <= keep <= n <= slots, n <= 1,048,576.  Works on 16-bit caches of any head_dim that is a multiple of 8 up to 256.
+ * as they were.  0 <= recent <= keep <= n <= slots, n <= 524,288.  Works on 16-bit caches of any head_dim that is a multiple of 8 up to 256.
  * workspace as above, it_cache_evict_workspace() bytes. */
 typedef struct it_cache_evict_args {
     int32_t kv_heads, head_dim;

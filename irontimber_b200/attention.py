@@ -203,19 +203,21 @@ def tree_attention(q, k_cache, v_cache, cached, out, parents=None, gate=None, sc
 
 def cache_evict(k_cache, v_cache, weights, n, keep, recent, kept=None, workspace=None, stream=None):
     """Cuts a cache of n slots to `keep` a KV head: the last `recent`, and of the others those with the largest weight (f32 [kv head, slot]; ties: the
-    lower slot).  They move to the front in their order, in place, in both caches and the weights; kept (int32 [kv head, keep]) gets the slots they had."""
+    lower slot).  They move to the front in their order, in place, in both caches and the weights; kept (int32 [kv head, keep]) gets the slots they had.
+    workspace: a uint8 tensor of cache_evict_workspace() bytes; None: one from torch's allocator."""
     index = weights.get_device()
     (slots, kv, dim), _, kc, vc = _caches(k_cache, v_cache, index)
     wp, wh = _weights(weights, kv, n, index)
-    ws, nbytes, kp, kh = 0, 0, 0, 0
+    kp = kh = 0
     if kept is not None:
         if kept.shape != (kv, keep) or kept.dtype is not torch.int32 or kept.get_device() != index or (keep > 1 and kept.stride(1) != 1):
             raise ValueError(f"kept is {tuple(kept.shape)} {kept.dtype}: int32 {(kv, keep)} with contiguous rows is wanted")
         kp, kh = kept.data_ptr(), kept.stride(0)
+    if workspace is None:
+        workspace = _workspace(cache_evict_workspace(kv, n, keep), index, stream)
     else:
-        workspace = _workspace(4 * kv * keep + 256, index, stream) if workspace is None else _check_workspace(workspace, index)
-        ws, nbytes = workspace.data_ptr(), workspace.numel()
-    args = _EVICT.pack(kv, dim, *kc, *vc, wp, wh, kp, kh, slots, n, keep, recent, ws, nbytes)
+        _check_workspace(workspace, index)
+    args = _EVICT.pack(kv, dim, *kc, *vc, wp, wh, kp, kh, slots, n, keep, recent, workspace.data_ptr(), workspace.numel())
     _launch(_load().it_cache_evict, args, index, stream)
 
 
@@ -248,6 +250,14 @@ def _tree_bytes(t, ct, rows, heads, kv, dim, cached=(1 << 30) - 1):
     """Bytes of workspace; by default for any number of cached slots, which is what a call that allocates asks for (it depends on them only while they are few)."""
     need = C.c_size_t()
     _lib.check(_lib.load().it_tree_attention_workspace(C.byref(TreeAttentionArgs(t, ct, rows, heads, kv, dim, cached=cached)), C.byref(need)))
+    return need.value
+
+
+@functools.lru_cache(maxsize=256)
+def cache_evict_workspace(kv_heads, n, keep):
+    """Bytes of workspace for an eviction of these sizes."""
+    need = C.c_size_t()
+    _lib.check(_lib.load().it_cache_evict_workspace(C.byref(CacheEvictArgs(kv_heads, 8, n=n, slots=n, keep=keep)), C.byref(need)))
     return need.value
 
 

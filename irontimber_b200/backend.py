@@ -283,8 +283,8 @@ class CudaBackend:
     def cache_evict(self, k_cache, v_cache, weights, n, keep, recent, kept=None, **options):
         """attention.cache_evict on this backend's stream."""
         from . import attention
-        if kept is None and options.get("workspace") is None:
-            options["workspace"] = self._workspace(4 * k_cache.shape[1] * keep + 256)
+        if options.get("workspace") is None:
+            options["workspace"] = self._workspace(attention.cache_evict_workspace(k_cache.shape[1], n, keep))
         attention.cache_evict(k_cache, v_cache, weights, n, keep, recent, kept, stream=self.torch_stream, **options)
 
     def _workspace(self, nbytes):

@@ -86,7 +86,7 @@ def tree_args(**change):
 def evict_args(**change):
     from irontimber_b200.attention import CacheEvictArgs
     a = dict(kv_heads=2, head_dim=64, k_cache=5 * A, kc_slot=128, kc_head=64, v_cache=6 * A, vc_slot=128, vc_head=64, weights=7 * A, w_head=300, kept=8 * A, kept_head=100,
-             slots=300, n=200, keep=100, recent=10)
+             slots=300, n=200, keep=100, recent=10, workspace=16 * A, workspace_bytes=1 << 20)
     a.update(change)
     return CacheEvictArgs(**a)
 
@@ -138,9 +138,9 @@ def test_tree_attention_refusals(lib, change, part):
 
 
 @pytest.mark.parametrize("change,part", [
-    (dict(kv_heads=0), "kv heads"), (dict(head_dim=12), "head dimension"), (dict(recent=101), "keep"), (dict(keep=201), "keep"), (dict(n=301), "keep"), (dict(recent=-1), "keep"), (dict(slots=1 << 21, n=(1 << 20) + 1), "keep"),
-    (dict(weights=None), "weights"), (dict(w_head=199), "weights"), (dict(k_cache=5 * A + 8), "16-byte"), (dict(vc_slot=60), "16-byte"), (dict(kept_head=99), "kept"), (dict(kept=None), "workspace"),
-    (dict(kept=None, workspace=A, workspace_bytes=799), "workspace"), (dict(kept=None, workspace=A + 128, workspace_bytes=1 << 20), "workspace")])
+    (dict(kv_heads=0), "kv heads"), (dict(head_dim=12), "head dimension"), (dict(recent=101), "keep"), (dict(keep=201), "keep"), (dict(n=301), "keep"), (dict(recent=-1), "keep"), (dict(slots=1 << 21, n=(1 << 19) + 1), "keep"),
+    (dict(weights=None), "weights"), (dict(w_head=199), "weights"), (dict(k_cache=5 * A + 8), "16-byte"), (dict(vc_slot=60), "16-byte"), (dict(kept_head=99), "kept"), (dict(workspace=None), "workspace"),
+    (dict(workspace_bytes=800), "workspace"), (dict(workspace=A + 128), "workspace")])
 def test_cache_evict_refusals(lib, change, part):
     refused(lib, lib.it_cache_evict, evict_args(**change), part)
 
@@ -162,8 +162,8 @@ def test_workspace_goes_by_sizes_alone(lib):
     assert lib.it_tree_attention_workspace(C.byref(tree_args(rows=0)), C.byref(n)) == 0 and n.value == 0
     # runs of a cache are at most one wave of CTAs: never more than this, however long it is
     assert tree_attention_workspace(256, 24, 4, 256, (1 << 30) - 1) < 64 << 20 and tree_attention_workspace(1, 1, 1, 256, (1 << 30) - 1) < 4 << 20
-    assert lib.it_cache_evict_workspace(C.byref(evict_args()), C.byref(n)) == 0 and n.value == 0
-    assert lib.it_cache_evict_workspace(C.byref(evict_args(kept=None)), C.byref(n)) == 0 and n.value >= 800
+    assert lib.it_cache_evict_workspace(C.byref(evict_args(workspace=None, weights=None)), C.byref(n)) == 0 and n.value >= 800
+    assert lib.it_cache_evict_workspace(C.byref(evict_args(keep=0, recent=0)), C.byref(n)) == 0 and n.value == 0
 
 
 def test_tensors_are_checked_before_the_library_sees_them(lib):

@@ -472,7 +472,8 @@ def fill(g, kv, n, what):
 @pytest.mark.parametrize("n,keep,recent,kv,dim,what", [
     (1, 1, 0, 1, 8, "rand"), (1, 0, 0, 2, 64, "rand"), (2, 1, 0, 2, 64, "ties"), (2, 1, 1, 2, 64, "rand"), (33, 32, 0, 1, 64, "odd"), (100, 100, 10, 2, 128, "rand"), (1200, 1024, 64, 8, 128, "rand"), (1200, 600, 600, 1, 80, "rand"),
     (2049, 2048, 7, 3, 256, "same"), (5000, 17, 3, 4, 256, "ties"), (8192, 4096, 0, 4, 256, "close"), (8193, 4096, 0, 4, 64, "odd"), (9000, 8999, 1, 2, 128, "falling"), (9000, 4500, 100, 2, 256, "rising"),
-    (30000, 10000, 129, 4, 256, "rand"), (70001, 35000, 1000, 1, 64, "ties"), (70000, 69999, 0, 2, 128, "odd")])
+    (30000, 10000, 129, 4, 256, "rand"), (70001, 35000, 1000, 1, 64, "ties"), (70000, 69999, 0, 2, 128, "odd"),
+    (4096, 2000, 5, 2, 64, "ties"), (4097, 2000, 5, 2, 64, "ties"), (200000, 150000, 77, 1, 64, "rising"), (262144, 200001, 3, 1, 16, "rand"), (300001, 100000, 64, 2, 64, "rand"), (524288, 524287, 1, 1, 8, "same")])
 def test_cache_evict(ops, n, keep, recent, kv, dim, what):
     g = gen(n + keep)
     spare = 11
