@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_con
     const int cand = p.n - p.recent, want = p.keep - p.recent;
     const int begin = rank * p.per, len = max(0, min(p.n - begin, p.per)), clen = max(0, min(cand - begin, p.per));      // this CTA's slots, and those of them that compete
     for (int i = blockIdx.x * EV_THREADS + tid; i < p.nflags; i += gridDim.x * EV_THREADS) p.flags[i] = 0u;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid; i < len; i += EV_THREADS) w_s[i] = w[begin + i];
     if (CL == 1 || want == 0) sync();                  // (else the first pass's barrier) every weight is read before any is written
     // ---- the smallest kept key; `left`: how many of the keys with the bits found so far are kept
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_con
         hist[tid] = 0; hist[tid + EV_THREADS] = 0;
         __syncthreads();
         const unsigned above = pass == 0 ? 0 : prefix >> up;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = tid; i < clen; i += EV_THREADS) {
             const unsigned key = ev_key(w_s[i]);
             if (pass == 0 || key >> up == above) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_con
     // ---- kept: the last slots, keys above `prefix`, and the first `left` of those equal to it, in slot order.  A warp has a run of its CTA's slots.
     const int wper = p.per / EV_WARPS, wb = warp * wper, we = min(len, wb + wper);
     unsigned gt = 0, eq = 0;
-#pragma unroll 2
+#pragma unroll 4
     for (int i = wb; i < we; i += 32) {
         const bool in = i + lane < we;
         const unsigned key = in ? ev_key(w_s[i + lane]) : 0u;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_con
     if (CL > 1 && lane < rank) { a += *cluster.map_shared_rank(&counts[0], lane); b += *cluster.map_shared_rank(&counts[1], lane); }
     unsigned gt0 = __reduce_add_sync(0xffffffffu, a), eq0 = __reduce_add_sync(0xffffffffu, b);
     const unsigned below = (1u << lane) - 1u;
-#pragma unroll 2
+#pragma unroll 4
     for (int i = wb; i < we; i += 32) {
         const bool in = i + lane < we;
         const float x = in ? w_s[i + lane] : 0.f;
@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) k_evict_move(const __grid_con
 struct EvPlan { int cluster, per, rank_head, blocks; size_t kept, ranks, flags, nflags, total; };
 EvPlan ev_plan(const it_cache_evict_args* a) {
     EvPlan pl;
-    pl.cluster = a->n <= 4096 ? 1 : a->n <= 262144 ? 8 : 16;
+    // us for 4 heads of dimension 8 with 1 / 8 / 16 CTAs: 4096 slots 11.2 / 14.2 / 18.3, 8192 16.4 / 16.0 / 20.3, 32,768 38 / 21 / 25, 131,072 - / 42 / 40, 262,144 - / 56 / 48
+    pl.cluster = a->n <= 6144 ? 1 : a->n <= 98304 ? 8 : 16;
     pl.per = (int)(((a->n + pl.cluster - 1) / pl.cluster + EV_UNIT - 1) / EV_UNIT * EV_UNIT);
     pl.rank_head = (int)((a->n + EV_BLOCK - 1) / EV_BLOCK + 1);
     pl.blocks = (int)((a->keep + EV_BLOCK - 1) / EV_BLOCK);

@@ -38,6 +38,18 @@ __global__ void __launch_bounds__(NR_WARPS * 32) k_norm_rope(const __grid_consta
     const int nq = p.q ? p.heads : 0, nkv = p.k ? p.kv_heads : 0;
     const int job = blockIdx.y * NR_WARPS + warp;
     const int add = p.base ? *p.base : 0;
+    const bool is_q = job < nq, is_v = job >= nq + nkv;
+    const int h = is_q ? job : is_v ? job - nq - nkv : job - nq;
+    const long long slot = p.slot0 + add + t;
+    const bool live = job < nq + 2 * nkv && (is_q || (slot >= 0 && slot < p.slots));
+    const TA* x = is_q ? (const TA*)p.q + t * p.q_row + h * p.q_head : is_v ? (const TA*)p.v + t * p.v_row + h * p.v_head : (const TA*)p.k + t * p.k_row + h * p.k_head;
+    float v[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {              // under way while the table is made
+        const int e = 4 * lane + 128 * j;
+        if (live && e < p.dim) load4(x + e, v[j]);
+        else v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
+    }
     if (p.pairs) {
         const int pos = p.positions ? p.positions[t] : p.pos0 + add + t;
         for (int i = threadIdx.x; i < p.pairs; i += NR_WARPS * 32) {
@@ -46,19 +58,7 @@ __global__ void __launch_bounds__(NR_WARPS * 32) k_norm_rope(const __grid_consta
         }
         __syncthreads();
     }
-    if (job >= nq + 2 * nkv) return;
-    const bool is_q = job < nq, is_v = job >= nq + nkv;
-    const int h = is_q ? job : is_v ? job - nq - nkv : job - nq;
-    const long long slot = p.slot0 + add + t;
-    if (!is_q && (slot < 0 || slot >= p.slots)) return;
-    const TA* x = is_q ? (const TA*)p.q + t * p.q_row + h * p.q_head : is_v ? (const TA*)p.v + t * p.v_row + h * p.v_head : (const TA*)p.k + t * p.k_row + h * p.k_head;
-    float v[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int e = 4 * lane + 128 * j;
-        if (e < p.dim) load4(x + e, v[j]);
-        else v[j][0] = v[j][1] = v[j][2] = v[j][3] = 0.f;
-    }
+    if (!live) return;
     if (!is_v) {
         const float* w = is_q ? p.q_norm : p.k_norm;
         if (w) {
