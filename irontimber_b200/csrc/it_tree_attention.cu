@@ -16,59 +16,68 @@
 
 namespace {
 
-// Joins the runs of one product row: out = sum of the runs' outputs, each scaled to the common maximum, over the sum of their sums.  Four groups of HD / 4 threads
-// take every fourth run; runs that saw nothing are not read.
+// Joins the runs of one product row: out = sum of the runs' outputs, each scaled to the common reference, over the sum of their sums, in a fixed order.  Four groups of
+// HD / 4 threads take every fourth run; runs that saw nothing are not read.  Latency: the gate and the first outputs are asked for before the weights are known, and every
+// warp forms the weights of all runs for itself instead of meeting the others.
 template <class TA, int NB>
 __global__ void __launch_bounds__(64 * NB) k_tree_join(const __grid_constant__ TaParams p) {
-    constexpr int HD = 64 * NB, LANES = HD / 4;
-    __shared__ float wgt[1024];
-    __shared__ float red[2][32];
+    constexpr int HD = 64 * NB, LANES = HD / 4, WARPS = 2 * NB, AHEAD = 4;
+    __shared__ float wgt[WARPS][TA_MAXSPLITS];
     __shared__ float4 acc[3][LANES];
+    const int tid = threadIdx.x, r = blockIdx.x, g = blockIdx.y, warp = tid >> 5, lane = tid & 31;
+    const int grp = tid / LANES, c = tid % LANES * 4;
+    const int t = ta_row(p, r), h = g * p.group + r - t * p.group;
+    float z[4] = { 0.f, 0.f, 0.f, 0.f };
+    // the gate is the caller's: nothing before this kernel in the call writes it
+    if (p.gate && grp == 0 && c < p.dim) load4((const TA*)p.gate + t * p.g_row + h * p.g_head + c, z);
     asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, r = blockIdx.x, g = blockIdx.y, warp = tid >> 5, lane = tid & 31, nw = blockDim.x >> 5;
     const size_t step = (size_t)p.kv_heads * p.pad_rows, at = (size_t)g * p.pad_rows + r;
+    const float* const o = p.part_o + at * HD + c;
+    float2 e[(TA_MAXSPLITS + 31) / 32];
+    float4 v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < (TA_MAXSPLITS + 31) / 32; k++) { const int s = lane + 32 * k; e[k] = s < p.splits ? __ldcg(&p.part_ml[s * step + at]) : make_float2(-INFINITY, 0.f); }
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) { const int s = grp + 4 * k; v[k] = s < p.splits ? __ldcg(reinterpret_cast<const float4*>(o + s * step * HD)) : make_float4(0.f, 0.f, 0.f, 0.f); }
     float top = -INFINITY;
-    for (int s = tid; s < p.splits; s += blockDim.x) top = fmaxf(top, __ldcg(&p.part_ml[s * step + at]).x);
+#pragma unroll
+    for (int k = 0; k < (TA_MAXSPLITS + 31) / 32; k++) top = fmaxf(top, e[k].x);
 #pragma unroll
     for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    if (lane == 0) red[0][warp] = top;
-    __syncthreads();
-    for (int k = 0; k < nw; k++) top = fmaxf(top, red[0][k]);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-    for (int s = tid; s < p.splits; s += blockDim.x) {
-        const float2 e = __ldcg(&p.part_ml[s * step + at]);
-        const float w = ex2(e.x - ref);
-        wgt[s] = e.x == -INFINITY && e.y == 0.f ? -1.f : w;           // -1: not written, not read
-        sum += e.y * w;
+#pragma unroll
+    for (int k = 0; k < (TA_MAXSPLITS + 31) / 32; k++) {
+        const int s = lane + 32 * k;
+        const float w = ex2(e[k].x - ref);
+        if (s < p.splits) wgt[warp][s] = e[k].x == -INFINITY && e[k].y == 0.f ? -1.f : w;           // -1: saw nothing
+        sum += e[k].y * w;
     }
-    // a fixed order, so that the same inputs give the same bits
 #pragma unroll
     for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-    if (lane == 0) red[1][warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-    for (int k = 0; k < nw; k++) sum += red[1][k];
-    const int grp = tid / LANES, c = tid % LANES * 4;
+    __syncwarp();
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, const float4& x) {
+        if (w < 0.f) return;
+        a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) if (grp + 4 * k < p.splits) add(wgt[warp][grp + 4 * k], v[k]);
 #pragma unroll 4
-    for (int s = grp; s < p.splits; s += 4) {
-        const float w = wgt[s];
-        if (w < 0.f) continue;
-        const float4 e = __ldcg(reinterpret_cast<const float4*>(p.part_o + (s * step + at) * HD + c));
-        a.x = fmaf(w, e.x, a.x); a.y = fmaf(w, e.y, a.y); a.z = fmaf(w, e.z, a.z); a.w = fmaf(w, e.w, a.w);
-    }
+    for (int s = grp + 4 * AHEAD; s < p.splits; s += 4) add(wgt[warp][s], __ldcg(reinterpret_cast<const float4*>(o + s * step * HD)));
     if (grp) acc[grp - 1][tid % LANES] = a;
     __syncthreads();
     if (p.stats && tid == 0) p.stats[at] = make_float2(ref, sum);
     if (grp || c >= p.dim) return;
 #pragma unroll
-    for (int k = 0; k < 3; k++) { const float4 e = acc[k][tid]; a.x += e.x; a.y += e.y; a.z += e.z; a.w += e.w; }
+    for (int k = 0; k < 3; k++) { const float4 x = acc[k][tid]; a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w; }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = ta_row(p, r), h = g * p.group + r - t * p.group;
-    float v[4] = { a.x * inv, a.y * inv, a.z * inv, a.w * inv };
-    ta_gate<TA>(p, t, h, c, v);
-    store4((TA*)p.out + t * p.o_row + h * p.o_head + c, v);
+    float out[4] = { a.x * inv, a.y * inv, a.z * inv, a.w * inv };
+    if (p.gate) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] /= 1.f + __expf(-z[i]);
+    }
+    store4((TA*)p.out + t * p.o_row + h * p.o_head + c, out);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
@@ -83,7 +92,7 @@ TaPlan ta_plan(const it_tree_attention_args* a, int sm_count) {
     pl.row_tiles = (prows + pl.nr - 1) / pl.nr;
     pl.pad_rows = pl.row_tiles * pl.nr;
     const long tiles = ((long)a->cached + a->rows + TA_KEYS - 1) / TA_KEYS, ctas = (long)a->kv_heads * pl.row_tiles;
-    long splits = sm_count / ctas;             // one wave of CTAs
+    long splits = sm_count / ctas;             // one wave of CTAs: at most TA_MAXSPLITS
     if (splits > tiles) splits = tiles;
     if (splits < 1) splits = 1;
     pl.splits = (int)splits;
@@ -153,7 +162,7 @@ IT_API int it_tree_attention_workspace(const it_tree_attention_args* a, size_t* 
     if (const int r = ta_check_sizes(a)) return r;
     IT_CHECK_ARG(nbytes, "it_tree_attention_workspace: null argument");
     // without a device: as many SMs as sm_100a parts have
-    *nbytes = a->rows ? ta_plan(a, 148).total : 0;
+    *nbytes = a->rows ? ta_plan(a, TA_MAXSPLITS).total : 0;
     return IT_OK;
 }
 
@@ -180,7 +189,7 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     it_ops_device dev;
     if (const int r = it_ops_current(stream, who, &dev)) return r;
     if (const int r = ta_prepare(dev.device)) return r;
-    const TaPlan pl = ta_plan(a, 148);
+    const TaPlan pl = ta_plan(a, TA_MAXSPLITS);
     IT_CHECK_ARG(a->workspace && it_aligned(a->workspace, 256) && a->workspace_bytes >= pl.total, "%s: a workspace of %zu bytes, 256-byte aligned, is needed", who, pl.total);
     CUtensorMap km, vm;
     if (const int r = ta_map(&km, a->k_cache, a->cache_type, a->head_dim, a->cached + T, a->kc_slot, a->kv_heads, a->kc_head)) return r;

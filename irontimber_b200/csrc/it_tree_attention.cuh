@@ -19,7 +19,7 @@ int it_tree_tc_weigh(const TaParams& p, int type, int nb, int nr, const CUtensor
 
 namespace {
 
-constexpr int TA_KEYS = 128, TA_MAXROWS = 256, TA_WORDS = TA_MAXROWS / 32;       // slots of a tile; rows of a call
+constexpr int TA_KEYS = 128, TA_MAXROWS = 256, TA_WORDS = TA_MAXROWS / 32, TA_MAXSPLITS = 148;       // slots of a tile; rows of a call; runs of a cache, one an SM
 constexpr float TA_LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -76,14 +76,6 @@ __device__ __forceinline__ void ta_ancestors(unsigned (*anc)[TA_WORDS], int* jum
 
 // Row t of product row r: r / group, by a product (exact: r < 2^18, group <= 2^10).
 __device__ __forceinline__ int ta_row(const TaParams& p, int r) { return p.group == 1 ? r : (int)__umulhi((unsigned)r, p.group_inv); }
-
-// The output gate on four neighbouring elements.
-template <class TA> __device__ __forceinline__ void ta_gate(const TaParams& p, int t, int h, int c, float (&v)[4]) {
-    if (!p.gate) return;
-    float z[4]; load4((const TA*)p.gate + t * p.g_row + h * p.g_head + c, z);
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] /= 1.f + __expf(-z[i]);
-}
 
 // Eight elements of a product row per lane; halves(): as f16 or bf16, for f32 activations the high and low halves, and the factor from products with them to log2 of the
 // exponential.

@@ -6,33 +6,39 @@
 //   K and V tiles   128 slots as boxes of 64 elements of a tensor map, 128-byte swizzle: K is read K-major, V (as V^T) MN-major
 //   Q               rows of 128-byte pieces, K-major; f32 activations as two sets of columns, high and low halves, added in f32 when they are read
 //   P               [slot][column], MN-major: a thread has one slot (a lane of tensor memory) and stores its columns as 16-byte pieces
-// Warps 0-7 (two groups of four; a group has half of the columns): scores out of tensor memory, exponentials against a reference that moves only when
+// Softmax warps (two or four groups of four; a group has its share of the columns): scores out of tensor memory, exponentials against a reference that moves only when
 // it has to (redux over the slots of a warp, an ordered atomicMax over the four), P; then the tile before: O^T out of tensor memory into f32 accumulators in registers.  Every tile's product starts from zero and is
 // added with a rounded f32 addition: chained over a long run in tensor memory the hardware's truncating accumulation loses f32's last bits (1.3e-5 of the result after 240 tiles of 64
-// slots chained in mma.sync accumulators).  Warps 8 and 10: copies.  Warp 9: issues whichever product has its inputs, the next tile's scores or this tile's O.
+// slots chained in mma.sync accumulators).  Two warps copy, one issues whichever product has its inputs, the next tile's scores or this tile's O.
 // What bounds it: 64 columns of f32 activations (128 with the low halves) 2 x 1024 tensor cycles a tile of 128 slots at head dimension 256; few columns: HBM.
 #include "it_tree_attention.cuh"
 
 namespace {
 
-constexpr int TC_THREADS = 384, TC_SOFT = 256;
 constexpr int TC_SMEM_LIMIT = 227 * 1024, TC_SMALL = 3072, TC_SLOTS_MAX = 6;
-constexpr int TC_SOFT_REGS = 216, TC_OTHER_REGS = 72;       // 216 x 256 + 72 x 128 = 64,512 = 168 x 384
 constexpr float TC_SHIFT = 6.f, TC_TOP = 15.f;              // p is 2^6 at the reference and may grow to 2^15 before the reference moves
 
 template <bool SPLIT, int NB, int NR> struct TcTree {
-    static constexpr int NC = NR * (SPLIT ? 2 : 1), NCB = NC > 64 ? 2 : 1, RW = NR / 2;       // columns of a product, 64-column blocks of P, product rows of a warp group
+    static constexpr int NC = NR * (SPLIT ? 2 : 1), NCB = NC > 64 ? 2 : 1;                    // columns of a product, 64-column blocks of P
     static constexpr int HD = 64 * NB, MT = NB / 2;                                           // M tiles of O^T
-    static constexpr int OR = MT == 2 ? NR : RW;                                              // accumulators of a thread: one element of d, this many product rows
-    static constexpr int QB = NB * NC * 128, PB = NCB * TA_KEYS * 128, SLOT = NB * TA_KEYS * 128, BOX = TA_KEYS * 128;
+    // Groups of four softmax warps, and product rows of one.  Four groups for 32 rows and more: a thread's share of a tile is unrolled code that runs a few times, at the speed of
+    // instruction-cache misses, and half the rows are half the code.
+    static constexpr int WGS = NR >= 32 ? 4 : 2, RW = NR / WGS, SOFT = 128 * WGS, THREADS = SOFT + 128;
+    static constexpr int OR = MT == 2 ? 2 * NR / WGS : RW;                                    // accumulators of a thread: one element of d, this many product rows
+    // setmaxnreg deals out the launch's registers: 216 x 256 + 72 x 128 = 168 x 384; 104 x 512 + 64 x 128 = 96 x 640
+    static constexpr int REGS = WGS == 2 ? 168 : 96, SOFT_REGS = WGS == 2 ? 216 : 104, OTHER_REGS = WGS == 2 ? 72 : 64;
+    static constexpr int QB = NB * NC * 128, PB = NCB * TA_KEYS * 128, BOX = TA_KEYS * 128, SLOT = NB * BOX;
     static constexpr int FIT = (TC_SMEM_LIMIT - TC_SMALL - QB - PB) / SLOT, SLOTS = FIT < TC_SLOTS_MAX ? FIT : TC_SLOTS_MAX;
     static constexpr int KS = (SLOTS + 1) / 2, VS = SLOTS - KS;
     static constexpr int Q = 0, P = QB, KR = P + PB, VR = KR + KS * SLOT, SMALL = VR + VS * SLOT, TOTAL = SMALL + TC_SMALL;
     // offsets from SMALL
-    static constexpr int BARS = 0, TMEM = 256, FLAG = 272, MAXES = 512, BASE = 1024, CORR = 1280, FAC = 2048, TROW = 2304;
+    static constexpr int BARS = 0, TMEM = 512, FLAG = 528, MAXES = 576, BASE = 1088, CORR = 1344, FAC = 2112, TROW = 2368;
     static constexpr int TCOLS = 2 * NC + MT * NC, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
-    static_assert(VS >= 1 && NR % 16 == 0 && NC <= 128 && NR <= 64 && NC % 16 == 0, "");
+    static_assert(VS >= 1 && NR % 16 == 0 && NC <= 128 && NR <= 64 && NC % 16 == 0 && RW % 8 == 0, "");
+    static_assert((2 * KS * NB + 2 * VS * MT + 6) * 8 <= TMEM, "");
+    static_assert(SOFT_REGS * SOFT + OTHER_REGS * 128 <= REGS * THREADS, "");
     static_assert(PB >= TA_MAXROWS * TA_WORDS * 4 + TA_MAXROWS * 4, "the ancestors are worked out in P's place");
+    static_assert(KS * SLOT >= NR * TA_KEYS * 4 && KS * SLOT >= NR * HD * 4, "sums and accumulators go through K's place");
 };
 
 // Shared-memory descriptors, 128-byte swizzle, version 1.  K-major: 8-row groups 1024 bytes apart.  MN-major: blocks of 64 elements `block` bytes apart, groups of 8 along K 1024 bytes apart.
@@ -50,6 +56,21 @@ template <class T> __host__ __device__ constexpr unsigned idesc(int n, bool mn) 
 __device__ __forceinline__ void mma_f16(unsigned d, unsigned long long a, unsigned long long b, unsigned id, bool acc) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
                  :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(acc ? 1u : 0u), "r"(0u) : "memory");
+}
+// The bounded waits of it_pipe.cuh with their retries rolled up: the kernel has a dozen of them, and what matters here is how much code lies between its parts.
+__device__ __forceinline__ bool tc_wait(unsigned bar, unsigned parity, volatile int* abort_flag, int* status, int site) {
+    if (mbar_test(bar, parity)) return true;
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!mbar_test_hint(bar, parity, IT_MBAR_SLEEP_NS)) {
+        if (*abort_flag) return false;
+        if (clock64() - t0 > WAIT_CLOCKS) { if (!*abort_flag) atomicExch(status, site); *abort_flag = 1; return false; }
+    }
+    return true;
+}
+// For a warp that goes on as one: true in every lane or in none.
+__device__ __forceinline__ bool tc_wait_warp(unsigned bar, unsigned parity, volatile int* abort_flag, int* status, int site) {
+    return __all_sync(0xffffffffu, tc_wait(bar, parity, abort_flag, status, site));
 }
 __device__ __forceinline__ void commit_to(unsigned bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory"); }
 __device__ __forceinline__ bool elect_one() {
@@ -86,18 +107,19 @@ __device__ __forceinline__ int ordered(float v) { const int i = __float_as_int(v
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
 template <int N> __device__ __forceinline__ void warp_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N> __device__ __forceinline__ void warp_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
-// Barriers of one group of four warps (wg 0 or 1), and of both.
+// Barriers of one group of four warps, and of all WGS groups.  The numbers are constants: a barrier whose number is a register makes the compiler reserve all sixteen.
 __device__ __forceinline__ void group_sync(int wg) {
-    if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else asm volatile("bar.sync 2, 128;" ::: "memory");
+    if (wg == 0) asm volatile("bar.sync 1, 128;" ::: "memory"); else if (wg == 1) asm volatile("bar.sync 2, 128;" ::: "memory");
+    else if (wg == 2) asm volatile("bar.sync 3, 128;" ::: "memory"); else asm volatile("bar.sync 4, 128;" ::: "memory");
 }
+template <int WGS> __device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 5, %0;" :: "n"(128 * WGS) : "memory"); }
 // Whether any thread of a group says so, with a barrier of the group.
-__device__ __forceinline__ bool group_any(int wg, bool q) {
+template <int N> __device__ __forceinline__ unsigned group_or(unsigned q) {
     unsigned r;
-    if (wg == 0) asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbarrier.cta.red.or.pred p, 1, 128, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r) : "r"(q ? 1u : 0u) : "memory");
-    else asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbarrier.cta.red.or.pred p, 2, 128, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r) : "r"(q ? 1u : 0u) : "memory");
-    return r != 0;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 q, %1, 0;\nbarrier.cta.red.or.pred p, %2, 128, q;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r) : "r"(q), "n"(N) : "memory");
+    return r;
 }
-__device__ __forceinline__ void groups_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
+__device__ __forceinline__ bool group_any(int wg, bool q) { return (wg == 0 ? group_or<1>(q) : wg == 1 ? group_or<2>(q) : wg == 2 ? group_or<3>(q) : group_or<4>(q)) != 0; }
 
 // Product rows [r0, r0 + NR) of KV head g as columns of Q^T; for each the factor from the product to log2 of its exponential, and its row t (rows behind the last: the
 // last one's).  A warp has all of its rows' loads under way at once: one after the other they were 7 us of a 64-row tile.
@@ -136,67 +158,77 @@ __device__ __noinline__ bool tc_walk(const int* parents, int t, int i) {
 }
 
 template <class T, bool SPLIT, int NB, int NR>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __launch_bounds__(TcTree<SPLIT, NB, NR>::THREADS, 1)
 k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TaParams p) {
     using L = TcTree<SPLIT, NB, NR>;
     using TA = typename std::conditional<SPLIT, float, T>::type;
-    constexpr int NC = L::NC, RW = L::RW, OR = L::OR, HD = L::HD, KS = L::KS, VS = L::VS;
+    constexpr int NC = L::NC, RW = L::RW, OR = L::OR, HD = L::HD, KS = L::KS, VS = L::VS, WGS = L::WGS, MT = L::MT, W0 = 4 * WGS;       // W0: the first warp behind the softmax warps
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, g = blockIdx.y, r0 = blockIdx.z * NR;
     unsigned char* const small = smem + L::SMALL;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(small + L::FLAG);
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(small + L::TMEM);
-    int* maxes = reinterpret_cast<int*>(small + L::MAXES);              // [2][2][32]
+    int* maxes = reinterpret_cast<int*>(small + L::MAXES);              // [2][NR]
     float* base_s = reinterpret_cast<float*>(small + L::BASE);          // [NR]
     float* corr_s = reinterpret_cast<float*>(small + L::CORR);          // [3][NR]
     float* fac = reinterpret_cast<float*>(small + L::FAC);              // [NR]
     int* trow = reinterpret_cast<int*>(small + L::TROW);                // [NR]
     const unsigned bars = smem_u32(small + L::BARS);
-    const unsigned kfull = bars, kempty = kfull + 8 * KS, vfull = kempty + 8 * KS, vempty = vfull + 8 * VS, sfull = vempty + 8 * VS, sfree = sfull + 16, pfull = sfree + 16, ofull = pfull + 8;
+    // K in boxes of 64 elements, V in pairs of them (an M tile of O^T): each has barriers of its own, so that the next tile's first box is asked for when this tile's is read
+    const unsigned kfull = bars, kempty = kfull + 8 * KS * NB, vfull = kempty + 8 * KS * NB, vempty = vfull + 8 * VS * MT, sfull = vempty + 8 * VS * MT, sfree = sfull + 16, pfull = sfree + 16, ofull = pfull + 8;
     const unsigned kring = smem_u32(smem + L::KR), vring = smem_u32(smem + L::VR);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TA_KEYS - 1) / TA_KEYS;
     // this run's tiles: the first `tiles % splits` runs have one more
     const int per = (int)((unsigned)tiles / (unsigned)p.splits), more = tiles - per * p.splits, tile0 = split * per + min(split, more), n = per + (split < more ? 1 : 0);
-    // Tile i of K (v = 0) or V, when its slot is free; copies of K and V have a warp each, since they wait for different products.
-    auto load = [&](int v, int i) {
-        const int s = i % (v ? VS : KS);
-        const unsigned dst = (v ? vring : kring) + s * L::SLOT, bar = (v ? vfull : kfull) + 8 * s;
-        mbar_expect_tx(bar, L::SLOT);
-#pragma unroll
-        for (int b = 0; b < NB; b++) tma_load_3d(dst + b * L::BOX, v ? &vmap : &kmap, 64 * b, (tile0 + i) * TA_KEYS, g, bar);
+    // Box b of tile i of K, pair m of tile i of V, when their places are free; copies of K and V have a warp each, since they wait for different products.
+    auto load_k = [&](int i, int b) {
+        const unsigned at = (unsigned)(i % KS * NB + b);
+        mbar_expect_tx(kfull + 8 * at, L::BOX);
+        tma_load_3d(kring + at * L::BOX, &kmap, 64 * b, (tile0 + i) * TA_KEYS, g, kfull + 8 * at);
     };
-    if (warp == 8 && lane == 0) {
+    auto load_v = [&](int i, int m) {
+        const unsigned at = (unsigned)(i % VS * MT + m);
+        mbar_expect_tx(vfull + 8 * at, 2 * L::BOX);
+        tma_load_3d(vring + 2 * at * L::BOX, &vmap, 128 * m, (tile0 + i) * TA_KEYS, g, vfull + 8 * at);
+        tma_load_3d(vring + (2 * at + 1) * L::BOX, &vmap, 128 * m + 64, (tile0 + i) * TA_KEYS, g, vfull + 8 * at);
+    };
+    if (warp == W0 && lane == 0) {
         *abort_flag = (smem_u32(smem) & 1023u) != 0;                 // the swizzle counts on it; never seen
-        for (int s = 0; s < KS; s++) { mbar_init(kfull + 8 * s, 1); mbar_init(kempty + 8 * s, 1); }
-        for (int s = 0; s < VS; s++) { mbar_init(vfull + 8 * s, 1); mbar_init(vempty + 8 * s, 1); }
-        for (int s = 0; s < 2; s++) { mbar_init(sfull + 8 * s, 1); mbar_init(sfree + 8 * s, 8); }
-        mbar_init(pfull, 8); mbar_init(ofull, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 #pragma unroll 1
-        for (int i = 0; i < 2 * min(n, KS); i++) if (!(i & 1) || i / 2 < VS) load(i & 1, i >> 1);        // the first tiles before anything else
+        for (int s = 0; s < 2 * (KS * NB + VS * MT); s++) mbar_init(bars + 8 * s, 1);
+        for (int s = 0; s < 2; s++) { mbar_init(sfull + 8 * s, 1); mbar_init(sfree + 8 * s, W0); }
+        mbar_init(pfull, W0); mbar_init(ofull, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // the first tile before anything else
+        if (n > 0) {
+#pragma unroll 1
+            for (int b = 0; b < NB; b++) load_k(0, b);
+#pragma unroll 1
+            for (int m = 0; m < MT; m++) load_v(0, m);
+        }
     }
-    if (warp == 9) {
+    if (warp == W0 + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)L::ALLOC) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (tid < 128) maxes[tid] = ordered(-INFINITY);
+    if (tid < 2 * NR) maxes[tid] = ordered(-INFINITY);
     __syncwarp();
-    tc_load_q<T, SPLIT, NB, NR, TC_THREADS / 32>(p, smem + L::Q, fac, trow, g, r0, warp, lane);
+    tc_load_q<T, SPLIT, NB, NR, L::THREADS / 32>(p, smem + L::Q, fac, trow, g, r0, warp, lane);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // Q before the products read it
     fence_before();
     __syncthreads();
     fence_after();
     const unsigned tmem = *tmem_slot, otm = tmem + 2 * NC;
 
-    if (warp < 8) {
-        warp_regs_inc<TC_SOFT_REGS>();
+    if (warp < W0) {
+        warp_regs_inc<L::SOFT_REGS>();
         const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
         const unsigned lanes = (unsigned)(quad * 32) << 16;
-        const int orow = L::MT == 2 ? 0 : wg * RW, d = (L::MT == 2 ? wg * 128 : 0) + key;        // first product row of the accumulators, their element of the head
-        const unsigned oaddr = otm + lanes + (L::MT == 2 ? wg * NC : 0) + orow;
+        const int mt = MT == 2 ? wg & 1 : 0, orow = MT == 2 ? (wg >> 1) * OR : wg * RW, d = mt * 128 + key;        // M tile and first product row of the accumulators, their element of the head
+        const unsigned oaddr = otm + lanes + mt * NC + orow;
         float acc[OR], l[RW], mrun = -INFINITY;                     // mrun: the running maximum of row `lane` of the group
 #pragma unroll
         for (int r = 0; r < OR; r++) acc[r] = 0.f;
@@ -208,7 +240,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
         unsigned vis[3] = { 0, 0, 0 };
         if (n > first_masked && n > 0) {
             unsigned (*anc)[TA_WORDS] = reinterpret_cast<unsigned (*)[TA_WORDS]>(smem + L::P);
-            if (p.parents) ta_ancestors<TC_SOFT>(anc, reinterpret_cast<int*>(smem + L::P + TA_MAXROWS * TA_WORDS * 4), p.parents, p.rows, tid, [] { groups_sync(); });
+            if (p.parents) ta_ancestors<L::SOFT>(anc, reinterpret_cast<int*>(smem + L::P + TA_MAXROWS * TA_WORDS * 4), p.parents, p.rows, tid, [] { groups_sync<WGS>(); });
 #pragma unroll
             for (int k = 0; k < 3; k++) {
                 if (first_masked + k >= n) break;
@@ -223,16 +255,37 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 }
                 vis[k] = m;
             }
-            groups_sync();                                          // before P takes the place of the ancestors
+            groups_sync<WGS>();                                     // before P takes the place of the ancestors
         }
         int exact = 0;                                              // references moved so far
+        auto collect = [&](int i) {                                 // O^T of tile i
+            ok = ok && tc_wait_warp(ofull, (unsigned)i & 1u, abort_flag, p.status, 52);
+            ok = ok && tc_wait_warp(pfull, (unsigned)i & 1u, abort_flag, p.status, 53);      // met long ago: the other groups' factors are seen through it
+            fence_after();
+            const float* const c = corr_s + (i % 3) * NR + orow;
+            constexpr int CH = OR < 16 ? OR : 16;
+#pragma unroll
+            for (int k = 0; k < OR; k += CH) {
+                float u[CH], v[SPLIT ? CH : 1];
+                tm_ld(u, oaddr + k);
+                if constexpr (SPLIT) tm_ld(v, oaddr + NR + k);
+                tm_wait(u);
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int e = 0; e < CH; e++) { asm volatile("" : "+f"(v[e])); u[e] += v[e]; }
+                }
+#pragma unroll
+                for (int e = 0; e < CH; e++) acc[k + e] = fmaf(acc[k + e], c[k + e], u[e]);
+            }
+            fence_before();
+        };
 #pragma unroll 1
         for (int i = 0; i <= n; i++) {                              // softmax of tile i, O^T of tile i - 1, P of tile i
             unsigned hi[RW / 2], lo[SPLIT ? RW / 2 : 1];
             const bool masked = i >= first_masked;
             if (i < n) {
                 const int buf = i & 1;
-                ok = ok && mbar_wait_warp(sfull + 8 * buf, (unsigned)(i >> 1) & 1u, abort_flag, p.status, 51);
+                ok = ok && tc_wait_warp(sfull + 8 * buf, (unsigned)(i >> 1) & 1u, abort_flag, p.status, 51);
                 fence_after();
                 float x[RW];
                 const unsigned sa = tmem + lanes + buf * NC + wg * RW;
@@ -268,7 +321,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                         const float m = warp_max(x[r]);
                         if (lane == r) mine = m;
                     }
-                    int* const best = maxes + ((exact & 1) * 2 + wg) * 32;
+                    int* const best = maxes + (exact & 1) * NR + wg * RW;
                     exact++;
                     if (lane < RW) atomicMax(best + lane, ordered(fmaxf(mrun, mine)));
                     group_sync(wg);
@@ -290,32 +343,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     if constexpr (SPLIT) { const float2 h = Ta16<T>::unpack(hi[r / 2]); lo[r / 2] = Ta16<T>::pack(a - h.x, b - h.y); }
                 }
             }
-            if (i > 0) {                                            // O^T of tile i - 1: frees it and P
-                ok = ok && mbar_wait_warp(ofull, (unsigned)(i - 1) & 1u, abort_flag, p.status, 52);
-                ok = ok && mbar_wait_warp(pfull, (unsigned)(i - 1) & 1u, abort_flag, p.status, 53);      // met long ago: the other group's factors are seen through it
-                fence_after();
-                const float* const c = corr_s + ((i - 1) % 3) * NR + orow;
-                constexpr int CH = 8, NCH = OR / CH;
-                float a[2][CH], b[2][CH];
-                tm_ld(a[0], oaddr);
-                if constexpr (SPLIT) tm_ld(b[0], oaddr + NR);
-#pragma unroll
-                for (int k = 0; k < NCH; k++) {                     // the next columns are on their way while these are added
-                    float (&u)[CH] = a[k & 1], (&v)[CH] = b[k & 1];
-                    tm_wait(u);
-                    if constexpr (SPLIT) {
-#pragma unroll
-                        for (int e = 0; e < CH; e++) asm volatile("" : "+f"(v[e]));
-                    }
-                    if (k + 1 < NCH) {
-                        tm_ld(a[(k + 1) & 1], oaddr + (k + 1) * CH);
-                        if constexpr (SPLIT) tm_ld(b[(k + 1) & 1], oaddr + NR + (k + 1) * CH);
-                    }
-#pragma unroll
-                    for (int e = 0; e < CH; e++) acc[k * CH + e] = fmaf(acc[k * CH + e], c[k * CH + e], SPLIT ? u[e] + v[e] : u[e]);
-                }
-                fence_before();
-            }
+            if (i > 0) collect(i - 1);                               // frees O^T and P
             if (i == n) break;
             unsigned char* const prow = smem + L::P + key * 128;
 #pragma unroll
@@ -328,7 +356,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             if (masked) {
                 // V elements that are not finite leave the product and go to the rows that see their slot
                 const int j0 = (tile0 + i) * TA_KEYS, from = max(cached - j0, 0), to = min(TA_KEYS, p.cached + p.rows - j0);
-                ok = ok && mbar_wait_warp(vfull + 8 * (i % VS), (unsigned)(i / VS) & 1u, abort_flag, p.status, 54);
+                ok = ok && tc_wait_warp(vfull + 8 * (i % VS * MT + mt), (unsigned)(i / VS) & 1u, abort_flag, p.status, 54);
                 unsigned char* const v = smem + L::VR + (i % VS) * L::SLOT + (d >> 6) * L::BOX + (d & 7) * 2;
                 bool any = false;
 #pragma unroll 1
@@ -344,8 +372,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
                     for (int r = 0; r < OR; r++) if ((rows >> r) & 1ull) acc[r] += bad;
                 }
-                if (L::MT == 1) groups_sync();              // both groups have looked at the elements that one of them clears
-                if (any && (L::MT == 2 || wg == 0))
+                groups_sync<WGS>();                         // all groups have looked at the elements that one of them clears
+                if (any && orow == 0)
 #pragma unroll 1
                     for (int k = from; k < to; k++) {
                         unsigned short* e = reinterpret_cast<unsigned short*>(v + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4));
@@ -378,17 +406,17 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             float* const o = p.part_o + (at + orow) * HD + d;
 #pragma unroll
             for (int r = 0; r < OR; r++) if (r0 + orow + r < p.prows) __stcg(o + r * HD, acc[r]);
-            groups_sync();
+            groups_sync<WGS>();
             if (tid < NR) p.part_ml[at + tid] = ml[tid];
         } else {
             // through shared memory, so that a loop can write whole rows, four elements a thread
             float* const os = reinterpret_cast<float*>(smem + L::KR);          // [NR][HD], where the sums were
-            groups_sync();
+            groups_sync<WGS>();
 #pragma unroll
             for (int r = 0; r < OR; r++) os[(orow + r) * HD + d] = acc[r];
-            groups_sync();
+            groups_sync<WGS>();
             if (p.stats && tid < NR) p.stats[(size_t)g * p.pad_rows + r0 + tid] = make_float2(ml[tid].x == -INFINITY ? 0.f : ml[tid].x, ml[tid].y);
-            constexpr int LN = HD / 4, STEP = TC_SOFT / LN, U = 4;              // threads of a row, rows at once, rows of a thread whose gates are on their way together
+            constexpr int LN = HD / 4, STEP = L::SOFT / LN, U = 4;              // threads of a row, rows at once, rows of a thread whose gates are on their way together
             const int c = tid % LN * 4;
 #pragma unroll 1
             for (int q = tid / LN; q < NR && c < p.dim; q += U * STEP) {
@@ -415,58 +443,85 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
         }
     } else {
-        warp_regs_dec<TC_OTHER_REGS>();
-        if (warp == 8 || warp == 10) {
-            // ---------------- copies of K, and of V
+        warp_regs_dec<L::OTHER_REGS>();
+        // Leaving after a wait that ran out: only when every copy has landed (bounded).
+        auto landed = [&](unsigned full, int from, int to, int ring) {
+#pragma unroll 1
+            for (int k = max(from, to - ring); k < to; k++) { const long long t0 = clock64(); while (!mbar_test(full + 8 * (k % ring), (unsigned)(k / ring) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
+        };
+        if (warp == W0) {
+            // ---------------- copies of K
             if (lane == 0) {
-                const int v = warp == 10, ring = v ? VS : KS;
-                const unsigned full = v ? vfull : kfull, empty = v ? vempty : kempty;
-                int i = min(n, min(KS, ring));          // asked for already
-                for (; i < n; i++) {
-                    if (i >= ring && !mbar_wait(empty + 8 * (i % ring), ((unsigned)(i / ring) & 1u) ^ 1u, abort_flag, p.status, 55)) break;
-                    load(v, i);
+                int k = NB;                         // boxes asked for
+#pragma unroll 1
+                for (; k < n * NB; k++) {
+                    if (k >= KS * NB && !tc_wait(kempty + 8 * (k % (KS * NB)), ((unsigned)(k / (KS * NB)) & 1u) ^ 1u, abort_flag, p.status, 55)) break;
+                    load_k(k / NB, k % NB);
                 }
-                if (*abort_flag)                        // leave only after every copy has landed (bounded)
-                    for (int k = i > ring ? i - ring : 0; k < i; k++) { const long long t0 = clock64(); while (!mbar_test(full + 8 * (k % ring), (unsigned)(k / ring) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
+                if (*abort_flag && n > 0) landed(kfull, 0, k, KS * NB);
             }
-        } else if (warp == 9) {
-            // ---------------- products: the scores of tile si, O^T of tile oi, whichever has its inputs
+        } else if (warp == W0 + 2) {
+            // ---------------- copies of V
+            if (lane == 0) {
+                int k = MT;
+#pragma unroll 1
+                for (; k < n * MT; k++) {
+                    if (k >= VS * MT && !tc_wait(vempty + 8 * (k % (VS * MT)), ((unsigned)(k / (VS * MT)) & 1u) ^ 1u, abort_flag, p.status, 56)) break;
+                    load_v(k / MT, k % MT);
+                }
+                if (*abort_flag && n > 0) landed(vfull, 0, k, VS * MT);
+            }
+        } else if (warp == W0 + 1) {
+            // ---------------- products: the scores of tile si, O^T of tile oi, whichever has its inputs.  Loops, not straight code: see WGS.
             if (elect_one()) {
                 const unsigned long long qd = desc_k(smem_u32(smem + L::Q)), pd = desc_mn(smem_u32(smem + L::P), L::BOX);
-                int si = 0, oi = 0; long long since = clock64();
-                while (oi < n) {
-                    if (si < n && mbar_poll(kfull + 8 * (si % KS), (unsigned)(si / KS) & 1u) && mbar_poll(sfree + 8 * (si & 1), ((unsigned)(si >> 1) & 1u) ^ 1u)) {
-                        fence_after();
-                        const unsigned long long kd = desc_k(kring + (si % KS) * L::SLOT);
+                int si = 0, oi = 0; long long since = clock64(); bool ok = true;
+#pragma unroll 1
+                while (ok && oi < n) {
+                    if (si < n && mbar_poll(sfree + 8 * (si & 1), ((unsigned)(si >> 1) & 1u) ^ 1u) && mbar_poll(kfull + 8 * (si % KS * NB), (unsigned)(si / KS) & 1u)) {
+#pragma unroll 1
+                        for (int b = 0; b < NB; b++) {
+                            const unsigned at = (unsigned)(si % KS * NB + b);
+                            ok = tc_wait(kfull + 8 * at, (unsigned)(si / KS) & 1u, abort_flag, p.status, 57);
+                            if (!ok) break;
+                            fence_after();
+                            const unsigned long long kd = desc_k(kring + at * L::BOX), qb = qd + (unsigned)(b * NC * 128 >> 4);
 #pragma unroll
-                        for (int k = 0; k < 4 * NB; k++)             // 16 elements of the head a step
-                            mma_f16(tmem + (si & 1) * NC, kd + (unsigned)(((k >> 2) * L::BOX + (k & 3) * 32) >> 4), qd + (unsigned)(((k >> 2) * NC * 128 + (k & 3) * 32) >> 4), idesc<T>(NC, false), k > 0);
-                        commit_to(sfull + 8 * (si & 1)); commit_to(kempty + 8 * (si % KS));
-                        si++; since = clock64();
-                    } else if (oi < si && mbar_poll(pfull, (unsigned)oi & 1u) && mbar_poll(vfull + 8 * (oi % VS), (unsigned)(oi / VS) & 1u)) {
-                        fence_after();
-#pragma unroll
-                        for (int m = 0; m < L::MT; m++) {
-                            const unsigned long long vd = desc_mn(vring + (oi % VS) * L::SLOT + m * 2 * L::BOX, L::BOX);
-#pragma unroll
-                            for (int k = 0; k < TA_KEYS / 16; k++)   // 16 slots a step
-                                mma_f16(otm + m * NC, vd + (unsigned)(k * 2048 >> 4), pd + (unsigned)(k * 2048 >> 4), idesc<T>(NC, true), k > 0);
+                            for (int k = 0; k < 4; k++) mma_f16(tmem + (si & 1) * NC, kd + (unsigned)(k * 32 >> 4), qb + (unsigned)(k * 32 >> 4), idesc<T>(NC, false), b + k > 0);     // 16 elements of the head a step
+                            commit_to(kempty + 8 * at);
                         }
-                        commit_to(ofull); commit_to(vempty + 8 * (oi % VS));
+                        if (ok) commit_to(sfull + 8 * (si & 1));
+                        si++; since = clock64();
+                    } else if (oi < si && mbar_poll(pfull, (unsigned)oi & 1u)) {
+#pragma unroll 1
+                        for (int m = 0; m < MT; m++) {
+                            const unsigned at = (unsigned)(oi % VS * MT + m);
+                            ok = tc_wait(vfull + 8 * at, (unsigned)(oi / VS) & 1u, abort_flag, p.status, 58);
+                            if (!ok) break;
+                            fence_after();
+                            unsigned long long vd = desc_mn(vring + 2 * at * L::BOX, L::BOX), pb = pd;
+#pragma unroll 1
+                            for (int k = 0; k < TA_KEYS / 16; k += 4) {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) mma_f16(otm + m * NC, vd + (unsigned)(j * 2048 >> 4), pb + (unsigned)(j * 2048 >> 4), idesc<T>(NC, true), k + j > 0);          // 16 slots a step
+                                vd += (unsigned)(4 * 2048 >> 4); pb += (unsigned)(4 * 2048 >> 4);
+                            }
+                            commit_to(vempty + 8 * at);
+                        }
+                        if (ok) commit_to(ofull);
                         oi++; since = clock64();
                     } else if (*abort_flag) break;
-                    else if (clock64() - since > WAIT_CLOCKS) { if (!*abort_flag) atomicExch(p.status, 57); *abort_flag = 1; break; }
+                    else if (clock64() - since > WAIT_CLOCKS) { if (!*abort_flag) atomicExch(p.status, 59); *abort_flag = 1; break; }
                 }
                 // the last commits must find the CTA's shared memory still its own (bounded)
-                if (si > 0) { const long long t0 = clock64(); while (!mbar_test(kempty + 8 * ((si - 1) % KS), (unsigned)((si - 1) / KS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
-                if (oi > 0) { const long long t0 = clock64(); while (!mbar_test(vempty + 8 * ((oi - 1) % VS), (unsigned)((oi - 1) / VS) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
+                landed(kempty, 0, si * NB, KS * NB); landed(vempty, 0, oi * MT, VS * MT);
             }
         }
     }
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == W0 + 1) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((unsigned)L::ALLOC) : "memory");
     }
@@ -475,6 +530,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 // ---- received weight --------------------------------------------------------------------------------------------------------
 // The scores of a 128-slot tile once more, against the finished maximum and sum of every product row: a thread has a slot and adds up its columns, so that nothing crosses
 // threads but the two groups' halves.  The CTA walks the product rows, NR at a time; the next ones are brought in while the last ones' exponentials are formed.
+constexpr int TW_THREADS = 256;
 template <bool SPLIT, int NB, int NR> struct TcWeights {
     using A = TcTree<SPLIT, NB, NR>;
     static constexpr int Q = 0, K = A::QB, ANC = K + A::SLOT, JUMP = ANC + TA_MAXROWS * TA_WORDS * 4, ROW = JUMP + TA_MAXROWS * 4, HALF = ROW + 3 * 4 * NR * 4, BARS = HALF + TA_KEYS * 4, TMEM = BARS + 32, FLAG = TMEM + 16,
@@ -482,11 +538,11 @@ template <bool SPLIT, int NB, int NR> struct TcWeights {
     static constexpr int ALLOC = 2 * A::NC < 32 ? 32 : 2 * A::NC;
 };
 template <class T, bool SPLIT, int NB, int NR>
-__global__ void __launch_bounds__(TC_SOFT)
+__global__ void __launch_bounds__(TW_THREADS)
 k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ TaParams p) {
     using L = TcTree<SPLIT, NB, NR>;
     using W = TcWeights<SPLIT, NB, NR>;
-    constexpr int NC = L::NC, RW = L::RW;
+    constexpr int NC = L::NC, RW = NR / 2;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tile = blockIdx.x, g = blockIdx.y;
     const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
@@ -509,12 +565,12 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     const bool masked = (tile + 1) * TA_KEYS > cached;
-    if (masked && p.parents) ta_ancestors<TC_SOFT>(anc, reinterpret_cast<int*>(smem + W::JUMP), p.parents, p.rows, tid, [] { __syncthreads(); });
+    if (masked && p.parents) ta_ancestors<TW_THREADS>(anc, reinterpret_cast<int*>(smem + W::JUMP), p.parents, p.rows, tid, [] { __syncthreads(); });
     asm volatile("griddepcontrol.wait;" ::: "memory");                // the statistics come from the kernel before
     const int steps = (p.prows + NR - 1) / NR;
     auto bring = [&](int i) {                                         // product rows of step i, and their statistics
         float* const rw = row + (i % 3) * 4 * NR;
-        tc_load_q<T, SPLIT, NB, NR, TC_SOFT / 32>(p, smem + W::Q, rw, reinterpret_cast<int*>(rw + 3 * NR), g, i * NR, warp, lane);
+        tc_load_q<T, SPLIT, NB, NR, TW_THREADS / 32>(p, smem + W::Q, rw, reinterpret_cast<int*>(rw + 3 * NR), g, i * NR, warp, lane);
         if (tid < NR) {
             const int r = i * NR + tid;
             const float2 st = r < p.prows ? __ldcg(&p.stats[(size_t)g * p.pad_rows + r]) : make_float2(0.f, 0.f);
@@ -538,11 +594,11 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         }
         __syncwarp();
     };
-    bool ok = mbar_wait_warp(kfull, 0, abort_flag, p.status, 61);
+    bool ok = tc_wait_warp(kfull, 0, abort_flag, p.status, 61);
     issue(0);
     float sum = 0.f;
     for (int i = 0; i < steps; i++) {
-        ok = ok && mbar_wait_warp(sfull + 8 * (i & 1), (unsigned)(i >> 1) & 1u, abort_flag, p.status, 62);
+        ok = ok && tc_wait_warp(sfull + 8 * (i & 1), (unsigned)(i >> 1) & 1u, abort_flag, p.status, 62);
         fence_after();
         if (i + 1 < steps) {                                          // the products of step i are done with Q
             bring(i + 1);
@@ -593,7 +649,8 @@ template <class T, bool SPLIT, int NB, int NR> int prepare_shape() {
     // setmaxnreg deals out the registers of the launch: a kernel compiled to fewer would wait for ever
     cudaFuncAttributes at;
     IT_CUDA(cudaFuncGetAttributes(&at, k_tree_attention_tc<T, SPLIT, NB, NR>));
-    if (at.numRegs * TC_THREADS < TC_SOFT_REGS * TC_SOFT + TC_OTHER_REGS * (TC_THREADS - TC_SOFT)) return it_fail(IT_ESTATE, "it_tree_attention: built with %d registers a thread", at.numRegs);
+    using L = TcTree<SPLIT, NB, NR>;
+    if (at.numRegs < L::REGS) return it_fail(IT_ESTATE, "it_tree_attention: built with %d registers a thread", at.numRegs);
     IT_CUDA(cudaFuncSetAttribute(k_tree_weights_tc<T, SPLIT, NB, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcWeights<SPLIT, NB, NR>::TOTAL));
     return IT_OK;
 }
@@ -605,11 +662,11 @@ template <class T, bool SPLIT, int NB> int prepare_dim() {
 template <class T, bool SPLIT> int prepare_type() { const int r = prepare_dim<T, SPLIT, 2>(); return r ? r : prepare_dim<T, SPLIT, 4>(); }
 
 template <class T, bool SPLIT, int NB, int NR> int run_shape(const TaParams& p, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
-    IT_CUDA(ta_launch(false, k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TC_THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, km, vm, p));
+    IT_CUDA(ta_launch(false, k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TcTree<SPLIT, NB, NR>::THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, km, vm, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB, int NR> int weigh_shape(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
-    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, p.kv_heads), dim3(TC_SOFT), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
+    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB> int run_dim(const TaParams& p, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
