@@ -21,6 +21,9 @@ constexpr float TC_SHIFT = 6.f, TC_TOP = 15.f;              // p is 2^6 at the r
 template <bool SPLIT, int NB, int NR> struct TcTree {
     static constexpr int NC = NR * (SPLIT ? 2 : 1), NCB = NC > 64 ? 2 : 1;                    // columns of a product, 64-column blocks of P
     static constexpr int HD = 64 * NB, MT = NB / 2;                                           // M tiles of O^T
+    // Accumulators that a score is spread over (f32 activations, where tensor memory has the columns): the hardware truncates at every step, and a chain of 16 of them
+    // cost more than half of the result's error at 16 and 32 rows (1.1e-6 of the result after 512 slots).
+    static constexpr int PARTS = !SPLIT || NR > 32 ? 1 : NR == 32 ? 2 : NB, SC = PARTS * NC;   // SC: columns of a tile's scores
     // Groups of four softmax warps, and product rows of one.  Four groups for 32 rows and more: a thread's share of a tile is unrolled code that runs a few times, at the speed of
     // instruction-cache misses, and half the rows are half the code.
     static constexpr int WGS = NR >= 32 ? 4 : 2, RW = NR / WGS, SOFT = 128 * WGS, THREADS = SOFT + 128;
@@ -33,7 +36,7 @@ template <bool SPLIT, int NB, int NR> struct TcTree {
     static constexpr int Q = 0, P = QB, KR = P + PB, VR = KR + KS * SLOT, SMALL = VR + VS * SLOT, TOTAL = SMALL + TC_SMALL;
     // offsets from SMALL
     static constexpr int BARS = 0, TMEM = 512, FLAG = 528, MAXES = 576, BASE = 1088, CORR = 1344, FAC = 2112, TROW = 2368;
-    static constexpr int TCOLS = 2 * NC + MT * NC, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
+    static constexpr int TCOLS = 2 * SC + MT * NC, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
     static_assert(VS >= 1 && NR % 16 == 0 && NC <= 128 && NR <= 64 && NC % 16 == 0 && RW % 8 == 0, "");
     static_assert((2 * KS * NB + 2 * VS * MT + 6) * 8 <= TMEM, "");
     static_assert(SOFT_REGS * SOFT + OTHER_REGS * 128 <= REGS * THREADS, "");
@@ -221,7 +224,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     fence_before();
     __syncthreads();
     fence_after();
-    const unsigned tmem = *tmem_slot, otm = tmem + 2 * NC;
+    const unsigned tmem = *tmem_slot, otm = tmem + 2 * L::SC;
 
     if (warp < W0) {
         warp_regs_inc<L::SOFT_REGS>();
@@ -288,15 +291,19 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 ok = ok && tc_wait_warp(sfull + 8 * buf, (unsigned)(i >> 1) & 1u, abort_flag, p.status, 51);
                 fence_after();
                 float x[RW];
-                const unsigned sa = tmem + lanes + buf * NC + wg * RW;
-                tm_ld(x, sa);
-                if constexpr (SPLIT) {
-                    float y[RW];
-                    tm_ld(y, sa + NR);
-                    tm_wait(x);
+                const unsigned sa = tmem + lanes + buf * L::SC + wg * RW;
+                if constexpr (SPLIT) {                              // the parts' low halves, then their high halves
+                    float y[2 * L::PARTS][RW];
 #pragma unroll
-                    for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
-                } else tm_wait(x);
+                    for (int k = 0; k < 2 * L::PARTS; k++) tm_ld(y[k], sa + (k % L::PARTS) * NC + (k < L::PARTS ? NR : 0));
+                    tm_wait(y[0]);
+#pragma unroll
+                    for (int r = 0; r < RW; r++) {
+                        x[r] = y[0][r];
+#pragma unroll
+                        for (int k = 1; k < 2 * L::PARTS; k++) { asm volatile("" : "+f"(y[k][r])); x[r] += y[k][r]; }
+                    }
+                } else { tm_ld(x, sa); tm_wait(x); }
                 fence_before();
                 __syncwarp();
                 if (lane == 0 && ok) mbar_arrive(sfree + 8 * buf);
@@ -487,7 +494,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                             fence_after();
                             const unsigned long long kd = desc_k(kring + at * L::BOX), qb = qd + (unsigned)(b * NC * 128 >> 4);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) mma_f16(tmem + (si & 1) * NC, kd + (unsigned)(k * 32 >> 4), qb + (unsigned)(k * 32 >> 4), idesc<T>(NC, false), b + k > 0);     // 16 elements of the head a step
+                            for (int k = 0; k < 4; k++) mma_f16(tmem + (si & 1) * L::SC + b * L::PARTS / NB * NC, kd + (unsigned)(k * 32 >> 4), qb + (unsigned)(k * 32 >> 4), idesc<T>(NC, false), b % (NB / L::PARTS) + k > 0);     // 16 elements of the head a step
                             commit_to(kempty + 8 * at);
                         }
                         if (ok) commit_to(sfull + 8 * (si & 1));
@@ -528,14 +535,16 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 }
 
 // ---- received weight --------------------------------------------------------------------------------------------------------
-// The scores of a 128-slot tile once more, against the finished maximum and sum of every product row: a thread has a slot and adds up its columns, so that nothing crosses
-// threads but the two groups' halves.  The CTA walks the product rows, NR at a time; the next ones are brought in while the last ones' exponentials are formed.
+// The scores of a 128-slot tile once more, against the finished reference and sum of every product row: a thread has a slot and adds up its columns, so that nothing crosses
+// threads but the two groups' halves.  A CTA walks tiles of a KV head; up to NR product rows are brought in once, more of them NR at a time for every tile.  The next scores are
+// formed while the last ones' exponentials are, and the next tile of K is on its way (one tile a CTA: 21 us at 8192 slots and 9 rows, most of it start-up).
 constexpr int TW_THREADS = 256;
 template <bool SPLIT, int NB, int NR> struct TcWeights {
     using A = TcTree<SPLIT, NB, NR>;
-    static constexpr int Q = 0, K = A::QB, ANC = K + A::SLOT, JUMP = ANC + TA_MAXROWS * TA_WORDS * 4, ROW = JUMP + TA_MAXROWS * 4, HALF = ROW + 3 * 4 * NR * 4, BARS = HALF + TA_KEYS * 4, TMEM = BARS + 32, FLAG = TMEM + 16,
-                         TOTAL = FLAG + 16;
+    static constexpr int Q = 0, K = A::QB, ANC = K + 2 * A::SLOT, JUMP = ANC + TA_MAXROWS * TA_WORDS * 4, ROW = JUMP + TA_MAXROWS * 4, HALF = ROW + 3 * 4 * NR * 4, BARS = HALF + 2 * TA_KEYS * 4, TMEM = BARS + 32,
+                         FLAG = TMEM + 16, TOTAL = FLAG + 16;
     static constexpr int ALLOC = 2 * A::NC < 32 ? 32 : 2 * A::NC;
+    static_assert(TOTAL <= TC_SMEM_LIMIT, "");
 };
 template <class T, bool SPLIT, int NB, int NR>
 __global__ void __launch_bounds__(TW_THREADS)
@@ -544,100 +553,127 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     using W = TcWeights<SPLIT, NB, NR>;
     constexpr int NC = L::NC, RW = NR / 2;
     extern __shared__ __align__(1024) unsigned char smem[];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tile = blockIdx.x, g = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = blockIdx.y;
     const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
-    const int cached = ta_cached(p), total = cached + p.rows;
-    if (tile * TA_KEYS >= total) { asm volatile("griddepcontrol.wait;" ::: "memory"); return; }
+    const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TA_KEYS - 1) / TA_KEYS;
+    const int nt = ((int)blockIdx.x < tiles) ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;      // tiles blockIdx.x, + gridDim.x, ...
+    if (nt == 0) { asm volatile("griddepcontrol.wait;" ::: "memory"); return; }
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + W::FLAG);
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(smem + W::TMEM);
-    const unsigned kfull = smem_u32(smem + W::BARS), sfull = kfull + 8;
+    const unsigned kfull = smem_u32(smem + W::BARS), sfull = kfull + 16;
     unsigned (*anc)[TA_WORDS] = reinterpret_cast<unsigned (*)[TA_WORDS]>(smem + W::ANC);
-    float* const row = reinterpret_cast<float*>(smem + W::ROW);       // [3][factor, base, 1 / sum, row t][NR]: a slow warp may still read step i - 1 while a fast one brings i + 1
-    if (tid == 0) {
-        *abort_flag = 0; mbar_init(kfull, 1); mbar_init(sfull, 1); mbar_init(sfull + 8, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        mbar_expect_tx(kfull, L::SLOT);
+    float* const row = reinterpret_cast<float*>(smem + W::ROW);       // [3][factor, base, 1 / sum, row t][NR]: a slow warp may still read step q - 1 while a fast one brings q + 1
+    auto load = [&](int j) {
+        const unsigned bar = kfull + 8 * (j & 1);
+        mbar_expect_tx(bar, L::SLOT);
 #pragma unroll
-        for (int b = 0; b < NB; b++) tma_load_3d(smem_u32(smem + W::K) + b * L::BOX, &kmap, 64 * b, tile * TA_KEYS, g, kfull);
+        for (int b = 0; b < NB; b++) tma_load_3d(smem_u32(smem + W::K) + (j & 1) * L::SLOT + b * L::BOX, &kmap, 64 * b, ((int)blockIdx.x + j * (int)gridDim.x) * TA_KEYS, g, bar);
+    };
+    if (tid == 0) {
+        *abort_flag = 0;
+        for (int k = 0; k < 4; k++) mbar_init(kfull + 8 * k, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        load(0);
+        if (nt > 1) load(1);
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)W::ALLOC) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const bool masked = (tile + 1) * TA_KEYS > cached;
-    if (masked && p.parents) ta_ancestors<TW_THREADS>(anc, reinterpret_cast<int*>(smem + W::JUMP), p.parents, p.rows, tid, [] { __syncthreads(); });
+    const int last_tile = (int)blockIdx.x + (nt - 1) * (int)gridDim.x;
+    if (p.parents && (last_tile + 1) * TA_KEYS > cached) ta_ancestors<TW_THREADS>(anc, reinterpret_cast<int*>(smem + W::JUMP), p.parents, p.rows, tid, [] { __syncthreads(); });
     asm volatile("griddepcontrol.wait;" ::: "memory");                // the statistics come from the kernel before
     const int steps = (p.prows + NR - 1) / NR;
-    auto bring = [&](int i) {                                         // product rows of step i, and their statistics
-        float* const rw = row + (i % 3) * 4 * NR;
+    auto bring = [&](int i, int q) {                                  // product rows of step i, and their statistics
+        float* const rw = row + (q % 3) * 4 * NR;
         tc_load_q<T, SPLIT, NB, NR, TW_THREADS / 32>(p, smem + W::Q, rw, reinterpret_cast<int*>(rw + 3 * NR), g, i * NR, warp, lane);
         if (tid < NR) {
             const int r = i * NR + tid;
             const float2 st = r < p.prows ? __ldcg(&p.stats[(size_t)g * p.pad_rows + r]) : make_float2(0.f, 0.f);
-            rw[NR + tid] = st.x; rw[2 * NR + tid] = st.y == 0.f ? 0.f : 1.f / st.y;
+            rw[NR + tid] = st.x; rw[2 * NR + tid] = st.y == 0.f ? 0.f : 1.f / st.y;          // rows behind the last: nothing
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     };
-    bring(0);
+    bring(0, 0);
     fence_before();
     __syncthreads();
     fence_after();
     const unsigned tmem = *tmem_slot;
-    const unsigned long long qd = desc_k(smem_u32(smem + W::Q)), kd = desc_k(smem_u32(smem + W::K));
-    auto issue = [&](int i) {
-        if (warp == 0 && elect_one()) {
-            fence_after();
+    const unsigned long long qd = desc_k(smem_u32(smem + W::Q));
+    bool ok = true;
+    auto issue = [&](int j, int q) {                                  // the scores of step q, a step of tile j
+        if (warp == 0) {
+            ok = ok && tc_wait_warp(kfull + 8 * (j & 1), (unsigned)(j >> 1) & 1u, abort_flag, p.status, 61);
+            if (elect_one()) {
+                const unsigned long long kd = desc_k(smem_u32(smem + W::K) + (j & 1) * L::SLOT);
+                fence_after();
+#pragma unroll 1
+                for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int k = 0; k < 4 * NB; k++)
-                mma_f16(tmem + (i & 1) * NC, kd + (unsigned)(((k >> 2) * L::BOX + (k & 3) * 32) >> 4), qd + (unsigned)(((k >> 2) * NC * 128 + (k & 3) * 32) >> 4), idesc<T>(NC, false), k > 0);
-            commit_to(sfull + 8 * (i & 1));
+                    for (int k = 0; k < 4; k++)
+                        mma_f16(tmem + (q & 1) * NC, kd + (unsigned)((b * L::BOX + k * 32) >> 4), qd + (unsigned)((b * NC * 128 + k * 32) >> 4), idesc<T>(NC, false), b + k > 0);
+                commit_to(sfull + 8 * (q & 1));
+            }
+            __syncwarp();
         }
-        __syncwarp();
     };
-    bool ok = tc_wait_warp(kfull, 0, abort_flag, p.status, 61);
-    issue(0);
-    float sum = 0.f;
-    for (int i = 0; i < steps; i++) {
-        ok = ok && tc_wait_warp(sfull + 8 * (i & 1), (unsigned)(i >> 1) & 1u, abort_flag, p.status, 62);
-        fence_after();
-        if (i + 1 < steps) {                                          // the products of step i are done with Q
-            bring(i + 1);
+    issue(0, 0);
+    int q = 0;
+#pragma unroll 1
+    for (int j = 0; j < nt; j++) {
+        const int tile = (int)blockIdx.x + j * (int)gridDim.x;
+        const bool masked = (tile + 1) * TA_KEYS > cached;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < steps; i++, q++) {
+            ok = ok && tc_wait_warp(sfull + 8 * (q & 1), (unsigned)(q >> 1) & 1u, abort_flag, p.status, 62);
+            fence_after();
+            const bool last = i + 1 == steps;
+            if (last && tid == 0 && j + 2 < nt && ok) load(j + 2);    // every product with this tile is done
+            if (!last || j + 1 < nt) {
+                if (steps > 1) bring(last ? 0 : i + 1, q + 1);        // the products of step q are done with Q
+                fence_before();
+                __syncthreads();                                      // everyone has read the scores of step q - 1
+                issue(last ? j + 1 : j, q + 1);
+            }
+            float x[RW];
+            const unsigned sa = tmem + ((unsigned)(quad * 32) << 16) + (q & 1) * NC + wg * RW;
+            tm_ld(x, sa);
+            if constexpr (SPLIT) {
+                float y[RW];
+                tm_ld(y, sa + NR);
+                tm_wait(x);
+#pragma unroll
+                for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
+            } else tm_wait(x);
             fence_before();
-            __syncthreads();
-            issue(i + 1);
+            const float* const rw = row + (steps > 1 ? q % 3 : 0) * 4 * NR + wg * RW;
+            if (!masked) {
+#pragma unroll
+                for (int r = 0; r < RW; r++) sum = fmaf(ex2(fmaf(x[r], rw[r], -rw[NR + r])), rw[2 * NR + r], sum);
+            } else {
+                // a masked score does not count, whatever it is; the sum of a row behind the last is 0 and its statistics are 0
+                const int t0 = tile * TA_KEYS + key;
+#pragma unroll
+                for (int r = 0; r < RW; r++) {
+                    const float e = ex2(fmaf(x[r], rw[r], -rw[NR + r])) * rw[2 * NR + r];
+                    if (ta_sees(p, anc, reinterpret_cast<const int*>(rw)[3 * NR + r], t0, cached)) sum += e;
+                }
+            }
         }
-        float x[RW];
-        const unsigned sa = tmem + ((unsigned)(quad * 32) << 16) + (i & 1) * NC + wg * RW;
-        tm_ld(x, sa);
-        if constexpr (SPLIT) {
-            float y[RW];
-            tm_ld(y, sa + NR);
-            tm_wait(x);
-#pragma unroll
-            for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
-        } else tm_wait(x);
-        fence_before();
-        const float* const rw = row + (i % 3) * 4 * NR + wg * RW;
-#pragma unroll
-        for (int r = 0; r < RW; r++) {
-            const int pr = i * NR + wg * RW + r;
-            if (pr >= p.prows || (masked && !ta_sees(p, anc, reinterpret_cast<const int*>(rw)[3 * NR + r], tile * TA_KEYS + key, cached))) continue;
-            sum += ex2(fmaf(x[r], rw[r], -rw[NR + r])) * rw[2 * NR + r];
+        float* const half = reinterpret_cast<float*>(smem + W::HALF) + (j & 1) * TA_KEYS;
+        if (wg == 1) half[key] = sum;
+        __syncthreads();
+        if (wg == 0 && tile * TA_KEYS + key < total) {
+            float* w = p.weights + (long long)g * p.w_head + tile * TA_KEYS + key;
+            *w = ok && !*abort_flag ? *w + (sum + half[key]) : NAN;
         }
     }
-    float* const half = reinterpret_cast<float*>(smem + W::HALF);
-    if (wg == 1) half[key] = sum;
     fence_before();
     __syncthreads();
-    if (wg == 0 && tile * TA_KEYS + key < total) {
-        float* w = p.weights + (long long)g * p.w_head + tile * TA_KEYS + key;
-        *w = ok && !*abort_flag ? *w + (sum + half[key]) : NAN;
-    }
     if (warp == 0) {
-        if (!ok && lane == 0) {                                       // leave only after the copy has landed (bounded)
-            const long long t0 = clock64();
-            while (!mbar_test(kfull, 0) && clock64() - t0 < WAIT_CLOCKS) { }
-        }
+        if (*abort_flag && lane == 0)                                 // leave only after the copies have landed (bounded)
+            for (int j = nt > 2 ? nt - 2 : 0; j < nt; j++) { const long long t0 = clock64(); while (!mbar_test(kfull + 8 * (j & 1), (unsigned)(j >> 1) & 1u) && clock64() - t0 < WAIT_CLOCKS) { } }
         __syncwarp();
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"((unsigned)W::ALLOC) : "memory");
@@ -666,7 +702,9 @@ template <class T, bool SPLIT, int NB, int NR> int run_shape(const TaParams& p, 
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB, int NR> int weigh_shape(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
-    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
+    // one wave of CTAs, as many tiles for each
+    const int tiles = (p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, most = p.kv_heads < TA_MAXSPLITS ? TA_MAXSPLITS / p.kv_heads : 1, rounds = (tiles + most - 1) / most;
+    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((tiles + rounds - 1) / rounds, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB> int run_dim(const TaParams& p, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
