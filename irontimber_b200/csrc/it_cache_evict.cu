@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_con
     int* ranks = p.ranks + (long long)g * p.rank_head;
     const int cand = p.n - p.recent, want = p.keep - p.recent;
     const int begin = rank * p.per, len = max(0, min(p.n - begin, p.per)), clen = max(0, min(cand - begin, p.per));      // this CTA's slots, and those of them that compete
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int i = blockIdx.x * EV_THREADS + tid; i < p.nflags; i += gridDim.x * EV_THREADS) p.flags[i] = 0u;
 #pragma unroll 8
     for (int i = tid; i < len; i += EV_THREADS) w_s[i] = w[begin + i];
@@ -249,10 +250,11 @@ int ev_prepare(int device) {
 }
 template <int CL> int ev_select(const EvParams& p, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)(p.kv_heads * CL)); cfg.blockDim = dim3(EV_THREADS); cfg.dynamicSmemBytes = (size_t)p.per * 4; cfg.stream = st; cfg.attrs = attr;
-    attr[0].id = cudaLaunchAttributeClusterDimension; attr[0].val.clusterDim.x = CL; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.numAttrs = CL > 1 ? 1 : 0;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension; attr[1].val.clusterDim.x = CL; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = CL > 1 ? 2 : 1;
     IT_CUDA(cudaLaunchKernelEx(&cfg, k_evict_select<CL>, p));
     return IT_OK;
 }
@@ -293,10 +295,6 @@ IT_API int it_cache_evict(void* stream, const it_cache_evict_args* a) {
     if (const int r = pl.cluster == 1 ? ev_select<1>(p, st) : pl.cluster == 8 ? ev_select<8>(p, st) : ev_select<16>(p, st)) return r;
     const unsigned lines = (unsigned)a->kv_heads * ((p.k != nullptr) + (p.v != nullptr));
     if (!lines) return IT_OK;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    cfg.gridDim = dim3(lines * (unsigned)pl.blocks); cfg.blockDim = dim3(EV_MOVE_THREADS); cfg.dynamicSmemBytes = (size_t)EV_BLOCK * p.row_bytes; cfg.stream = st; cfg.attrs = attr; cfg.numAttrs = 1;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
-    IT_CUDA(cudaLaunchKernelEx(&cfg, k_evict_move, p));
+    IT_CUDA(it_launch_early(k_evict_move, dim3(lines * (unsigned)pl.blocks), dim3(EV_MOVE_THREADS), (size_t)EV_BLOCK * p.row_bytes, st, p));
     return IT_OK;
 }

@@ -37,6 +37,7 @@ __global__ void __launch_bounds__(NR_WARPS * 32) k_norm_rope(const __grid_consta
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.x;
     const int nq = p.q ? p.heads : 0, nkv = p.k ? p.kv_heads : 0;
     const int job = blockIdx.y * NR_WARPS + warp;
+    asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
     const int add = p.base ? *p.base : 0;
     const bool is_q = job < nq, is_v = job >= nq + nkv;
     const int h = is_q ? job : is_v ? job - nq - nkv : job - nq;
@@ -208,9 +209,9 @@ IT_API int it_norm_rope(void* stream, const it_norm_rope_args* a) {
     const int jobs = (a->q ? a->heads : 0) + (a->k ? 2 * a->kv_heads : 0);
     const dim3 grid((unsigned)a->rows, (unsigned)((jobs + NR_WARPS - 1) / NR_WARPS));
     const cudaStream_t st = (cudaStream_t)stream;
-    if (a->type == IT_F32) k_norm_rope<float, __half><<<grid, NR_WARPS * 32, 0, st>>>(p);
-    else if (a->type == IT_F16) k_norm_rope<__half, __half><<<grid, NR_WARPS * 32, 0, st>>>(p);
-    else k_norm_rope<__nv_bfloat16, __nv_bfloat16><<<grid, NR_WARPS * 32, 0, st>>>(p);
-    IT_LAUNCH_CHECK("k_norm_rope");
+    const dim3 block(NR_WARPS * 32);
+    if (a->type == IT_F32) IT_CUDA(it_launch_early(k_norm_rope<float, __half>, grid, block, 0, st, p));
+    else if (a->type == IT_F16) IT_CUDA(it_launch_early(k_norm_rope<__half, __half>, grid, block, 0, st, p));
+    else IT_CUDA(it_launch_early(k_norm_rope<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, st, p));
     return IT_OK;
 }

@@ -139,7 +139,7 @@ int ta_prepare(int device) {
 }
 
 int ta_join(const TaParams& p, int type, int nb, cudaStream_t st) {
-    auto go = [&](auto kern) -> int { IT_CUDA(ta_launch(true, kern, dim3(p.prows, p.kv_heads), dim3(64 * nb), 0, st, p)); return IT_OK; };
+    auto go = [&](auto kern) -> int { IT_CUDA(it_launch_early(kern, dim3(p.prows, p.kv_heads), dim3(64 * nb), 0, st, p)); return IT_OK; };
     if (type == IT_F32) return nb == 2 ? go(k_tree_join<float, 2>) : go(k_tree_join<float, 4>);
     if (type == IT_F16) return nb == 2 ? go(k_tree_join<__half, 2>) : go(k_tree_join<__half, 4>);
     return nb == 2 ? go(k_tree_join<__nv_bfloat16, 2>) : go(k_tree_join<__nv_bfloat16, 4>);

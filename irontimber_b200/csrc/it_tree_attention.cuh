@@ -114,16 +114,6 @@ template <class T> struct TaRow<T, true> {
     }
 };
 
-// A launch that may begin while the kernel before it in the stream still runs; it waits for that kernel itself.
-template <typename... KArgs, typename... Args> cudaError_t ta_launch(bool early, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = early ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, args...);
-}
-
 // Whether row t sees slot j.
 __device__ __forceinline__ bool ta_sees(const TaParams& p, const unsigned (*anc)[TA_WORDS], int t, int j, int cached) {
     const int i = j - cached;

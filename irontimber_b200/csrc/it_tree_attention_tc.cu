@@ -103,8 +103,22 @@ template <int N> __device__ __forceinline__ void tm_wait(float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) asm volatile("" : "+f"(v[i]));
 }
-// Maximum over a warp (NaN left out, as by fmaxf).
-__device__ __forceinline__ float warp_max(float v) { float r; asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v)); return r; }
+// Maximum over the warp of each of N values (NaN left out, as by fmaxf): lane r gets that of value r, for r < N.  Halves what a lane carries at every step; a redux a value costs the
+// sub-core 16 cycles each, 1050 for four warps of 16 values.
+template <int N> __device__ __forceinline__ float warp_max(float (&v)[N], int lane) {
+#pragma unroll
+    for (int h = N / 2; h > 0; h >>= 1) {
+        const bool up = lane & h;
+#pragma unroll
+        for (int i = 0; i < h; i++) {
+            const float keep = up ? v[i + h] : v[i], give = up ? v[i] : v[i + h];
+            v[i] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, h));
+        }
+    }
+#pragma unroll
+    for (int h = N; h < 32; h <<= 1) v[0] = fmaxf(v[0], __shfl_xor_sync(0xffffffffu, v[0], h));
+    return v[0];
+}
 // Integers in the order of the floats.
 __device__ __forceinline__ int ordered(float v) { const int i = __float_as_int(v); return i ^ ((i >> 31) & 0x7fffffff); }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
@@ -183,6 +197,23 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     const unsigned kring = smem_u32(smem + L::KR), vring = smem_u32(smem + L::VR);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp == W0 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" :: "l"(&vmap) : "memory");
+        *abort_flag = (smem_u32(smem) & 1023u) != 0;                 // the swizzle counts on it; never seen
+#pragma unroll 1
+        for (int s = 0; s < 2 * (KS * NB + VS * MT); s++) mbar_init(bars + 8 * s, 1);
+        for (int s = 0; s < 2; s++) { mbar_init(sfull + 8 * s, 1); mbar_init(sfree + 8 * s, W0); }
+        mbar_init(pfull, W0); mbar_init(ofull, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == W0 + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)L::ALLOC) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid < 2 * NR) maxes[tid] = ordered(-INFINITY);
+    __syncwarp();
+    asm volatile("griddepcontrol.wait;" ::: "memory");               // the kernel may have begun while the one before it still ran; from here on it reads what that one wrote
     const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TA_KEYS - 1) / TA_KEYS;
     // this run's tiles: the first `tiles % splits` runs have one more
     const int per = (int)((unsigned)tiles / (unsigned)p.splits), more = tiles - per * p.splits, tile0 = split * per + min(split, more), n = per + (split < more ? 1 : 0);
@@ -198,26 +229,12 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
         tma_load_3d(vring + 2 * at * L::BOX, &vmap, 128 * m, (tile0 + i) * TA_KEYS, g, vfull + 8 * at);
         tma_load_3d(vring + (2 * at + 1) * L::BOX, &vmap, 128 * m + 64, (tile0 + i) * TA_KEYS, g, vfull + 8 * at);
     };
-    if (warp == W0 && lane == 0) {
-        *abort_flag = (smem_u32(smem) & 1023u) != 0;                 // the swizzle counts on it; never seen
+    if (warp == W0 && lane == 0 && n > 0) {                          // the first tile before anything else
 #pragma unroll 1
-        for (int s = 0; s < 2 * (KS * NB + VS * MT); s++) mbar_init(bars + 8 * s, 1);
-        for (int s = 0; s < 2; s++) { mbar_init(sfull + 8 * s, 1); mbar_init(sfree + 8 * s, W0); }
-        mbar_init(pfull, W0); mbar_init(ofull, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        // the first tile before anything else
-        if (n > 0) {
+        for (int b = 0; b < NB; b++) load_k(0, b);
 #pragma unroll 1
-            for (int b = 0; b < NB; b++) load_k(0, b);
-#pragma unroll 1
-            for (int m = 0; m < MT; m++) load_v(0, m);
-        }
+        for (int m = 0; m < MT; m++) load_v(0, m);
     }
-    if (warp == W0 + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"((unsigned)L::ALLOC) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    if (tid < 2 * NR) maxes[tid] = ordered(-INFINITY);
     __syncwarp();
     tc_load_q<T, SPLIT, NB, NR, L::THREADS / 32>(p, smem + L::Q, fac, trow, g, r0, warp, lane);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // Q before the products read it
@@ -320,14 +337,13 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 }
                 if (move) {
                     const unsigned see = masked ? (i == first_masked ? vis[0] : i == first_masked + 1 ? vis[1] : vis[2]) : 0xffffffffu;
-                    float mine = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < RW; r++) {
                         x[r] *= f[r];
                         if (!((see >> r) & 1u)) x[r] = -INFINITY;
-                        const float m = warp_max(x[r]);
-                        if (lane == r) mine = m;
+                        y[r] = x[r];
                     }
+                    const float mine = warp_max(y, lane);
                     int* const best = maxes + (exact & 1) * NR + wg * RW;
                     exact++;
                     if (lane < RW) atomicMax(best + lane, ordered(fmaxf(mrun, mine)));
@@ -698,13 +714,13 @@ template <class T, bool SPLIT, int NB> int prepare_dim() {
 template <class T, bool SPLIT> int prepare_type() { const int r = prepare_dim<T, SPLIT, 2>(); return r ? r : prepare_dim<T, SPLIT, 4>(); }
 
 template <class T, bool SPLIT, int NB, int NR> int run_shape(const TaParams& p, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
-    IT_CUDA(ta_launch(false, k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TcTree<SPLIT, NB, NR>::THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, km, vm, p));
+    IT_CUDA(it_launch_early(k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TcTree<SPLIT, NB, NR>::THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, km, vm, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB, int NR> int weigh_shape(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
     // one wave of CTAs, as many tiles for each
     const int tiles = (p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, most = p.kv_heads < TA_MAXSPLITS ? TA_MAXSPLITS / p.kv_heads : 1, rounds = (tiles + most - 1) / most;
-    IT_CUDA(ta_launch(true, k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((tiles + rounds - 1) / rounds, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
+    IT_CUDA(it_launch_early(k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((tiles + rounds - 1) / rounds, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB> int run_dim(const TaParams& p, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
