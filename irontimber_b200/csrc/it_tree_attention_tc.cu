@@ -28,8 +28,8 @@ template <bool SPLIT, int NB, int NR> struct TcTree {
     // instruction-cache misses, and half the rows are half the code.
     static constexpr int WGS = NR >= 32 ? 4 : 2, RW = NR / WGS, SOFT = 128 * WGS, THREADS = SOFT + 128;
     static constexpr int OR = MT == 2 ? 2 * NR / WGS : RW;                                    // accumulators of a thread: one element of d, this many product rows
-    // setmaxnreg deals out the launch's registers: 216 x 256 + 72 x 128 = 168 x 384; 104 x 512 + 64 x 128 = 96 x 640
-    static constexpr int REGS = WGS == 2 ? 168 : 96, SOFT_REGS = WGS == 2 ? 216 : 104, OTHER_REGS = WGS == 2 ? 72 : 64;
+    // setmaxnreg deals out the launch's registers: 216 x 256 + 72 x 128 = 168 x 384; 112 x 512 + 32 x 128 = 96 x 640
+    static constexpr int REGS = WGS == 2 ? 168 : 96, SOFT_REGS = WGS == 2 ? 216 : 112, OTHER_REGS = WGS == 2 ? 72 : 32;
     static constexpr int QB = NB * NC * 128, PB = NCB * TA_KEYS * 128, BOX = TA_KEYS * 128, SLOT = NB * BOX;
     static constexpr int FIT = (TC_SMEM_LIMIT - TC_SMALL - QB - PB) / SLOT, SLOTS = FIT < TC_SLOTS_MAX ? FIT : TC_SLOTS_MAX;
     static constexpr int KS = (SLOTS + 1) / 2, VS = SLOTS - KS;
@@ -329,8 +329,9 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 const float *const f = fac + wg * RW, *const bs = base_s + wg * RW;
                 float* const c = corr_s + (i % 3) * NR + wg * RW;
                 bool move = i == 0 || masked;
-                float y[RW], top = -INFINITY;
+                float y[RW];
                 if (!move) {
+                    float top = -INFINITY;
 #pragma unroll
                     for (int r = 0; r < RW; r++) { y[r] = fmaf(x[r], f[r], -bs[r]); top = fmaxf(top, y[r]); }
                     move = group_any(wg, top > TC_TOP);             // the same answer in all four warps
@@ -339,8 +340,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     const unsigned see = masked ? (i == first_masked ? vis[0] : i == first_masked + 1 ? vis[1] : vis[2]) : 0xffffffffu;
 #pragma unroll
                     for (int r = 0; r < RW; r++) {
-                        x[r] *= f[r];
-                        if (!((see >> r) & 1u)) x[r] = -INFINITY;
+                        x[r] = (see >> r) & 1u ? x[r] * f[r] : -INFINITY;
                         y[r] = x[r];
                     }
                     const float mine = warp_max(y, lane);
