@@ -27,7 +27,6 @@ template <bool SPLIT, int NB, int NR> struct TcTree {
     // Groups of four softmax warps, and product rows of one.  Four groups for 32 rows and more: a thread's share of a tile is unrolled code that runs a few times, at the speed of
     // instruction-cache misses, and half the rows are half the code.
     static constexpr int WGS = NR >= 32 ? 4 : 2, RW = NR / WGS, SOFT = 128 * WGS, THREADS = SOFT + 128;
-    static constexpr int OR = MT == 2 ? 2 * NR / WGS : RW;                                    // accumulators of a thread: one element of d, this many product rows
     // setmaxnreg deals out the launch's registers: 216 x 256 + 72 x 128 = 168 x 384; 112 x 512 + 32 x 128 = 96 x 640
     static constexpr int REGS = WGS == 2 ? 168 : 96, SOFT_REGS = WGS == 2 ? 216 : 112, OTHER_REGS = WGS == 2 ? 72 : 32;
     static constexpr int QB = NB * NC * 128, PB = NCB * TA_KEYS * 128, BOX = TA_KEYS * 128, SLOT = NB * BOX;
@@ -38,7 +37,7 @@ template <bool SPLIT, int NB, int NR> struct TcTree {
     static constexpr int BARS = 0, TMEM = 512, FLAG = 528, MAXES = 576, BASE = 1088, CORR = 1344, FAC = 2112, TROW = 2368;
     static constexpr int TCOLS = 2 * SC + MT * NC, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
     static_assert(VS >= 1 && NR % 16 == 0 && NC <= 128 && NR <= 64 && NC % 16 == 0 && RW % 8 == 0, "");
-    static_assert((2 * KS * NB + 2 * VS * MT + 6) * 8 <= TMEM, "");
+    static_assert((2 * KS * NB + 2 * VS * MT + 5 + MT) * 8 <= TMEM, "");
     static_assert(SOFT_REGS * SOFT + OTHER_REGS * 128 <= REGS * THREADS, "");
     static_assert(PB >= TA_MAXROWS * TA_WORDS * 4 + TA_MAXROWS * 4, "the ancestors are worked out in P's place");
     static_assert(KS * SLOT >= NR * TA_KEYS * 4 && KS * SLOT >= NR * HD * 4, "sums and accumulators go through K's place");
@@ -179,7 +178,7 @@ __global__ void __launch_bounds__(TcTree<SPLIT, NB, NR>::THREADS, 1)
 k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TaParams p) {
     using L = TcTree<SPLIT, NB, NR>;
     using TA = typename std::conditional<SPLIT, float, T>::type;
-    constexpr int NC = L::NC, RW = L::RW, OR = L::OR, HD = L::HD, KS = L::KS, VS = L::VS, WGS = L::WGS, MT = L::MT, W0 = 4 * WGS;       // W0: the first warp behind the softmax warps
+    constexpr int NC = L::NC, RW = L::RW, HD = L::HD, KS = L::KS, VS = L::VS, WGS = L::WGS, MT = L::MT, W0 = 4 * WGS;       // W0: the first warp behind the softmax warps
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, g = blockIdx.y, r0 = blockIdx.z * NR;
@@ -188,12 +187,12 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     unsigned* tmem_slot = reinterpret_cast<unsigned*>(small + L::TMEM);
     int* maxes = reinterpret_cast<int*>(small + L::MAXES);              // [2][NR]
     float* base_s = reinterpret_cast<float*>(small + L::BASE);          // [NR]
-    float* corr_s = reinterpret_cast<float*>(small + L::CORR);          // [3][NR]
+    float* corr_s = reinterpret_cast<float*>(small + L::CORR);          // [2][NR]: a group's rows are its own, the tile before is taken over after this one's scores
     float* fac = reinterpret_cast<float*>(small + L::FAC);              // [NR]
     int* trow = reinterpret_cast<int*>(small + L::TROW);                // [NR]
     const unsigned bars = smem_u32(small + L::BARS);
     // K in boxes of 64 elements, V in pairs of them (an M tile of O^T): each has barriers of its own, so that the next tile's first box is asked for when this tile's is read
-    const unsigned kfull = bars, kempty = kfull + 8 * KS * NB, vfull = kempty + 8 * KS * NB, vempty = vfull + 8 * VS * MT, sfull = vempty + 8 * VS * MT, sfree = sfull + 16, pfull = sfree + 16, ofull = pfull + 8;
+    const unsigned kfull = bars, kempty = kfull + 8 * KS * NB, vfull = kempty + 8 * KS * NB, vempty = vfull + 8 * VS * MT, sfull = vempty + 8 * VS * MT, sfree = sfull + 16, pfull = sfree + 16, ofull = pfull + 8;       // (one an M tile)
     const unsigned kring = smem_u32(smem + L::KR), vring = smem_u32(smem + L::VR);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -204,7 +203,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll 1
         for (int s = 0; s < 2 * (KS * NB + VS * MT); s++) mbar_init(bars + 8 * s, 1);
         for (int s = 0; s < 2; s++) { mbar_init(sfull + 8 * s, 1); mbar_init(sfree + 8 * s, W0); }
-        mbar_init(pfull, W0); mbar_init(ofull, 1);
+        mbar_init(pfull, W0);
+        for (int m = 0; m < MT; m++) mbar_init(ofull + 8 * m, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == W0 + 1) {
@@ -247,11 +247,12 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
         warp_regs_inc<L::SOFT_REGS>();
         const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
         const unsigned lanes = (unsigned)(quad * 32) << 16;
-        const int mt = MT == 2 ? wg & 1 : 0, orow = MT == 2 ? (wg >> 1) * OR : wg * RW, d = mt * 128 + key;        // M tile and first product row of the accumulators, their element of the head
-        const unsigned oaddr = otm + lanes + mt * NC + orow;
-        float acc[OR], l[RW], mrun = -INFINITY;                     // mrun: the running maximum of row `lane` of the group
+        const unsigned oaddr = otm + lanes + wg * RW;               // the accumulators: elements `key` and 128 + `key` of the head, the group's product rows
+        float acc[MT][RW], l[RW], mrun = -INFINITY;                 // mrun: the reference of row `lane` of the group
 #pragma unroll
-        for (int r = 0; r < OR; r++) acc[r] = 0.f;
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int r = 0; r < RW; r++) acc[m][r] = 0.f;
 #pragma unroll
         for (int r = 0; r < RW; r++) l[r] = 0.f;
         bool ok = true;
@@ -278,24 +279,27 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             groups_sync<WGS>();                                     // before P takes the place of the ancestors
         }
         int exact = 0;                                              // references moved so far
-        auto collect = [&](int i) {                                 // O^T of tile i
-            ok = ok && tc_wait_warp(ofull, (unsigned)i & 1u, abort_flag, p.status, 52);
-            ok = ok && tc_wait_warp(pfull, (unsigned)i & 1u, abort_flag, p.status, 53);      // met long ago: the other groups' factors are seen through it
-            fence_after();
-            const float* const c = corr_s + (i % 3) * NR + orow;
-            constexpr int CH = OR < 16 ? OR : 16;
+        // O^T of tile i.  What the first M tile gave is taken over while the second is still under way.
+        auto collect = [&](int i) {
+            const float* const c = corr_s + (i & 1) * NR + wg * RW;
 #pragma unroll
-            for (int k = 0; k < OR; k += CH) {
-                float u[CH], v[SPLIT ? CH : 1];
-                tm_ld(u, oaddr + k);
-                if constexpr (SPLIT) tm_ld(v, oaddr + NR + k);
-                tm_wait(u);
-                if constexpr (SPLIT) {
+            for (int m = 0; m < MT; m++) {
+                ok = ok && tc_wait_warp(ofull + 8 * m, (unsigned)i & 1u, abort_flag, p.status, 52);
+                fence_after();
+                constexpr int CH = RW < 16 ? RW : 16;
 #pragma unroll
-                    for (int e = 0; e < CH; e++) { asm volatile("" : "+f"(v[e])); u[e] += v[e]; }
+                for (int k = 0; k < RW; k += CH) {
+                    float u[CH], v[SPLIT ? CH : 1];
+                    tm_ld(u, oaddr + m * NC + k);
+                    if constexpr (SPLIT) tm_ld(v, oaddr + m * NC + NR + k);
+                    tm_wait(u);
+                    if constexpr (SPLIT) {
+#pragma unroll
+                        for (int e = 0; e < CH; e++) { asm volatile("" : "+f"(v[e])); u[e] += v[e]; }
+                    }
+#pragma unroll
+                    for (int e = 0; e < CH; e++) acc[m][k + e] = fmaf(acc[m][k + e], c[k + e], u[e]);
                 }
-#pragma unroll
-                for (int e = 0; e < CH; e++) acc[k + e] = fmaf(acc[k + e], c[k + e], u[e]);
             }
             fence_before();
         };
@@ -327,7 +331,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 // Exponents against the rows' references.  A reference need not be the maximum: it moves when an exponent would pass f16's range, in the first tile, and in
                 // masked tiles (a row may have seen nothing before), which spares all other tiles the maximum over slots.
                 const float *const f = fac + wg * RW, *const bs = base_s + wg * RW;
-                float* const c = corr_s + (i % 3) * NR + wg * RW;
+                float* const c = corr_s + (i & 1) * NR + wg * RW;
                 bool move = i == 0 || masked;
                 float y[RW];
                 if (!move) {
@@ -379,28 +383,36 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             if (masked) {
                 // V elements that are not finite leave the product and go to the rows that see their slot
                 const int j0 = (tile0 + i) * TA_KEYS, from = max(cached - j0, 0), to = min(TA_KEYS, p.cached + p.rows - j0);
-                ok = ok && tc_wait_warp(vfull + 8 * (i % VS * MT + mt), (unsigned)(i / VS) & 1u, abort_flag, p.status, 54);
-                unsigned char* const v = smem + L::VR + (i % VS) * L::SLOT + (d >> 6) * L::BOX + (d & 7) * 2;
-                bool any = false;
-#pragma unroll 1
-                for (int k = from; k < to; k++) {
-                    const unsigned short raw = *reinterpret_cast<const unsigned short*>(v + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4));
-                    if ((raw & Ta16<T>::EXP) != Ta16<T>::EXP) continue;
-                    any = true;
-                    unsigned long long rows = 0;
-#pragma unroll 1
-                    for (int r = 0; r < OR; r++)
-                        if (j0 + k - cached < p.rows && tc_walk(p.parents, trow[orow + r], j0 + k - cached)) rows |= 1ull << r;
-                    const float bad = Ta16<T>::unpack(raw).x;
+                bool any[MT];
 #pragma unroll
-                    for (int r = 0; r < OR; r++) if ((rows >> r) & 1ull) acc[r] += bad;
-                }
-                groups_sync<WGS>();                         // all groups have looked at the elements that one of them clears
-                if (any && orow == 0)
+                for (int m = 0; m < MT; m++) {
+                    ok = ok && tc_wait_warp(vfull + 8 * (i % VS * MT + m), (unsigned)(i / VS) & 1u, abort_flag, p.status, 54);
+                    const unsigned char* const v = smem + L::VR + (i % VS) * L::SLOT + (2 * m + (key >> 6)) * L::BOX + (key & 7) * 2;
+                    any[m] = false;
 #pragma unroll 1
                     for (int k = from; k < to; k++) {
-                        unsigned short* e = reinterpret_cast<unsigned short*>(v + k * 128 + ((((d & 63) >> 3) ^ (k & 7)) << 4));
-                        if ((*e & Ta16<T>::EXP) == Ta16<T>::EXP) *e = 0;
+                        const unsigned short raw = *reinterpret_cast<const unsigned short*>(v + k * 128 + ((((key & 63) >> 3) ^ (k & 7)) << 4));
+                        if ((raw & Ta16<T>::EXP) != Ta16<T>::EXP) continue;
+                        any[m] = true;
+                        unsigned rows = 0;
+#pragma unroll 1
+                        for (int r = 0; r < RW; r++)
+                            if (j0 + k - cached < p.rows && tc_walk(p.parents, trow[wg * RW + r], j0 + k - cached)) rows |= 1u << r;
+                        const float bad = Ta16<T>::unpack(raw).x;
+#pragma unroll
+                        for (int r = 0; r < RW; r++) if ((rows >> r) & 1u) acc[m][r] += bad;
+                    }
+                }
+                groups_sync<WGS>();                         // all groups have looked at the elements that one of them clears
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+                    if (any[m] && wg == 0) {
+                        unsigned char* const v = smem + L::VR + (i % VS) * L::SLOT + (2 * m + (key >> 6)) * L::BOX + (key & 7) * 2;
+#pragma unroll 1
+                        for (int k = from; k < to; k++) {
+                            unsigned short* e = reinterpret_cast<unsigned short*>(v + k * 128 + ((((key & 63) >> 3) ^ (k & 7)) << 4));
+                            if ((*e & Ta16<T>::EXP) == Ta16<T>::EXP) *e = 0;
+                        }
                     }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -426,9 +438,13 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
         if (quad == 0 && lane < RW) ml[wg * RW + lane].x = mrun == -INFINITY ? mrun : base_s[wg * RW + lane];
         if (p.splits > 1) {
             const size_t at = ((size_t)split * p.kv_heads + g) * p.pad_rows + r0;
-            float* const o = p.part_o + (at + orow) * HD + d;
+            float* const o = p.part_o + (at + wg * RW) * HD + key;
 #pragma unroll
-            for (int r = 0; r < OR; r++) if (r0 + orow + r < p.prows) __stcg(o + r * HD, acc[r]);
+            for (int r = 0; r < RW; r++)
+                if (r0 + wg * RW + r < p.prows) {
+#pragma unroll
+                    for (int m = 0; m < MT; m++) __stcg(o + r * HD + 128 * m, acc[m][r]);
+                }
             groups_sync<WGS>();
             if (tid < NR) p.part_ml[at + tid] = ml[tid];
         } else {
@@ -436,7 +452,9 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             float* const os = reinterpret_cast<float*>(smem + L::KR);          // [NR][HD], where the sums were
             groups_sync<WGS>();
 #pragma unroll
-            for (int r = 0; r < OR; r++) os[(orow + r) * HD + d] = acc[r];
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int r = 0; r < RW; r++) os[(wg * RW + r) * HD + 128 * m + key] = acc[m][r];
             groups_sync<WGS>();
             if (p.stats && tid < NR) p.stats[(size_t)g * p.pad_rows + r0 + tid] = make_float2(ml[tid].x == -INFINITY ? 0.f : ml[tid].x, ml[tid].y);
             constexpr int LN = HD / 4, STEP = L::SOFT / LN, U = 4;              // threads of a row, rows at once, rows of a thread whose gates are on their way together
@@ -529,9 +547,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                                 for (int j = 0; j < 4; j++) mma_f16(otm + m * NC, vd + (unsigned)(j * 2048 >> 4), pb + (unsigned)(j * 2048 >> 4), idesc<T>(NC, true), k + j > 0);          // 16 slots a step
                                 vd += (unsigned)(4 * 2048 >> 4); pb += (unsigned)(4 * 2048 >> 4);
                             }
-                            commit_to(vempty + 8 * at);
+                            commit_to(ofull + 8 * m); commit_to(vempty + 8 * at);
                         }
-                        if (ok) commit_to(ofull);
                         oi++; since = clock64();
                     } else if (*abort_flag) break;
                     else if (clock64() - since > WAIT_CLOCKS) { if (!*abort_flag) atomicExch(p.status, 59); *abort_flag = 1; break; }
