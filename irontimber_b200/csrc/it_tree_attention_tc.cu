@@ -516,45 +516,38 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             // ---------------- products: the scores of tile si, O^T of tile oi, whichever has its inputs.  Loops, not straight code: see WGS.
             if (elect_one()) {
                 const unsigned long long qd = desc_k(smem_u32(smem + L::Q)), pd = desc_mn(smem_u32(smem + L::P), L::BOX);
-                int si = 0, oi = 0; long long since = clock64(); bool ok = true;
+                int si = 0, kb = 0, oi = 0, om = 0; long long since = clock64();          // tile of the scores, box of K, tile and M tile of the products that come next
 #pragma unroll 1
-                while (ok && oi < n) {
-                    if (si < n && mbar_poll(sfree + 8 * (si & 1), ((unsigned)(si >> 1) & 1u) ^ 1u) && mbar_poll(kfull + 8 * (si % KS * NB), (unsigned)(si / KS) & 1u)) {
+                while (oi < n) {
+                    const unsigned va = (unsigned)(oi % VS * MT + om), ka = (unsigned)(kb % (KS * NB));
+                    if (oi < si && (om > 0 || mbar_poll(pfull, (unsigned)oi & 1u)) && mbar_poll(vfull + 8 * va, (unsigned)(oi / VS) & 1u)) {
+                        fence_after();
+                        unsigned long long vd = desc_mn(vring + 2 * va * L::BOX, L::BOX), pb = pd;
 #pragma unroll 1
-                        for (int b = 0; b < NB; b++) {
-                            const unsigned at = (unsigned)(si % KS * NB + b);
-                            ok = tc_wait(kfull + 8 * at, (unsigned)(si / KS) & 1u, abort_flag, p.status, 57);
-                            if (!ok) break;
-                            fence_after();
-                            const unsigned long long kd = desc_k(kring + at * L::BOX), qb = qd + (unsigned)(b * NC * 128 >> 4);
+                        for (int k = 0; k < TA_KEYS / 16; k += 4) {
 #pragma unroll
-                            for (int k = 0; k < 4; k++) mma_f16(tmem + (si & 1) * L::SC + b * L::PARTS / NB * NC, kd + (unsigned)(k * 32 >> 4), qb + (unsigned)(k * 32 >> 4), idesc<T>(NC, false), b % (NB / L::PARTS) + k > 0);     // 16 elements of the head a step
-                            commit_to(kempty + 8 * at);
+                            for (int j = 0; j < 4; j++) mma_f16(otm + om * NC, vd + (unsigned)(j * 2048 >> 4), pb + (unsigned)(j * 2048 >> 4), idesc<T>(NC, true), k + j > 0);          // 16 slots a step
+                            vd += (unsigned)(4 * 2048 >> 4); pb += (unsigned)(4 * 2048 >> 4);
                         }
-                        if (ok) commit_to(sfull + 8 * (si & 1));
-                        si++; since = clock64();
-                    } else if (oi < si && mbar_poll(pfull, (unsigned)oi & 1u)) {
-#pragma unroll 1
-                        for (int m = 0; m < MT; m++) {
-                            const unsigned at = (unsigned)(oi % VS * MT + m);
-                            ok = tc_wait(vfull + 8 * at, (unsigned)(oi / VS) & 1u, abort_flag, p.status, 58);
-                            if (!ok) break;
-                            fence_after();
-                            unsigned long long vd = desc_mn(vring + 2 * at * L::BOX, L::BOX), pb = pd;
-#pragma unroll 1
-                            for (int k = 0; k < TA_KEYS / 16; k += 4) {
+                        commit_to(ofull + 8 * om); commit_to(vempty + 8 * va);
+                        if (++om == MT) { om = 0; oi++; }
+                        since = clock64();
+                    } else if (si < n && (kb % NB || mbar_poll(sfree + 8 * (si & 1), ((unsigned)(si >> 1) & 1u) ^ 1u)) && mbar_poll(kfull + 8 * ka, (unsigned)(si / KS) & 1u)) {
+                        // a box at a time, so that a product whose P comes meanwhile does not wait for K
+                        const int b = kb % NB;
+                        fence_after();
+                        const unsigned long long kd = desc_k(kring + ka * L::BOX), qb = qd + (unsigned)(b * NC * 128 >> 4);
 #pragma unroll
-                                for (int j = 0; j < 4; j++) mma_f16(otm + m * NC, vd + (unsigned)(j * 2048 >> 4), pb + (unsigned)(j * 2048 >> 4), idesc<T>(NC, true), k + j > 0);          // 16 slots a step
-                                vd += (unsigned)(4 * 2048 >> 4); pb += (unsigned)(4 * 2048 >> 4);
-                            }
-                            commit_to(ofull + 8 * m); commit_to(vempty + 8 * at);
-                        }
-                        oi++; since = clock64();
+                        for (int k = 0; k < 4; k++)
+                            mma_f16(tmem + (si & 1) * L::SC + b * L::PARTS / NB * NC, kd + (unsigned)(k * 32 >> 4), qb + (unsigned)(k * 32 >> 4), idesc<T>(NC, false), b % (NB / L::PARTS) + k > 0);     // 16 elements of the head a step
+                        commit_to(kempty + 8 * ka);
+                        if (b == NB - 1) { commit_to(sfull + 8 * (si & 1)); si++; }
+                        kb++; since = clock64();
                     } else if (*abort_flag) break;
                     else if (clock64() - since > WAIT_CLOCKS) { if (!*abort_flag) atomicExch(p.status, 59); *abort_flag = 1; break; }
                 }
                 // the last commits must find the CTA's shared memory still its own (bounded)
-                landed(kempty, 0, si * NB, KS * NB); landed(vempty, 0, oi * MT, VS * MT);
+                landed(kempty, 0, kb, KS * NB); landed(vempty, 0, oi * MT + om, VS * MT);
             }
         }
     }
