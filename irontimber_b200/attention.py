@@ -90,27 +90,34 @@ assert (_NORM_ROPE.size, _TREE.size, _EVICT.size) == (C.sizeof(NormRopeArgs), C.
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
 _current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 _NONE3 = (0, 0, 0)
+_F16, _BF16, _F32, _I32T = torch.float16, torch.bfloat16, torch.float32, torch.int32
 
 
 def _three(x, name, shape, dtype, index):
     """Address and outer strides of a [a, b, element] tensor of this shape with contiguous elements."""
     st = x.stride()
-    if len(st) != 3 or x.shape != shape:
+    if x.shape != shape or x.dtype is not dtype or x.get_device() != index or st[2] != 1:
+        _refuse_three(x, name, shape, dtype, index)
+    return x.data_ptr(), st[0], st[1]
+
+
+def _refuse_three(x, name, shape, dtype, index):
+    if x.shape != shape:
         raise ValueError(f"{name} has the shape {tuple(x.shape)}, not {tuple(shape)}")
     if x.dtype is not dtype:
         raise TypeError(f"{name} is {x.dtype}, not {dtype}")
     if x.get_device() != index:
         raise ValueError(f"{name} is on {x.device}, not on the device of the others")
-    if st[2] != 1 and shape[2] > 1:
+    if shape[2] > 1:
         raise ValueError(f"the elements of a head of {name} are not contiguous")
-    return x.data_ptr(), st[0], st[1]
 
 
 def _flat(x, name, n, dtype, index):
     """Address of a contiguous vector of at least n elements; 0 for None."""
     if x is None:
         return 0
-    if x.dim() != 1 or x.shape[0] < n or x.dtype is not dtype or x.get_device() != index or (n > 1 and x.stride(0) != 1):
+    st = x.stride()
+    if len(st) != 1 or x.numel() < n or x.dtype is not dtype or x.get_device() != index or (st[0] != 1 and n > 1):
         raise ValueError(f"{name} is {tuple(x.shape)} {x.dtype} on {x.device}: a contiguous vector of {n} {dtype} on the device of the others is wanted")
     return x.data_ptr()
 
@@ -118,17 +125,21 @@ def _flat(x, name, n, dtype, index):
 def _caches(k, v, index):
     """Shape, type and the addresses and strides of a pair of caches."""
     shape, dtype = k.shape, k.dtype
-    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+    if dtype is not _F16 and dtype is not _BF16:
         raise TypeError(f"a cache is float16 or bfloat16, not {dtype}")
-    if len(shape) != 3:
-        raise ValueError(f"k_cache has the shape {tuple(shape)}, not three dimensions")
-    return shape, TYPES[dtype], _three(k, "k_cache", shape, dtype, index), _three(v, "v_cache", shape, dtype, index)
+    st = k.stride()
+    if len(st) != 3 or st[2] != 1 or k.get_device() != index:
+        if len(st) != 3:
+            raise ValueError(f"k_cache has the shape {tuple(shape)}, not three dimensions")
+        _refuse_three(k, "k_cache", shape, dtype, index)
+    return shape, TYPES[dtype], (k.data_ptr(), st[0], st[1]), _three(v, "v_cache", shape, dtype, index)
 
 
 def _rows(x, name):
-    if x.dim() != 3:
-        raise ValueError(f"{name} has the shape {tuple(x.shape)}, not three dimensions")
-    return x.shape
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} has the shape {tuple(shape)}, not three dimensions")
+    return shape
 
 
 def _launch(call, args, index, stream):
@@ -153,27 +164,27 @@ def norm_rope(rope, q, k, v, q_out, k_cache, v_cache, slot0, positions, q_norm=N
     rotation.  positions: int32 tensor [row], or the position of row 0.  base: int32 tensor whose value is added to slots (and to positions that
     are a number), read on the device.  q and q_out, or k, v and the caches, may be None."""
     some, name = (q, "q") if q is not None else (k, "k")
-    rows, heads, dim = _rows(some, name)
+    shape = rows, heads, dim = _rows(some, name)
     act, index = some.dtype, some.get_device()
     t = ct = TYPES.get(act, -1)
     kv, slots, qp, qo, kp, vp, kc, vc = 1, 0, _NONE3, _NONE3, _NONE3, _NONE3, _NONE3, _NONE3
     if t == 0:
         ct = 1
     if q is not None:
-        qp, qo = _three(q, "q", q.shape, act, index), _three(q_out, "q_out", q.shape, act, index)
+        qp, qo = _three(q, "q", shape, act, index), _three(q_out, "q_out", shape, act, index)
     if k is not None:
         (slots, kv, d), ct, kc, vc = _caches(k_cache, v_cache, index)
         want = (rows, kv, dim)
-        if d != dim or k.shape != want:
-            raise ValueError(f"caches of {kv} heads of {d} for k of {tuple(k.shape)} behind q of {rows} rows of {dim}")
+        if d != dim:
+            raise ValueError(f"caches of {kv} heads of {d} for heads of {dim}")
         kp, vp = _three(k, "k", want, act, index), _three(v, "v", want, act, index)
     pos0 = 0
     if isinstance(positions, torch.Tensor):
-        positions = _flat(positions, "positions", rows, torch.int32, index)
+        positions = _flat(positions, "positions", rows, _I32T, index)
     else:
         pos0, positions = positions, 0
-    args = _NORM_ROPE.pack(t, ct, rows, heads, kv, dim, rope.handle.value if rope is not None else 0, *qp, *kp, *vp, *qo, *kc, *vc, slots, slot0, positions, _flat(base, "base", 1, torch.int32, index),
-                           _flat(q_norm, "q_norm", dim, torch.float32, index), _flat(k_norm, "k_norm", dim, torch.float32, index), pos0, eps)
+    args = _NORM_ROPE.pack(t, ct, rows, heads, kv, dim, rope.handle.value if rope is not None else 0, *qp, *kp, *vp, *qo, *kc, *vc, slots, slot0, positions, _flat(base, "base", 1, _I32T, index),
+                           _flat(q_norm, "q_norm", dim, _F32, index), _flat(k_norm, "k_norm", dim, _F32, index), pos0, eps)
     _launch(_load().it_norm_rope, args, index, stream)
 
 
@@ -192,7 +203,7 @@ def tree_attention(q, k_cache, v_cache, cached, out, parents=None, gate=None, sc
     qp, op = _three(q, "q", shape, act, index), _three(out, "out", shape, act, index)
     gp = _three(gate, "gate", shape, act, index) if gate is not None else _NONE3
     wp, wh = _weights(weights, kv, cached + rows, index) if weights is not None else (0, 0)
-    parents, length = _flat(parents, "parents", rows, torch.int32, index), _flat(length, "length", 1, torch.int32, index)
+    parents, length = _flat(parents, "parents", rows, _I32T, index), _flat(length, "length", 1, _I32T, index)
     if workspace is None:
         workspace = _workspace(_tree_bytes(t, ct, rows, heads, kv, dim), index, stream)
     else:
@@ -225,9 +236,10 @@ _load = _lib.load
 
 
 def _weights(w, kv, n, index):
-    if w.dim() != 2 or w.shape[0] != kv or w.shape[1] < n or w.dtype is not torch.float32 or w.get_device() != index or (n > 1 and w.stride(1) != 1):
+    st, shape = w.stride(), w.shape
+    if len(st) != 2 or shape[0] != kv or shape[1] < n or w.dtype is not _F32 or w.get_device() != index or (st[1] != 1 and n > 1):
         raise ValueError(f"weights are {tuple(w.shape)} {w.dtype} on {w.device}: f32 [{kv}, {n} or more] with contiguous rows on the device of the others are wanted")
-    return w.data_ptr(), w.stride(0)
+    return w.data_ptr(), st[0]
 
 
 def _workspace(nbytes, index, stream):

@@ -185,7 +185,7 @@ def test_tensors_are_checked_before_the_library_sees_them(lib):
         attention.tree_attention(q, kc, kc.clone(), 10, torch.zeros_like(q), parents=torch.zeros(3, dtype=torch.int64))
     with pytest.raises(ValueError, match="kept is"):
         attention.cache_evict(kc, kc.clone(), torch.zeros(2, 50), 40, 20, 3, torch.zeros(2, 19, dtype=torch.int32))
-    with pytest.raises(ValueError, match="caches of 2 heads"):
+    with pytest.raises(ValueError, match="k has the shape"):
         attention.norm_rope(None, q, torch.zeros(3, 1, 64), torch.zeros(3, 1, 64), torch.zeros_like(q), kc, kc.clone(), 0, 0)
     # another device than the CUDA ones is refused by the types of the pair first, when those do not fit
     from irontimber_b200._lib import IronTimberError
