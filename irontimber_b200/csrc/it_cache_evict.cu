@@ -249,13 +249,7 @@ int ev_prepare(int device) {
     return IT_OK;
 }
 template <int CL> int ev_select(const EvParams& p, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    cfg.gridDim = dim3((unsigned)(p.kv_heads * CL)); cfg.blockDim = dim3(EV_THREADS); cfg.dynamicSmemBytes = (size_t)p.per * 4; cfg.stream = st; cfg.attrs = attr;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension; attr[1].val.clusterDim.x = CL; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.numAttrs = CL > 1 ? 2 : 1;
-    IT_CUDA(cudaLaunchKernelEx(&cfg, k_evict_select<CL>, p));
+    IT_CUDA(it_launch_early(k_evict_select<CL>, dim3((unsigned)(p.kv_heads * CL)), dim3(EV_THREADS), (size_t)p.per * 4, st, CL, p));
     return IT_OK;
 }
 
@@ -295,6 +289,6 @@ IT_API int it_cache_evict(void* stream, const it_cache_evict_args* a) {
     if (const int r = pl.cluster == 1 ? ev_select<1>(p, st) : pl.cluster == 8 ? ev_select<8>(p, st) : ev_select<16>(p, st)) return r;
     const unsigned lines = (unsigned)a->kv_heads * ((p.k != nullptr) + (p.v != nullptr));
     if (!lines) return IT_OK;
-    IT_CUDA(it_launch_early(k_evict_move, dim3(lines * (unsigned)pl.blocks), dim3(EV_MOVE_THREADS), (size_t)EV_BLOCK * p.row_bytes, st, p));
+    IT_CUDA(it_launch_early(k_evict_move, dim3(lines * (unsigned)pl.blocks), dim3(EV_MOVE_THREADS), (size_t)EV_BLOCK * p.row_bytes, st, 1, p));
     return IT_OK;
 }

@@ -210,8 +210,8 @@ IT_API int it_norm_rope(void* stream, const it_norm_rope_args* a) {
     const dim3 grid((unsigned)a->rows, (unsigned)((jobs + NR_WARPS - 1) / NR_WARPS));
     const cudaStream_t st = (cudaStream_t)stream;
     const dim3 block(NR_WARPS * 32);
-    if (a->type == IT_F32) IT_CUDA(it_launch_early(k_norm_rope<float, __half>, grid, block, 0, st, p));
-    else if (a->type == IT_F16) IT_CUDA(it_launch_early(k_norm_rope<__half, __half>, grid, block, 0, st, p));
-    else IT_CUDA(it_launch_early(k_norm_rope<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, st, p));
+    if (a->type == IT_F32) IT_CUDA(it_launch_early(k_norm_rope<float, __half>, grid, block, 0, st, 1, p));
+    else if (a->type == IT_F16) IT_CUDA(it_launch_early(k_norm_rope<__half, __half>, grid, block, 0, st, 1, p));
+    else IT_CUDA(it_launch_early(k_norm_rope<__nv_bfloat16, __nv_bfloat16>, grid, block, 0, st, 1, p));
     return IT_OK;
 }

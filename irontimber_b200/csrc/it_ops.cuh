@@ -31,12 +31,13 @@ static inline bool it_strides_ok(int64_t n0, int64_t s0, int64_t n1, int64_t s1,
 
 // A launch that may begin while the kernel before it in the stream still runs.  Every kernel here that is launched so waits (griddepcontrol.wait) before it touches
 // global memory, so that a chain of them is ordered like plain launches; what overlaps is the launch itself and the kernel's start (2 us of a short call).
-template <typename... KArgs, typename... Args> static inline cudaError_t it_launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const Args&... args) {
+template <typename... KArgs, typename... Args> static inline cudaError_t it_launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension; attr[1].val.clusterDim.x = (unsigned)cluster; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 

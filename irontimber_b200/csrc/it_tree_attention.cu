@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(64 * NB) k_tree_join(const __grid_constant__ T
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
 // How a call is cut: rows of a CTA's product tile, tiles of product rows, runs of the cache.
-struct TaPlan { int nb, nr, pad_rows, row_tiles, splits; size_t part_o, part_ml, stats, total; };
+struct TaPlan { int nb, nr, pad_rows, row_tiles, splits; bool joined; size_t part_o, part_ml, stats, total; };
 
 TaPlan ta_plan(const it_tree_attention_args* a, int sm_count) {
     TaPlan pl;
@@ -96,11 +96,14 @@ TaPlan ta_plan(const it_tree_attention_args* a, int sm_count) {
     if (splits > tiles) splits = tiles;
     if (splits < 1) splits = 1;
     pl.splits = (int)splits;
+    // The runs of a short cache join inside the kernel, as a cluster (512 slots, one row: 7.8 us against 8.2, and a launch of the host's).  A cluster's CTAs have to be in one GPC, which
+    // holds 16 of them or more: where eight GPCs cannot have all clusters at once, the others' second wave costs more (24 clusters of six, 30,011 slots: 231 us against 107).
+    pl.joined = splits == 1 || (splits <= TA_JOIN && splits == tiles && ctas <= 8 * (16 / splits));
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t rows = (size_t)a->kv_heads * pl.pad_rows;
     pl.part_o = 0;
-    pl.part_ml = splits > 1 ? up((size_t)splits * rows * 64 * pl.nb * 4) : 0;
-    pl.stats = pl.part_ml + (splits > 1 ? up((size_t)splits * rows * 8) : 0);
+    pl.part_ml = !pl.joined ? up((size_t)splits * rows * 64 * pl.nb * 4) : 0;
+    pl.stats = pl.part_ml + (!pl.joined ? up((size_t)splits * rows * 8) : 0);
     pl.total = pl.stats + up(rows * 8);        // the statistics of a call without weights are not kept, but sizes do not depend on pointers
     return pl;
 }
@@ -139,7 +142,7 @@ int ta_prepare(int device) {
 }
 
 int ta_join(const TaParams& p, int type, int nb, cudaStream_t st) {
-    auto go = [&](auto kern) -> int { IT_CUDA(it_launch_early(kern, dim3(p.prows, p.kv_heads), dim3(64 * nb), 0, st, p)); return IT_OK; };
+    auto go = [&](auto kern) -> int { IT_CUDA(it_launch_early(kern, dim3(p.prows, p.kv_heads), dim3(64 * nb), 0, st, 1, p)); return IT_OK; };
     if (type == IT_F32) return nb == 2 ? go(k_tree_join<float, 2>) : go(k_tree_join<float, 4>);
     if (type == IT_F16) return nb == 2 ? go(k_tree_join<__half, 2>) : go(k_tree_join<__half, 4>);
     return nb == 2 ? go(k_tree_join<__nv_bfloat16, 2>) : go(k_tree_join<__nv_bfloat16, 4>);
@@ -200,9 +203,9 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     p.part_o = (float*)(ws + pl.part_o); p.part_ml = (float2*)(ws + pl.part_ml); p.stats = a->weights ? (float2*)(ws + pl.stats) : nullptr; p.status = dev.status_dev;
     p.q_row = a->q_row; p.q_head = a->q_head; p.g_row = a->g_row; p.g_head = a->g_head; p.o_row = a->o_row; p.o_head = a->o_head; p.w_head = a->w_head;
     p.rows = a->rows; p.heads = a->heads; p.group = a->heads / a->kv_heads; p.kv_heads = a->kv_heads; p.dim = a->head_dim; p.cached = (int)a->cached; p.splits = pl.splits;
-    p.prows = a->rows * p.group; p.pad_rows = pl.pad_rows; p.group_inv = (unsigned)((0x100000000ull + p.group - 1) / p.group); p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale;
+    p.prows = a->rows * p.group; p.pad_rows = pl.pad_rows; p.joined = pl.joined; p.group_inv = (unsigned)((0x100000000ull + p.group - 1) / p.group); p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale;
     const cudaStream_t st = (cudaStream_t)stream;
     if (const int r = it_tree_tc_run(p, a->type, pl.nb, pl.nr, pl.row_tiles, km, vm, st)) return r;
-    if (p.splits > 1) if (const int r = ta_join(p, a->type, pl.nb, st)) return r;
+    if (!p.joined) if (const int r = ta_join(p, a->type, pl.nb, st)) return r;
     return p.weights ? it_tree_tc_weigh(p, a->type, pl.nb, pl.nr, km, st) : IT_OK;
 }

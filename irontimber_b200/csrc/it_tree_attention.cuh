@@ -9,7 +9,7 @@ struct TaParams {
     const void *q, *gate; void* out; const int *parents, *length; float* weights;
     float* part_o; float2* part_ml; float2* stats; int* status;
     long long q_row, q_head, g_row, g_head, o_row, o_head, w_head;
-    int rows, heads, group, kv_heads, dim, cached, splits, prows, pad_rows; unsigned group_inv; float scale;
+    int rows, heads, group, kv_heads, dim, cached, splits, prows, pad_rows, joined; unsigned group_inv; float scale;
 };
 
 // it_tree_attention_tc.cu.  nb: 64-element pieces of a head, nr: product rows of a CTA (16, 32 or 64).
@@ -19,7 +19,7 @@ int it_tree_tc_weigh(const TaParams& p, int type, int nb, int nr, const CUtensor
 
 namespace {
 
-constexpr int TA_KEYS = 128, TA_MAXROWS = 256, TA_WORDS = TA_MAXROWS / 32, TA_MAXSPLITS = 148;       // slots of a tile; rows of a call; runs of a cache, one an SM
+constexpr int TA_KEYS = 128, TA_MAXROWS = 256, TA_WORDS = TA_MAXROWS / 32, TA_MAXSPLITS = 148, TA_JOIN = 8;       // slots of a tile; rows of a call; runs of a cache, one an SM; runs that join in a cluster (the portable size)
 constexpr float TA_LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }

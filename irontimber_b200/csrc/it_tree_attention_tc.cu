@@ -16,6 +16,7 @@
 namespace {
 
 constexpr int TC_SMEM_LIMIT = 227 * 1024, TC_SMALL = 3072, TC_SLOTS_MAX = 6;
+constexpr int TC_JOIN = TA_JOIN;                            // runs that join in a cluster, at most
 constexpr float TC_SHIFT = 6.f, TC_TOP = 15.f;              // p is 2^6 at the reference and may grow to 2^15 before the reference moves
 
 template <bool SPLIT, int NB, int NR> struct TcTree {
@@ -137,6 +138,16 @@ template <int N> __device__ __forceinline__ unsigned group_or(unsigned q) {
 }
 __device__ __forceinline__ bool group_any(int wg, bool q) { return (wg == 0 ? group_or<1>(q) : wg == 1 ? group_or<2>(q) : wg == 2 ? group_or<3>(q) : group_or<4>(q)) != 0; }
 
+// The cluster's barrier, and its CTAs' shared memory.
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ unsigned cluster_addr(unsigned a, int rank) { unsigned r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank)); return r; }
+__device__ __forceinline__ float2 ld_cluster2(unsigned a, int rank) {
+    float2 v; asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_addr(a, rank)) : "memory"); return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(unsigned a, int rank) {
+    float4 v; asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr(a, rank)) : "memory"); return v;
+}
+
 // Product rows [r0, r0 + NR) of KV head g as columns of Q^T; for each the factor from the product to log2 of its exponential, and its row t (rows behind the last: the
 // last one's).  A warp has all of its rows' loads under way at once: one after the other they were 7 us of a 64-row tile.
 template <class T, bool SPLIT, int NB, int NR, int NW>
@@ -243,6 +254,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     fence_after();
     const unsigned tmem = *tmem_slot, otm = tmem + 2 * L::SC;
 
+    float2* const ml = reinterpret_cast<float2*>(smem + L::P);       // [NR], at the end: references and sums of the rows
+    float* const os = reinterpret_cast<float*>(smem + L::KR);        // [NR][HD], at the end: accumulators
     if (warp < W0) {
         warp_regs_inc<L::SOFT_REGS>();
         const int wg = warp >> 2, quad = warp & 3, key = quad * 32 + lane;
@@ -421,7 +434,6 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
         }
         // ---- every product is done: the rings are free.  The rows' sums are those of the slots' threads.
         float* const sums = reinterpret_cast<float*>(smem + L::KR);            // [NR][128]
-        float2* const ml = reinterpret_cast<float2*>(smem + L::P);             // [NR]
 #pragma unroll
         for (int r = 0; r < RW; r++) sums[(wg * RW + r) * TA_KEYS + key] = l[r];
         group_sync(wg);
@@ -436,7 +448,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             if (lane == 0) ml[row].y = bad ? NAN : v;
         }
         if (quad == 0 && lane < RW) ml[wg * RW + lane].x = mrun == -INFINITY ? mrun : base_s[wg * RW + lane];
-        if (p.splits > 1) {
+        if (!p.joined) {
             const size_t at = ((size_t)split * p.kv_heads + g) * p.pad_rows + r0;
             float* const o = p.part_o + (at + wg * RW) * HD + key;
 #pragma unroll
@@ -448,40 +460,53 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             groups_sync<WGS>();
             if (tid < NR) p.part_ml[at + tid] = ml[tid];
         } else {
-            // through shared memory, so that a loop can write whole rows, four elements a thread
-            float* const os = reinterpret_cast<float*>(smem + L::KR);          // [NR][HD], where the sums were
-            groups_sync<WGS>();
+            groups_sync<WGS>();                                     // the sums, in whose place the accumulators go, are read
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int r = 0; r < RW; r++) os[(wg * RW + r) * HD + 128 * m + key] = acc[m][r];
-            groups_sync<WGS>();
-            if (p.stats && tid < NR) p.stats[(size_t)g * p.pad_rows + r0 + tid] = make_float2(ml[tid].x == -INFINITY ? 0.f : ml[tid].x, ml[tid].y);
-            constexpr int LN = HD / 4, STEP = L::SOFT / LN, U = 4;              // threads of a row, rows at once, rows of a thread whose gates are on their way together
+            // The runs of a short cache are a cluster, and join here: a run finishes every splits-th row, four elements a thread, reading the others' sums and accumulators
+            // from their shared memory.  Saves the partial results and a launch.
+            cluster_sync();
+            constexpr int LN = HD / 4, STEP = L::SOFT / LN;          // threads of a row, rows at once
             const int c = tid % LN * 4;
+            const unsigned mla = smem_u32(ml), osa = smem_u32(os) + 4 * c;
 #pragma unroll 1
-            for (int q = tid / LN; q < NR && c < p.dim; q += U * STEP) {
-                float z[U][4];
+            for (int q = tid / LN; c < p.dim; q += STEP) {
+                const int r = split + p.splits * q, row = r0 + r;
+                if (r >= NR || row >= p.prows) break;
+                const int t = trow[r], h = g * p.group + row - t * p.group;
+                float z[4] = { 0.f, 0.f, 0.f, 0.f };
+                if (p.gate) load4((const TA*)p.gate + t * p.g_row + h * p.g_head + c, z);
+                float2 e[TC_JOIN];
+                float top = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int r = q + u * STEP, row = r0 + r;
-                    if (p.gate && r < NR && row < p.prows) { const int t = trow[r]; load4((const TA*)p.gate + t * p.g_row + (g * p.group + row - t * p.group) * p.g_head + c, z[u]); }
+                for (int k = 0; k < TC_JOIN; k++) {
+                    e[k] = k < p.splits ? ld_cluster2(mla + 8 * r, k) : make_float2(-INFINITY, 0.f);
+                    top = fmaxf(top, e[k].x);
                 }
+                const float ref = top == -INFINITY ? 0.f : top;
+                float sum = 0.f, o[4] = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int r = q + u * STEP, row = r0 + r;
-                    if (r >= NR || row >= p.prows) break;
-                    const int t = trow[r], h = g * p.group + row - t * p.group;
-                    const float sum = ml[r].y, inv = sum == 0.f ? 0.f : 1.f / sum;
-                    const float4 v = *reinterpret_cast<const float4*>(os + r * HD + c);
-                    float o[4] = { v.x * inv, v.y * inv, v.z * inv, v.w * inv };
-                    if (p.gate) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[e] /= 1.f + __expf(-z[u][e]);
-                    }
-                    store4((TA*)p.out + t * p.o_row + h * p.o_head + c, o);
+                for (int k = 0; k < TC_JOIN; k++) {
+                    if (k >= p.splits || (e[k].x == -INFINITY && e[k].y == 0.f)) continue;       // saw nothing
+                    const float w = ex2(e[k].x - ref);
+                    const float4 v = ld_cluster4(osa + (unsigned)(r * HD * 4), k);
+                    sum = fmaf(e[k].y, w, sum);
+                    o[0] = fmaf(v.x, w, o[0]); o[1] = fmaf(v.y, w, o[1]); o[2] = fmaf(v.z, w, o[2]); o[3] = fmaf(v.w, w, o[3]);
                 }
+                if (p.stats && c == 0) p.stats[(size_t)g * p.pad_rows + row] = make_float2(ref, sum);
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] *= inv;
+                if (p.gate) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[i] /= 1.f + __expf(-z[i]);
+                }
+                store4((TA*)p.out + t * p.o_row + h * p.o_head + c, o);
             }
+            __syncwarp();
+            cluster_sync();                                         // nobody leaves while its shared memory may still be read
         }
     } else {
         warp_regs_dec<L::OTHER_REGS>();
@@ -550,6 +575,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 landed(kempty, 0, kb, KS * NB); landed(vempty, 0, oi * MT + om, VS * MT);
             }
         }
+        __syncwarp();
+        if (p.joined) { cluster_sync(); cluster_sync(); }
     }
     __syncwarp();
     fence_before();
@@ -724,13 +751,13 @@ template <class T, bool SPLIT, int NB> int prepare_dim() {
 template <class T, bool SPLIT> int prepare_type() { const int r = prepare_dim<T, SPLIT, 2>(); return r ? r : prepare_dim<T, SPLIT, 4>(); }
 
 template <class T, bool SPLIT, int NB, int NR> int run_shape(const TaParams& p, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
-    IT_CUDA(it_launch_early(k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TcTree<SPLIT, NB, NR>::THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, km, vm, p));
+    IT_CUDA(it_launch_early(k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TcTree<SPLIT, NB, NR>::THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, p.joined ? p.splits : 1, km, vm, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB, int NR> int weigh_shape(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
     // one wave of CTAs, as many tiles for each
     const int tiles = (p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, most = p.kv_heads < TA_MAXSPLITS ? TA_MAXSPLITS / p.kv_heads : 1, rounds = (tiles + most - 1) / most;
-    IT_CUDA(it_launch_early(k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((tiles + rounds - 1) / rounds, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, km, p));
+    IT_CUDA(it_launch_early(k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((tiles + rounds - 1) / rounds, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, 1, km, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB> int run_dim(const TaParams& p, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
