@@ -335,7 +335,7 @@ int it_argmax_static(void* stream, const float* logits_dev, size_t n, uint32_t* 
  * order without waiting and without allocating; the arena and stream of a context (it_arena_ptr, it_ctx_stream) are such pointers and such a
  * stream.  Strides count elements; the elements of a head are contiguous.  head_dim is a multiple of 8 up to 256, heads a multiple of kv_heads.  Types
  * are pairs: f32 activations over an f16 cache (as in the engine), or f16 / bf16 for both.  Activation pointers and strides are
- * aligned to 4 elements, cache pointers to 16 bytes and cache strides to 8 elements.  A cache is [slot][kv head][head_dim] or [kv head][slot][head_dim] or
+ * aligned to 4 elements, cache pointers to 16 bytes and cache strides to 8 elements, norm weights to 16 bytes.  At most 1024 query heads share a kv head.  A cache is [slot][kv head][head_dim] or [kv head][slot][head_dim] or
  * any other pair of strides; k and v may lie in one buffer.  All may be recorded in a CUDA graph once one call of that entry point on that device
  * has been made outside of recording.  A call of no rows (keep 0) looks at no pointer and does nothing.  Sums, norms, softmax statistics and accumulators are f32 (angles: 64-bit fractions of a turn). */
 enum { IT_F32 = 0, IT_F16 = 1, IT_BF16 = 2 };
