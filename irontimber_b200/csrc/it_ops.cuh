@@ -29,8 +29,9 @@ static inline bool it_strides_ok(int64_t n0, int64_t s0, int64_t n1, int64_t s1,
     return n0 <= 1 || n1 <= 1 || (s0 <= s1 ? s1 >= (n0 - 1) * s0 + d : s0 >= (n1 - 1) * s1 + d);
 }
 
-// A launch that may begin while the kernel before it in the stream still runs.  Every kernel here that is launched so waits (griddepcontrol.wait) before it touches
-// global memory, so that a chain of them is ordered like plain launches; what overlaps is the launch itself and the kernel's start (2 us of a short call).
+// A launch that may begin while the kernel before it in the stream still runs.  The first kernel of every call waits (griddepcontrol.wait) before it touches global memory, and the later ones
+// before they touch what the call writes, so that a chain of them is ordered like plain launches; what overlaps is the launch itself and the kernel's start (1.5 us of a short call).
+// A kernel whose successors read the caller's tensors before their wait must not let them begin before its own.
 template <typename... KArgs, typename... Args> static inline cudaError_t it_launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(64 * NB) k_tree_join(const __grid_constant__ T
     const int grp = tid / LANES, c = tid % LANES * 4;
     const int t = ta_row(p, r), h = g * p.group + r - t * p.group;
     float z[4] = { 0.f, 0.f, 0.f, 0.f };
-    // the gate is the caller's: nothing before this kernel in the call writes it
+    // The gate is the caller's: nothing in this call writes it, and the kernel before lets this one begin only when whatever wrote it has ended.
     if (p.gate && grp == 0 && c < p.dim) load4((const TA*)p.gate + t * p.g_row + h * p.g_head + c, z);
     asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
     const size_t step = (size_t)p.kv_heads * p.pad_rows, at = (size_t)g * p.pad_rows + r;

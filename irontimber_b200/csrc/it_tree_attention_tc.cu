@@ -206,7 +206,6 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     const unsigned kfull = bars, kempty = kfull + 8 * KS * NB, vfull = kempty + 8 * KS * NB, vempty = vfull + 8 * VS * MT, sfull = vempty + 8 * VS * MT, sfree = sfull + 16, pfull = sfree + 16, ofull = pfull + 8;       // (one an M tile)
     const unsigned kring = smem_u32(smem + L::KR), vring = smem_u32(smem + L::VR);
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == W0 && lane == 0) {
         asm volatile("prefetch.tensormap [%0];" :: "l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" :: "l"(&vmap) : "memory");
@@ -224,7 +223,9 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     }
     if (tid < 2 * NR) maxes[tid] = ordered(-INFINITY);
     __syncwarp();
-    asm volatile("griddepcontrol.wait;" ::: "memory");               // the kernel may have begun while the one before it still ran; from here on it reads what that one wrote
+    // The kernel may have begun while the one before it still ran; from here on it reads what that one wrote.  Only then may the kernels behind it begin: they read the caller's
+    // gate, cache and parents before they wait for this one.
+    asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;" ::: "memory");
     const int cached = ta_cached(p), total = cached + p.rows, tiles = (total + TA_KEYS - 1) / TA_KEYS;
     // this run's tiles: the first `tiles % splits` runs have one more
     const int per = (int)((unsigned)tiles / (unsigned)p.splits), more = tiles - per * p.splits, tile0 = split * per + min(split, more), n = per + (split < more ? 1 : 0);

@@ -586,6 +586,41 @@ def test_a_request_that_drafts_trees_and_cuts_its_cache(ops):
         be.close()
 
 
+def test_inputs_of_a_kernel_that_lets_others_begin_early(ops):
+    """The library's products let the next kernel begin while they run; q, gate and parents that such a kernel (and one behind it) writes have to be complete when they are read."""
+    import numpy as np
+    from irontimber_b200.backend import CudaBackend
+    e, heads, dim, cached = 5120, 2, 64, 128 * 40
+    width = 2 * heads * dim
+    be = CudaBackend(0, arena_floats=1 << 20)
+    try:
+        rng = np.random.default_rng(4)
+        w_big, w = be.mat_synth(1, 60000, e), be.mat_synth(2, width, e)
+        q8 = be.q8_rows(e, 4)
+        be.set_signs(np.ones(e, np.float32))
+        Y = 4 * e
+        x, y = be.view(0, 4, e), be.view(Y, 4, width)
+        q, z = y[:, :heads * dim].view(4, heads, dim), y[:, heads * dim:].view(4, heads, dim)
+        with torch.cuda.stream(be.torch_stream):
+            kc, vc = (torch.randn(cached + 4, 1, dim, device="cuda").half() for _ in range(2))
+            out, want, got = torch.empty(4, heads, dim, device="cuda"), torch.empty(4, heads, dim, device="cuda"), torch.zeros(1, cached + 4, device="cuda")
+            ref = torch.zeros(1, cached + 4, device="cuda")
+            par = torch.tensor([-1, 0, 0, 1], dtype=torch.int32, device="cuda")
+            for turn in range(40):
+                y.fill_(float("nan"))
+                be.upload(0, rng.standard_normal((4, e)).astype(np.float32))
+                be.had_q8(e, 4, 0, e, q8)
+                be.mv(w_big, 4, q8, Y + 4 * width, 60000)
+                be.mv(w, 4, q8, Y, width)                            # q and gate, right in front of the call that reads them
+                be.tree_attention(q, kc, vc, cached, out, parents=par, gate=z, scale=1e-3, weights=got)
+                be.sync()
+                be.tree_attention(q, kc, vc, cached, want, parents=par, gate=z, scale=1e-3, weights=ref)
+                be.sync()
+                assert torch.equal(out, want) and torch.equal(got, ref) and torch.isfinite(out).all()
+    finally:
+        be.close()
+
+
 def test_first_refusals_on_a_device(ops):
     from irontimber_b200._lib import IronTimberError
     q, kc, vc, g = make("f32", 2, 100, 4, 2, 64, 1)
