@@ -83,3 +83,40 @@ static inline bool it_attn_takes_tiled(int hd, int nh, int nkv, int slot0, int n
 // k_gdn_rows (it_gdn_prefill.cu) is built for a state size of 128 and for three tokens or more: the warp that stores a state row first waits for
 // the other warp's read of it at the third token.
 static inline bool it_gdn_rows_takes(int sd, int nt) { return sd == 128 && nt >= 3; }
+
+// ---- attention of a token, chain or tree over a caller's cache ------------------------------------------------------------------
+// How k_tree_attention_tc (it_tree_attention_tc.cu) is cut: product rows (rows x query heads of a KV head) of a CTA, tiles of them, and runs of the cache (tiles of 128 slots), one
+// wave of CTAs.  The runs of a short cache join inside the kernel, as a cluster (512 slots, one row: 7.8 us against 8.2, and a launch of the host's); a cluster's CTAs
+// have to be in one GPC, which holds 16 of them or more, and where eight GPCs cannot have all clusters at once the others' second wave costs more (24 clusters
+// of six, 30,011 slots: 231 us against 107).
+#define IT_TREE_JOIN 8                             // runs that join in a cluster, at most: the portable size
+struct it_tree_cut { int nr, row_tiles, splits; bool joined; };
+static inline it_tree_cut it_tree_cut_by(int nr, long prows, long kv_heads, long tiles, int sm_count) {
+    it_tree_cut c;
+    c.nr = nr; c.row_tiles = (int)((prows + nr - 1) / nr);
+    const long ctas = kv_heads * c.row_tiles;
+    long splits = sm_count / ctas;
+    splits = splits > tiles ? tiles : splits;
+    c.splits = splits < 1 ? 1 : (int)splits;
+    c.joined = c.splits == 1 || (c.splits <= IT_TREE_JOIN && c.splits == tiles && ctas <= 8 * (16 / c.splits));
+    return c;
+}
+// Which of 16, 32 and 64 product rows: a start (code that runs once, q), a time for each tile of a run, and the partial results, written and read.  A tile's time hardly grows with its rows, so
+// few rows a CTA pay while they leave no run longer.  The constants are fitted to the choice, not to the times: on the measurements below it is never more than 6 % behind the best.
+// us with 16 / 32 / 64, f32, 24 over 4 heads of 256:  3 rows at 500 slots 8.8 / 10.0 / 11.0, at 8190 17.9 / 16.3 / 18.3;  6 at 500 9.5 / 11.2 / 12.9, at 30,011 46.8 / 38.4 / 34.2
+//   12 at 100 12.0 / 14.1 / 18.8, at 2091 14.3 / 13.9 / 16.6, at 8190 28.1 / 22.2 / 22.6, at 30,011 72.5 / 50.1 / 43.5;  20 at 500 12.6 / 12.9 / 14.9, at 8190 42.0 / 27.7 / 24.1
+//   64 at 100 22.6 / 17.5 / 20.2, at 500 27.6 / 22.5 / 21.9, at 2091 50.4 / 32.2 / 28.6, at 30,011 467 / 178 / 110;  f16, 32 over 8 of 128: 8 at 500 7.7 / 8.8 / 10.5, 32 at 8190 40.6 / 29.0 / 24.8
+static inline it_tree_cut it_tree_cut_of(long prows, long kv_heads, int head_dim, long tiles, int sm_count) {
+    it_tree_cut best = {};
+    double least = 0;
+    for (int i = 0; i < 3; i++) {
+        const double start[3] = { 13.8, 15.2, 20.7 }, wide[3] = { 2.15, 2.7, 2.65 }, narrow[3] = { 1.85, 1.15, 1.2 };
+        const it_tree_cut c = it_tree_cut_by(16 << i, prows, kv_heads, tiles, sm_count);
+        const long waves = (kv_heads * c.row_tiles * c.splits + sm_count - 1) / sm_count, run = (tiles + c.splits - 1) / c.splits;
+        const double partial = c.joined ? -1.0 : (double)c.splits * prows * kv_heads * (head_dim <= 128 ? 128 : 256) * 8 / 4.7e6;
+        const double us = waves * (start[i] + run * (head_dim <= 128 ? narrow[i] : wide[i])) + partial;
+        if (i == 0 || us < least) { best = c; least = us; }
+        if (c.row_tiles == 1) break;               // more rows a CTA than there are
+    }
+    return best;
+}

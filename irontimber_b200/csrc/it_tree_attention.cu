@@ -12,6 +12,7 @@
 // Masks: only tiles that reach behind the cached slots look at them.  A masked score is replaced, whatever it was; there a non-finite V element is
 // taken out of the product and added to the rows that do see it (0 * inf would be NaN in those that do not).
 #include "it_tree_attention.cuh"
+#include "it_route.h"
 #include <mutex>
 
 namespace {
@@ -84,26 +85,18 @@ __global__ void __launch_bounds__(64 * NB) k_tree_join(const __grid_constant__ T
 // How a call is cut: rows of a CTA's product tile, tiles of product rows, runs of the cache.
 struct TaPlan { int nb, nr, pad_rows, row_tiles, splits; bool joined; size_t part_o, part_ml, stats, total; };
 
-TaPlan ta_plan(const it_tree_attention_args* a, int sm_count) {
+long ta_tiles(const it_tree_attention_args* a) { return ((long)a->cached + a->rows + TA_KEYS - 1) / TA_KEYS; }
+TaPlan ta_plan(const it_tree_attention_args* a, const it_tree_cut& c) {
     TaPlan pl;
-    const int group = a->heads / a->kv_heads, prows = a->rows * group;
     pl.nb = a->head_dim <= 128 ? 2 : 4;
-    pl.nr = prows <= 16 ? 16 : prows <= 32 ? 32 : 64;
-    pl.row_tiles = (prows + pl.nr - 1) / pl.nr;
+    pl.nr = c.nr; pl.row_tiles = c.row_tiles; pl.splits = c.splits; pl.joined = c.joined;
     pl.pad_rows = pl.row_tiles * pl.nr;
-    const long tiles = ((long)a->cached + a->rows + TA_KEYS - 1) / TA_KEYS, ctas = (long)a->kv_heads * pl.row_tiles;
-    long splits = sm_count / ctas;             // one wave of CTAs: at most TA_MAXSPLITS
-    if (splits > tiles) splits = tiles;
-    if (splits < 1) splits = 1;
-    pl.splits = (int)splits;
-    // The runs of a short cache join inside the kernel, as a cluster (512 slots, one row: 7.8 us against 8.2, and a launch of the host's).  A cluster's CTAs have to be in one GPC, which
-    // holds 16 of them or more: where eight GPCs cannot have all clusters at once, the others' second wave costs more (24 clusters of six, 30,011 slots: 231 us against 107).
-    pl.joined = splits == 1 || (splits <= TA_JOIN && splits == tiles && ctas <= 8 * (16 / splits));
+    const size_t splits = (size_t)pl.splits;
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t rows = (size_t)a->kv_heads * pl.pad_rows;
     pl.part_o = 0;
-    pl.part_ml = !pl.joined ? up((size_t)splits * rows * 64 * pl.nb * 4) : 0;
-    pl.stats = pl.part_ml + (!pl.joined ? up((size_t)splits * rows * 8) : 0);
+    pl.part_ml = !pl.joined ? up(splits * rows * 64 * pl.nb * 4) : 0;
+    pl.stats = pl.part_ml + (!pl.joined ? up(splits * rows * 8) : 0);
     pl.total = pl.stats + up(rows * 8);        // the statistics of a call without weights are not kept, but sizes do not depend on pointers
     return pl;
 }
@@ -164,8 +157,14 @@ int ta_check_sizes(const it_tree_attention_args* a) {
 IT_API int it_tree_attention_workspace(const it_tree_attention_args* a, size_t* nbytes) {
     if (const int r = ta_check_sizes(a)) return r;
     IT_CHECK_ARG(nbytes, "it_tree_attention_workspace: null argument");
-    // without a device: as many SMs as sm_100a parts have
-    *nbytes = a->rows ? ta_plan(a, TA_MAXSPLITS).total : 0;
+    // the most that any cut of these sizes asks for: it then grows with `cached`, and a workspace for a long cache serves a shorter one, which may be cut another way
+    *nbytes = 0;
+    for (int nr = 16; a->rows && nr <= 64; nr *= 2) {
+        const it_tree_cut c = it_tree_cut_by(nr, (long)a->rows * (a->heads / a->kv_heads), a->kv_heads, ta_tiles(a), TA_MAXSPLITS);
+        const size_t n = ta_plan(a, c).total;
+        if (n > *nbytes) *nbytes = n;
+        if (c.row_tiles == 1) break;
+    }
     return IT_OK;
 }
 
@@ -192,7 +191,7 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     it_ops_device dev;
     if (const int r = it_ops_current(stream, who, &dev)) return r;
     if (const int r = ta_prepare(dev.device)) return r;
-    const TaPlan pl = ta_plan(a, TA_MAXSPLITS);
+    const TaPlan pl = ta_plan(a, it_tree_cut_of((long)a->rows * (a->heads / a->kv_heads), a->kv_heads, a->head_dim, ta_tiles(a), TA_MAXSPLITS));
     IT_CHECK_ARG(a->workspace && it_aligned(a->workspace, 256) && a->workspace_bytes >= pl.total, "%s: a workspace of %zu bytes, 256-byte aligned, is needed", who, pl.total);
     CUtensorMap km, vm;
     if (const int r = ta_map(&km, a->k_cache, a->cache_type, a->head_dim, a->cached + T, a->kc_slot, a->kv_heads, a->kc_head)) return r;
@@ -207,5 +206,6 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     const cudaStream_t st = (cudaStream_t)stream;
     if (const int r = it_tree_tc_run(p, a->type, pl.nb, pl.nr, pl.row_tiles, km, vm, st)) return r;
     if (!p.joined) if (const int r = ta_join(p, a->type, pl.nb, st)) return r;
-    return p.weights ? it_tree_tc_weigh(p, a->type, pl.nb, pl.nr, km, st) : IT_OK;
+    // the second walk has no runs to cut: as many product rows at once as there are, up to 64
+    return p.weights ? it_tree_tc_weigh(p, a->type, pl.nb, p.prows <= 16 ? 16 : p.prows <= 32 ? 32 : 64, km, st) : IT_OK;
 }

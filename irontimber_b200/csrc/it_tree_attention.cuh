@@ -19,7 +19,7 @@ int it_tree_tc_weigh(const TaParams& p, int type, int nb, int nr, const CUtensor
 
 namespace {
 
-constexpr int TA_KEYS = 128, TA_MAXROWS = 256, TA_WORDS = TA_MAXROWS / 32, TA_MAXSPLITS = 148, TA_JOIN = 8;       // slots of a tile; rows of a call; runs of a cache, one an SM; runs that join in a cluster (the portable size)
+constexpr int TA_KEYS = 128, TA_MAXROWS = 256, TA_WORDS = TA_MAXROWS / 32, TA_MAXSPLITS = 148;       // slots of a tile; rows of a call; runs of a cache, one an SM
 constexpr float TA_LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }

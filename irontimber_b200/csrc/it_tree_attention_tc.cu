@@ -12,11 +12,12 @@
 // slots chained in mma.sync accumulators).  Two warps copy, one issues whichever product has its inputs, the next tile's scores or this tile's O.
 // What bounds it: 64 columns of f32 activations (128 with the low halves) 2 x 1024 tensor cycles a tile of 128 slots at head dimension 256; few columns: HBM.
 #include "it_tree_attention.cuh"
+#include "it_route.h"
 
 namespace {
 
 constexpr int TC_SMEM_LIMIT = 227 * 1024, TC_SMALL = 3072, TC_SLOTS_MAX = 6;
-constexpr int TC_JOIN = TA_JOIN;                            // runs that join in a cluster, at most
+constexpr int TC_JOIN = IT_TREE_JOIN;                            // runs that join in a cluster, at most
 constexpr float TC_SHIFT = 6.f, TC_TOP = 15.f;              // p is 2^6 at the reference and may grow to 2^15 before the reference moves
 
 template <bool SPLIT, int NB, int NR> struct TcTree {
