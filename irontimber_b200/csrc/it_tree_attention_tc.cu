@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int TC_SMEM_LIMIT = 227 * 1024, TC_SMALL = 3072, TC_SLOTS_MAX = 6;
+constexpr int TC_SMEM_LIMIT = 227 * 1024, TC_SMALL = 3 * 1024, TC_SLOTS_MAX = 6;
 constexpr int TC_JOIN = IT_TREE_JOIN;                            // runs that join in a cluster, at most
 constexpr float TC_SHIFT = 6.f, TC_TOP = 15.f;              // p is 2^6 at the reference and may grow to 2^15 before the reference moves
 

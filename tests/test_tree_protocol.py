@@ -7,7 +7,7 @@ import random
 
 import pytest
 
-KEYS, LIMIT, SMALL = 128, 227 * 1024, 3072
+KEYS, LIMIT, SMALL = 128, 227 * 1024, 3 * 1024
 
 
 def shape(split, nb, nr):
