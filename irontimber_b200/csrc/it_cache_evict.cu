@@ -3,9 +3,11 @@
 // Per KV head: the last `recent` slots stay, and of the others the keep - recent with the largest weight, ties to the lower slot; what stays moves to the front in
 // its old order, in place.
 //
-// k_evict_select: a cluster of CTAs has a head (one CTA for short caches) and holds its weights in shared memory: one read for all passes.  The smallest kept weight is found
-// by a radix search of 11 + 11 + 10 bits (unsigned keys in the weights' order, NaN lowest); every CTA sums its share of the histogram's bins over the cluster and
-// hands the sums out (reading all histograms from every CTA took 12 us a pass).  Then ballots give every kept slot its place, in order; the weights move here.
+// k_evict_select: a cluster of CTAs has a head (one CTA for short caches) and holds its weights in shared memory: one read for all passes.  The smallest kept weight is looked for
+// from the top: a histogram over 2048 bins spread where such weights lie finds the bin that holds it, and the few weights of that bin are brought together and ranked; only where
+// they are many, or lie outside, does the search go on 11 bits at a time (unsigned keys in the weights' order, NaN lowest).  Every CTA sums its share of a histogram's bins over the
+// cluster and hands the sums out (reading all histograms from every CTA took 12 us a pass).  Three passes of 11 bits for all took 5.1 / 11.0 / 20.8 us at 1200 / 8192 / 131,072
+// slots of 4 heads, this 4.3 / 8.6 / 19.9.  Then ballots give every kept slot its place, in order; the weights move here.
 // k_evict_move: rows of a head are whole runs of memory, blocks of 64 of them a CTA.  In place, a block's destination may hold rows that others still have to read; kept slots are in order
 // and never before their place, so those are rows of at most two earlier blocks (the select kernel notes how many kept slots lie before every 64th).  A block reads its
 // rows into shared memory, says so, waits for those two, and writes.  Blocks are numbered as they start, so whom a block waits for has started before it.
@@ -17,8 +19,8 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048, EV_BLOCK = 64, EV_MOVE_THREADS = 256;
-constexpr int EV_UNIT = EV_WARPS * EV_BLOCK;          // slots of a CTA are a multiple of it: every warp has whole blocks
+constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048, EV_BLOCK = 64, EV_MOVE_THREADS = 256, EV_CAND = EV_THREADS, EV_RANK = 128;
+constexpr int EV_UNIT = EV_WARPS * EV_BLOCK, EV_PER = 32 * 32 * EV_WARPS;          // slots of a CTA are a multiple of the first (every warp has whole blocks) and at most the second (a lane for every 32 of a warp's)
 
 struct EvParams {
     char *k, *v; float* weights; int *kept, *ranks, *status; unsigned *flags;       // flags: [0] blocks started, then one per block: its rows are read
@@ -33,11 +35,18 @@ __device__ __forceinline__ unsigned ev_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// A first histogram's bin, in the keys' order: 64 an octave of the weights from 2^-22 to 2^10, where received attention lies, everything else in the outer two.  The keys' own upper bits
+// give four an octave, in which a warp's additions meet.
+constexpr int EV_SHIFT = 17;
+constexpr unsigned EV_FIRST = (0x80000000u >> EV_SHIFT) + ((127 - 22) << (23 - EV_SHIFT)) - 1;      // bin 0 ends with it
+__device__ __forceinline__ unsigned ev_bin(unsigned key) { return (unsigned)min(max((int)(key >> EV_SHIFT) - (int)EV_FIRST, 0), EV_BINS - 1); }
+
 template <int CL>
 __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_constant__ EvParams p) {
     extern __shared__ float w_s[];                     // [per]
     __shared__ unsigned hist[EV_BINS], total[EV_BINS];
-    __shared__ unsigned scan[EV_WARPS], found[2], warp_gt[EV_WARPS], warp_eq[EV_WARPS], counts[2];
+    __shared__ unsigned mine[EV_CAND], all[EV_CAND], few[EV_RANK];
+    __shared__ unsigned scan[EV_WARPS], found[4], warp_gt[EV_WARPS], warp_eq[EV_WARPS], counts[2], nmine, nfew;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = CL > 1 ? (int)cluster.block_rank() : 0, g = blockIdx.x / CL;
@@ -48,72 +57,135 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_con
     int* ranks = p.ranks + (long long)g * p.rank_head;
     const int cand = p.n - p.recent, want = p.keep - p.recent;
     const int begin = rank * p.per, len = max(0, min(p.n - begin, p.per)), clen = max(0, min(cand - begin, p.per));      // this CTA's slots, and those of them that compete
+    hist[tid] = 0; hist[tid + EV_THREADS] = 0;
+    if (tid == 0) nmine = nfew = 0;
+    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int i = blockIdx.x * EV_THREADS + tid; i < p.nflags; i += gridDim.x * EV_THREADS) p.flags[i] = 0u;
 #pragma unroll 8
-    for (int i = tid; i < len; i += EV_THREADS) w_s[i] = w[begin + i];
-    if (CL == 1 || want == 0) sync();                  // (else the first pass's barrier) every weight is read before any is written
-    // ---- the smallest kept key; `left`: how many of the keys with the bits found so far are kept
+    for (int i = tid; i < (len + 31) / 32 * 32; i += EV_THREADS) {
+        const float x = i < len ? w[begin + i] : 0.f;
+        const unsigned bin = ev_bin(ev_key(x)), low = __ballot_sync(0xffffffffu, i < clen && bin == 0);      // the slots that nothing looks at, in one addition
+        if (i < len) w_s[i] = x;
+        if (i < clen && bin > 0) atomicAdd(&hist[bin], 1u);
+        if (lane == 0 && low) atomicAdd(&hist[0], (unsigned)__popc(low));
+    }
+    sync();                                            // every weight is read before any is written
+    // ---- the smallest kept key: keys whose bits from `shift` up are `prefix` hold it, `count` of them, of which the `left` largest are kept
     unsigned prefix = want ? 0u : 0xffffffffu, left = (unsigned)want;
-    if (want)
+    if (want) {
+        int shift = 32, bins = EV_BINS;
+        bool spread = true;
 #pragma unroll 1
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048, up = shift + (pass == 2 ? 10 : 11);
-        hist[tid] = 0; hist[tid + EV_THREADS] = 0;
-        __syncthreads();
-        const unsigned above = pass == 0 ? 0 : prefix >> up;
+        while (true) {
+            // the bin in which the count from the top reaches `left`
+            const unsigned* sums = hist;
+            if (CL > 1) {
+                constexpr int SHARE = EV_BINS / CL;
+                if (tid < SHARE) {
+                    const int b = rank * SHARE + tid;
+                    unsigned c[CL], s = 0;
+#pragma unroll
+                    for (int r = 0; r < CL; r++) c[r] = *cluster.map_shared_rank(&hist[b], r);
+#pragma unroll
+                    for (int r = 0; r < CL; r++) s += c[r];
+#pragma unroll
+                    for (int r = 0; r < CL; r++) *cluster.map_shared_rank(&total[b], r) = s;
+                }
+                sync();
+                sums = total;
+            }
+            // two bins a thread, the highest first
+            const int top = bins - 1 - 2 * tid;
+            const unsigned c0 = top >= 0 ? sums[top] : 0u, c1 = top >= 1 ? sums[top - 1] : 0u, sum = c0 + c1;
+            unsigned inc = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) { const unsigned o = __shfl_up_sync(0xffffffffu, inc, d); if (lane >= d) inc += o; }
+            if (lane == 31) scan[warp] = inc;
+            __syncthreads();
+            const unsigned before = inc - sum + __reduce_add_sync(0xffffffffu, lane < warp ? scan[lane] : 0u);
+            if (before < left && before + sum >= left) {          // one thread
+                const bool first = before + c0 >= left;
+                found[0] = (unsigned)(first ? top : top - 1); found[1] = left - (first ? before : before + c0); found[2] = first ? c0 : c1;
+            }
+            __syncthreads();
+            const unsigned bin = found[0], count = found[2];
+            if (!spread) { prefix = prefix << (31 - __clz(bins)) | bin; left = found[1]; shift -= 31 - __clz(bins); }
+            else if (bin > 0 && bin < EV_BINS - 1) { prefix = EV_FIRST + bin; left = found[1]; shift = EV_SHIFT; }
+            const bool open = shift == 32;                          // an outer bin: nothing is known, from the start with the keys' own bits
+            spread = false;
+            if (shift == 0) break;
+            if (!open && count <= EV_CAND) {
+                // few enough for one a thread: bit by bit, each a count over the block, down to EV_RANK of them, then everyone's place among those (17 counts: 2.4 us)
 #pragma unroll 8
-        for (int i = tid; i < clen; i += EV_THREADS) {
-            const unsigned key = ev_key(w_s[i]);
-            if (pass == 0 || key >> up == above) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
-        }
-        sync();
-        const unsigned* sums = hist;
-        if (CL > 1) {
-            constexpr int SHARE = EV_BINS / CL;
-            if (tid < SHARE) {
-                const int b = rank * SHARE + tid;
-                unsigned c[CL], s = 0;
-#pragma unroll
-                for (int r = 0; r < CL; r++) c[r] = *cluster.map_shared_rank(&hist[b], r);
-#pragma unroll
-                for (int r = 0; r < CL; r++) s += c[r];
-#pragma unroll
-                for (int r = 0; r < CL; r++) *cluster.map_shared_rank(&total[b], r) = s;
+                for (int i = tid; i < clen; i += EV_THREADS) {
+                    const unsigned key = ev_key(w_s[i]);
+                    if (key >> shift == prefix) mine[atomicAdd(&nmine, 1u)] = key;
+                }
+                sync();
+                const unsigned* list = mine;
+                if (CL > 1) {
+                    if (warp < CL) {
+                        const unsigned nr = lane < CL ? *cluster.map_shared_rank(&nmine, lane) : 0u, at = __reduce_add_sync(0xffffffffu, lane < warp ? nr : 0u), n = __shfl_sync(0xffffffffu, nr, warp);
+                        const unsigned* from = cluster.map_shared_rank(mine, warp);
+                        for (unsigned i = lane; i < n; i += 32) all[at + i] = from[i];
+                    }
+                    __syncthreads();
+                    list = all;
+                }
+                bool in = tid < (int)count;
+                unsigned key = in ? list[tid] : 0u;
+                unsigned n = count, bit = 1u << (shift - 1);
+                prefix <<= shift;
+                for (; n > EV_RANK && bit; bit >>= 1) {
+                    const unsigned set = (unsigned)__syncthreads_count(in && (key & bit)), up = set >= left;
+                    if (up) prefix |= bit; else left -= set;
+                    n = up ? set : n - set;
+                    in = in && ((key & bit) != 0) == up;
+                }
+                if (bit) {                                          // (else all of them are equal)
+                    if (n < count) {
+                        if (in) few[atomicAdd(&nfew, 1u)] = key;
+                        __syncthreads();
+                        list = few;
+                        if (tid < (int)n) key = few[tid];
+                    }
+                    if (tid < (int)n) {                             // the first warps only
+                        unsigned more = 0, same = 0;
+#pragma unroll 16
+                        for (unsigned i = 0; i < n; i++) { const unsigned o = list[i]; more += o > key; same += o == key; }
+                        if (more < left && more + same >= left) { found[0] = key; found[3] = left - more; }          // equal keys write equal values
+                    }
+                    __syncthreads();
+                    prefix = found[0]; left = found[3];
+                }
+                break;
+            }
+            // the next eleven bits, or the last ones, of the keys that have these
+            const int bits = shift > 11 ? 11 : shift, down = shift - bits;
+            bins = 1 << bits;
+            sync();                                                 // everyone has read the sums before
+            hist[tid] = 0; hist[tid + EV_THREADS] = 0;
+            __syncthreads();
+#pragma unroll 8
+            for (int i = tid; i < clen; i += EV_THREADS) {
+                const unsigned key = ev_key(w_s[i]);
+                if (open || key >> shift == prefix) atomicAdd(&hist[(key >> down) & (bins - 1)], 1u);
             }
             sync();
-            sums = total;
         }
-        // two bins a thread, the highest first; the scan finds the bin in which the count reaches `left`
-        const int top = bins - 1 - 2 * tid;
-        const unsigned c0 = top >= 0 ? sums[top] : 0u, c1 = top >= 1 ? sums[top - 1] : 0u, sum = c0 + c1;
-        unsigned inc = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) { const unsigned o = __shfl_up_sync(0xffffffffu, inc, d); if (lane >= d) inc += o; }
-        if (lane == 31) scan[warp] = inc;
-        __syncthreads();
-        unsigned before = inc - sum;
-        {
-            const unsigned s = lane < warp ? scan[lane] : 0u;
-            before += __reduce_add_sync(0xffffffffu, s);
-        }
-        if (before < left && before + sum >= left) {          // one thread
-            const bool first = before + c0 >= left;
-            found[0] = (unsigned)(first ? top : top - 1); found[1] = left - (first ? before : before + c0);
-        }
-        __syncthreads();
-        prefix |= found[0] << shift; left = found[1];
     }
     // ---- kept: the last slots, keys above `prefix`, and the first `left` of those equal to it, in slot order.  A warp has a run of its CTA's slots.
     const int wper = p.per / EV_WARPS, wb = warp * wper, we = min(len, wb + wper);
-    unsigned gt = 0, eq = 0;
+    unsigned gt = 0, eq = 0, is_gt = 0, is_eq = 0;             // is_*: of the run's `lane`th 32 slots
 #pragma unroll 4
     for (int i = wb; i < we; i += 32) {
         const bool in = i + lane < we;
         const unsigned key = in ? ev_key(w_s[i + lane]) : 0u;
         const bool last = begin + i + lane >= cand;
-        gt += __popc(__ballot_sync(0xffffffffu, in && (last || key > prefix)));
-        eq += __popc(__ballot_sync(0xffffffffu, in && !last && key == prefix));
+        const unsigned bg = __ballot_sync(0xffffffffu, in && (last || key > prefix)), be = __ballot_sync(0xffffffffu, in && !last && key == prefix);
+        if (lane == (i - wb) / 32) { is_gt = bg; is_eq = be; }
+        gt += __popc(bg); eq += __popc(be);
     }
     if (lane == 0) { warp_gt[warp] = gt; warp_eq[warp] = eq; }
     __syncthreads();
@@ -128,16 +200,12 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_evict_select(const __grid_con
     const unsigned below = (1u << lane) - 1u;
 #pragma unroll 4
     for (int i = wb; i < we; i += 32) {
-        const bool in = i + lane < we;
-        const float x = in ? w_s[i + lane] : 0.f;
-        const unsigned key = ev_key(x);
-        const bool last = begin + i + lane >= cand, more = in && (last || key > prefix), same = in && !last && key == prefix;
-        const unsigned bg = __ballot_sync(0xffffffffu, more), be = __ballot_sync(0xffffffffu, same);
+        const unsigned bg = __shfl_sync(0xffffffffu, is_gt, (i - wb) / 32), be = __shfl_sync(0xffffffffu, is_eq, (i - wb) / 32);
         if (lane == 0 && i % EV_BLOCK == 0) ranks[(begin + i) / EV_BLOCK] = (int)(gt0 + min(eq0, left));
         const unsigned e = eq0 + __popc(be & below);
-        if (more || (same && e < left)) {
+        if ((bg >> lane & 1u) || ((be >> lane & 1u) && e < left)) {
             const unsigned at = gt0 + __popc(bg & below) + min(e, left);
-            kept[at] = begin + i + lane; w[at] = x;
+            kept[at] = begin + i + lane; w[at] = w_s[i + lane];
         }
         gt0 += __popc(bg); eq0 += __popc(be);
     }
@@ -206,8 +274,9 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) k_evict_move(const __grid_con
 struct EvPlan { int cluster, per, rank_head, blocks; size_t kept, ranks, flags, nflags, total; };
 EvPlan ev_plan(const it_cache_evict_args* a) {
     EvPlan pl;
-    // us for 4 heads of dimension 8 with 1 / 8 / 16 CTAs: 4096 slots 11.2 / 14.2 / 18.3, 8192 16.4 / 16.0 / 20.3, 32,768 38 / 21 / 25, 131,072 - / 42 / 40, 262,144 - / 56 / 48
-    pl.cluster = a->n <= 6144 ? 1 : a->n <= 98304 ? 8 : 16;
+    // us of the selection, 4 heads, with 1 / 8 / 16 CTAs a head: 1200 slots 4.3 / 7.2 / 11.0, 4096 7.7 / 8.5 / 12.0, 8192 11.0 / 8.6 / 12.2, 32,768 34.0 / 11.5 / 13.8,
+    // 65,536 - / 15.5 / 16.2, 131,072 - / 23.4 / 19.9, 262,144 - / 39.8 / 28.1
+    pl.cluster = a->n <= 5120 ? 1 : a->n <= 81920 ? 8 : 16;
     pl.per = (int)(((a->n + pl.cluster - 1) / pl.cluster + EV_UNIT - 1) / EV_UNIT * EV_UNIT);
     pl.rank_head = (int)((a->n + EV_BLOCK - 1) / EV_BLOCK + 1);
     pl.blocks = (int)((a->keep + EV_BLOCK - 1) / EV_BLOCK);
@@ -231,7 +300,7 @@ int ev_check_sizes(const it_cache_evict_args* a) {
 }
 
 template <int CL> int ev_prepare_select() {
-    IT_CUDA(cudaFuncSetAttribute(k_evict_select<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 32768 * 4));
+    IT_CUDA(cudaFuncSetAttribute(k_evict_select<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_PER * 4));
     if (CL > 8) IT_CUDA(cudaFuncSetAttribute(k_evict_select<CL>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     return IT_OK;
 }

@@ -491,6 +491,40 @@ def test_cache_evict(ops, n, keep, recent, kv, dim, what):
         assert torch.equal(w[h, :keep].view(torch.int32), w0[h, at].view(torch.int32)) and torch.equal(w[h, keep:].view(torch.int32), w0[h, keep:].view(torch.int32))
 
 
+@pytest.mark.parametrize("n", [1100, 2500, 7000, 90000])
+@pytest.mark.parametrize("together,equal", [(1, False), (127, False), (128, False), (129, False), (129, True), (600, False), (1024, False), (1024, True), (1025, False), (1025, True)])
+def test_cache_evict_weights_close_together(ops, n, together, equal):
+    """The smallest kept weight is one of `together` that agree in sign, exponent and six bits, at either end of them and in their middle; the others lie far on both sides."""
+    g = gen(n + together)
+    w = torch.cat((1.0 + torch.arange(together, device="cuda").float() * 2.0 ** -23 * (0 if equal else 117), torch.rand(n - together, generator=g, device="cuda") * 0.5))
+    w[together:][torch.rand(n - together, generator=g, device="cuda") < 0.4] += 3.0
+    w = w[torch.randperm(n, generator=g, device="cuda")]
+    above = int((w >= 3.0).sum())
+    for keep in {above + 1, above + (together + 1) // 2, above + together}:
+        kc, now = torch.arange(n, device="cuda").half()[:, None, None].expand(n, 1, 8).contiguous(), w[None].clone()
+        was, kept = kc.clone(), torch.empty(1, keep, dtype=torch.int32, device="cuda")
+        ops.cache_evict(kc, kc.clone(), now, n, keep, 0, kept)
+        at = torch.tensor(evict_plain(w.cpu(), n, keep, 0), dtype=torch.long, device="cuda")
+        assert torch.equal(kept[0].long(), at), keep
+        assert torch.equal(kc[:keep], was[at]) and torch.equal(now[0, :keep], w[at])
+
+
+@pytest.mark.parametrize("n", [900, 6000, 90000])
+@pytest.mark.parametrize("scale,shift", [(2.0 ** -40, 0.0), (2.0 ** 30, 0.0), (-1.0, 0.0), (2.0 ** -21, -2.0 ** -22), (2.0 ** 11, 0.0), (2.0 ** -149 * 900, 0.0)])
+def test_cache_evict_weights_of_any_size(ops, n, scale, shift):
+    """Weights far below one, far above, negative, around the ends of the range that the first histogram spreads over, and below the normal numbers."""
+    g = gen(n)
+    w = torch.rand(2, n, generator=g, device="cuda") * scale + shift
+    for keep, recent in ((1, 0), (n // 3, 5), (n - 1, 0)):
+        kc, now = randn(g, n, 2, 8).half(), w.clone()
+        was, kept = kc.clone(), torch.empty(2, keep, dtype=torch.int32, device="cuda")
+        ops.cache_evict(kc, kc.clone(), now, n, keep, recent, kept)
+        for h in range(2):
+            at = torch.tensor(evict_plain(w[h].cpu(), n, keep, recent), dtype=torch.long, device="cuda")
+            assert torch.equal(kept[h].long(), at), (keep, h)
+            assert torch.equal(kc[:keep, h], was[at, h]) and torch.equal(now[h, :keep].view(torch.int32), w[h, at].view(torch.int32))
+
+
 def test_cache_evict_layouts(ops):
     """[kv head][slot] caches, k and v in one buffer, weights and kept with strides, without kept (its own workspace), bf16."""
     g = gen(1)
