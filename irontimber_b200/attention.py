@@ -90,6 +90,7 @@ assert (_NORM_ROPE.size, _TREE.size, _EVICT.size) == (C.sizeof(NormRopeArgs), C.
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
 _current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 _NONE3 = (0, 0, 0)
+_MOST_CACHED = (1 << 30) - 1
 _F16, _BF16, _F32, _I32T = torch.float16, torch.bfloat16, torch.float32, torch.int32
 
 
@@ -205,7 +206,7 @@ def tree_attention(q, k_cache, v_cache, cached, out, parents=None, gate=None, sc
     wp, wh = _weights(weights, kv, cached + rows, index) if weights is not None else (0, 0)
     parents, length = _flat(parents, "parents", rows, _I32T, index), _flat(length, "length", 1, _I32T, index)
     if workspace is None:
-        workspace = _workspace(_tree_bytes(t, ct, rows, heads, kv, dim), index, stream)
+        workspace = _workspace(_tree_bytes(t, ct, rows, heads, kv, dim) if not wp else _tree_bytes(t, ct, rows, heads, kv, dim, min((cached | 4095) + 1, _MOST_CACHED), True), index, stream)
     else:
         _check_workspace(workspace, index)
     args = _TREE.pack(t, ct, rows, heads, kv, dim, *qp, *gp, *op, *kc, *vc, slots, cached, parents, length, wp, wh, workspace.data_ptr(), workspace.numel(), scale)
@@ -258,10 +259,10 @@ def _check_workspace(w, index):
 
 
 @functools.lru_cache(maxsize=256)
-def _tree_bytes(t, ct, rows, heads, kv, dim, cached=(1 << 30) - 1):
-    """Bytes of workspace; by default for any number of cached slots, which is what a call that allocates asks for (it depends on them only while they are few)."""
+def _tree_bytes(t, ct, rows, heads, kv, dim, cached=_MOST_CACHED, weights=False):
+    """Bytes of workspace.  A call that allocates asks for any number of cached slots if it has no weights (they then matter only while they are few), else for the next 4096."""
     need = C.c_size_t()
-    _lib.check(_lib.load().it_tree_attention_workspace(C.byref(TreeAttentionArgs(t, ct, rows, heads, kv, dim, cached=cached)), C.byref(need)))
+    _lib.check(_lib.load().it_tree_attention_workspace(C.byref(TreeAttentionArgs(t, ct, rows, heads, kv, dim, cached=cached, weights=256 if weights else None)), C.byref(need)))
     return need.value
 
 
@@ -273,7 +274,7 @@ def cache_evict_workspace(kv_heads, n, keep):
     return need.value
 
 
-def tree_attention_workspace(rows, heads, kv_heads, head_dim, cached, dtype=torch.float32):
-    """Bytes of workspace for a call of these sizes."""
+def tree_attention_workspace(rows, heads, kv_heads, head_dim, cached, dtype=torch.float32, weights=False):
+    """Bytes of workspace for a call of these sizes, with weights or without; enough for fewer cached slots too."""
     t = TYPES.get(dtype, -1)
-    return _tree_bytes(t, 1 if t == 0 else t, rows, heads, kv_heads, head_dim, cached)
+    return _tree_bytes(t, 1 if t == 0 else t, rows, heads, kv_heads, head_dim, cached, bool(weights))

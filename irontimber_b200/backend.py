@@ -277,7 +277,7 @@ class CudaBackend:
         orders its uses, those of recorded graphs too, and a larger one does not replace one that a recorded graph knows."""
         from . import attention
         if options.get("workspace") is None:
-            options["workspace"] = self._workspace(attention.tree_attention_workspace(q.shape[0], q.shape[1], k_cache.shape[1], q.shape[2], (1 << 30) - 1, q.dtype))
+            options["workspace"] = self._workspace(attention.tree_attention_workspace(q.shape[0], q.shape[1], k_cache.shape[1], q.shape[2], min(k_cache.shape[0], (1 << 30) - 1), q.dtype, options.get("weights") is not None))
         attention.tree_attention(q, k_cache, v_cache, cached, out, stream=self.torch_stream, **options)
 
     def cache_evict(self, k_cache, v_cache, weights, n, keep, recent, kept=None, **options):

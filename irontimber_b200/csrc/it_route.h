@@ -90,6 +90,10 @@ static inline bool it_gdn_rows_takes(int sd, int nt) { return sd == 128 && nt >=
 // have to be in one GPC, which holds 16 of them or more, and where eight GPCs cannot have all clusters at once the others' second wave costs more (24 clusters
 // of six, 30,011 slots: 231 us against 107).
 #define IT_TREE_JOIN 8                             // runs that join in a cluster, at most: the portable size
+// Whether scores are kept for the received weights, 4 bytes a product row and slot of workspace, instead of being formed again by a second walk over K: while they take no more
+// memory than the K and V that are read, or have 64 rows.
+#define IT_TREE_SCORES 256
+static inline bool it_tree_keeps_scores(long prows, int head_dim) { return prows <= 64 || (prows <= head_dim && prows <= IT_TREE_SCORES); }
 struct it_tree_cut { int nr, row_tiles, splits; bool joined; };
 static inline it_tree_cut it_tree_cut_by(int nr, long prows, long kv_heads, long tiles, int sm_count) {
     it_tree_cut c;

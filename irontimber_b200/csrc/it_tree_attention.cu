@@ -17,15 +17,86 @@
 
 namespace {
 
+constexpr int TA_JOINROWS = 8;                    // product rows whose received weights are formed beside the joining of runs, at most
+
+// weights[g][slot] += ex2(score - reference) / sum over the product rows, from the scores that k_tree_attention_tc left.  CTA b has one tile of slots or, where the rows are few, several; a lane
+// has four slots, and the sums of the warps that share a tile meet in a fixed order.  Latency and L2: 4 bytes a row and slot, written and read, in place of a second walk over K with its
+// products (9 rows at 8192 slots: 30.5 us for the call with the walk).  JOIN: references and sums are those of runs, and joined here, so that few rows' weights need not wait for a kernel more;
+// many rows' would be read by every CTA (60 rows at 30,000 slots: 68 us for the call against 49).
+template <int WARPS, bool JOIN> __device__ __forceinline__ void ta_weigh(const TaParams& p, int b, int g, int tid) {
+    __shared__ float part[WARPS][TA_KEYS];
+    __shared__ float2 stat[JOIN ? TA_JOINROWS : 1];
+    const int warp = tid >> 5, lane = tid & 31, groups = p.tile_warps, first = warp % groups, tile = b * (WARPS / groups) + warp / groups;
+    const int total = ta_cached(p) + p.rows, rows = tile * TA_KEYS < total ? p.prows : 0;
+    const float* const s = p.scores + (long long)g * p.prows * p.s_row + (long long)tile * TA_KEYS + 4 * lane;
+    const float2* const stats = p.stats + (size_t)g * p.pad_rows;
+    constexpr int AHEAD = 4;
+    float4 x[AHEAD];
+    float2 e[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) {
+        const int r = first + k * groups;
+        x[k] = r < rows ? __ldcg(reinterpret_cast<const float4*>(s + r * p.s_row)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        e[k] = !JOIN && r < rows ? __ldcg(stats + r) : make_float2(0.f, 0.f);
+    }
+    if constexpr (JOIN) {
+#pragma unroll 1
+        for (int r = warp; r < p.prows; r += WARPS) {
+            float2 f[(TA_MAXSPLITS + 31) / 32];
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < (TA_MAXSPLITS + 31) / 32; k++) {
+                const int q = lane + 32 * k;
+                f[k] = q < p.splits ? __ldcg(&p.part_ml[((size_t)q * p.kv_heads + g) * p.pad_rows + r]) : make_float2(-INFINITY, 0.f);
+            }
+#pragma unroll
+            for (int k = 0; k < (TA_MAXSPLITS + 31) / 32; k++) top = fmaxf(top, f[k].x);
+#pragma unroll
+            for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < (TA_MAXSPLITS + 31) / 32; k++) sum += f[k].y * ex2(f[k].x - ref);
+#pragma unroll
+            for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+            if (lane == 0) stat[r] = make_float2(ref, sum);
+        }
+        __syncthreads();
+    }
+    float a[4] = { 0.f, 0.f, 0.f, 0.f };
+    auto add = [&](const float4& v, float2 st) {
+        const float inv = st.y == 0.f ? 0.f : 1.f / st.y;
+        a[0] = fmaf(ex2(v.x - st.x), inv, a[0]); a[1] = fmaf(ex2(v.y - st.x), inv, a[1]); a[2] = fmaf(ex2(v.z - st.x), inv, a[2]); a[3] = fmaf(ex2(v.w - st.x), inv, a[3]);
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; k++) if (first + k * groups < rows) add(x[k], JOIN ? stat[first + k * groups] : e[k]);
+#pragma unroll 4
+    for (int r = first + AHEAD * groups; r < rows; r += groups) add(__ldcg(reinterpret_cast<const float4*>(s + r * p.s_row)), JOIN ? stat[r] : __ldcg(stats + r));
+    store4(&part[warp][4 * lane], a);
+    __syncthreads();
+    for (int k = tid; k < WARPS / groups * TA_KEYS; k += 32 * WARPS) {
+        const int w0 = k / TA_KEYS * groups, c = k % TA_KEYS;
+        const long long slot = (long long)b * (WARPS / groups) * TA_KEYS + k;
+        if (slot >= total) break;
+        float sum = part[w0][c];
+        for (int w = 1; w < groups; w++) sum += part[w0 + w][c];
+        p.weights[g * p.w_head + slot] += sum;
+    }
+}
+
 // Joins the runs of one product row: out = sum of the runs' outputs, each scaled to the common reference, over the sum of their sums, in a fixed order.  Four groups of
 // HD / 4 threads take every fourth run; runs that saw nothing are not read.  Latency: the gate and the first outputs are asked for before the weights are known, and every
-// warp forms the weights of all runs for itself instead of meeting the others.
+// warp forms the weights of all runs for itself instead of meeting the others.  CTAs behind the rows' form received weights.
 template <class TA, int NB>
 __global__ void __launch_bounds__(64 * NB) k_tree_join(const __grid_constant__ TaParams p) {
     constexpr int HD = 64 * NB, LANES = HD / 4, WARPS = 2 * NB, AHEAD = 4;
     __shared__ float wgt[WARPS][TA_MAXSPLITS];
     __shared__ float4 acc[3][LANES];
     const int tid = threadIdx.x, r = blockIdx.x, g = blockIdx.y, warp = tid >> 5, lane = tid & 31;
+    if (r >= p.prows) {
+        asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
+        ta_weigh<WARPS, true>(p, r - p.prows, g, tid);
+        return;
+    }
     const int grp = tid / LANES, c = tid % LANES * 4;
     const int t = ta_row(p, r), h = g * p.group + r - t * p.group;
     float z[4] = { 0.f, 0.f, 0.f, 0.f };
@@ -81,9 +152,15 @@ __global__ void __launch_bounds__(64 * NB) k_tree_join(const __grid_constant__ T
     store4((TA*)p.out + t * p.o_row + h * p.o_head + c, out);
 }
 
+// The received weights of runs that have joined.
+__global__ void __launch_bounds__(256) k_tree_weights(const __grid_constant__ TaParams p) {
+    asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
+    ta_weigh<8, false>(p, blockIdx.x, blockIdx.y, threadIdx.x);
+}
+
 // ---- host side ---------------------------------------------------------------------------------------------------------------
 // How a call is cut: rows of a CTA's product tile, tiles of product rows, runs of the cache.
-struct TaPlan { int nb, nr, pad_rows, row_tiles, splits; bool joined; size_t part_o, part_ml, stats, total; };
+struct TaPlan { int nb, nr, pad_rows, row_tiles, splits; bool joined, scores; size_t part_o, part_ml, stats, kept, total; };
 
 long ta_tiles(const it_tree_attention_args* a) { return ((long)a->cached + a->rows + TA_KEYS - 1) / TA_KEYS; }
 TaPlan ta_plan(const it_tree_attention_args* a, const it_tree_cut& c) {
@@ -97,7 +174,10 @@ TaPlan ta_plan(const it_tree_attention_args* a, const it_tree_cut& c) {
     pl.part_o = 0;
     pl.part_ml = !pl.joined ? up(splits * rows * 64 * pl.nb * 4) : 0;
     pl.stats = pl.part_ml + (!pl.joined ? up(splits * rows * 8) : 0);
-    pl.total = pl.stats + up(rows * 8);        // the statistics of a call without weights are not kept, but sizes do not depend on pointers
+    pl.kept = pl.stats + up(rows * 8);
+    const size_t prows = (size_t)a->rows * (a->heads / a->kv_heads);
+    pl.scores = a->weights && it_tree_keeps_scores((long)prows, a->head_dim);
+    pl.total = pl.kept + (pl.scores ? prows * a->kv_heads * ta_tiles(a) * TA_KEYS * 4 : 0);
     return pl;
 }
 
@@ -128,14 +208,24 @@ int ta_prepare(int device) {
     if (done[device]) return IT_OK;
     if (const int r = it_tree_tc_prepare()) return r;
     auto load = [](auto kern) -> int { cudaFuncAttributes at; IT_CUDA(cudaFuncGetAttributes(&at, kern)); return IT_OK; };
-    for (const int r : { load(k_tree_join<float, 2>), load(k_tree_join<float, 4>), load(k_tree_join<__half, 2>), load(k_tree_join<__half, 4>), load(k_tree_join<__nv_bfloat16, 2>), load(k_tree_join<__nv_bfloat16, 4>) })
+    for (const int r : { load(k_tree_join<float, 2>), load(k_tree_join<float, 4>), load(k_tree_join<__half, 2>), load(k_tree_join<__half, 4>), load(k_tree_join<__nv_bfloat16, 2>), load(k_tree_join<__nv_bfloat16, 4>), load(k_tree_weights) })
         if (r) return r;
     done[device] = true;
     return IT_OK;
 }
 
-int ta_join(const TaParams& p, int type, int nb, cudaStream_t st) {
-    auto go = [&](auto kern) -> int { IT_CUDA(it_launch_early(kern, dim3(p.prows, p.kv_heads), dim3(64 * nb), 0, st, 1, p)); return IT_OK; };
+// CTAs of `warps` warps that form received weights.  All warps of one share a tile, or, where there are many tiles, as many as have four rows each (one row at 30,000 slots: 33.5 us for the call
+// with a tile a CTA, 29.3).
+int ta_weigh_ctas(TaParams& p, int warps) {
+    const int tiles = (p.cached + p.rows + TA_KEYS - 1) / TA_KEYS;
+    p.tile_warps = warps;
+    while (p.tile_warps > 1 && 4 * (p.tile_warps / 2) >= p.prows && (long)tiles * p.kv_heads > 2 * TA_MAXSPLITS) p.tile_warps /= 2;
+    const int each = warps / p.tile_warps;
+    return (tiles + each - 1) / each;
+}
+int ta_join(TaParams& p, int type, int nb, cudaStream_t st) {
+    const int more = p.scores && p.prows <= TA_JOINROWS ? ta_weigh_ctas(p, 2 * nb) : 0;
+    auto go = [&](auto kern) -> int { IT_CUDA(it_launch_early(kern, dim3(p.prows + more, p.kv_heads), dim3(64 * nb), 0, st, 1, p)); return IT_OK; };
     if (type == IT_F32) return nb == 2 ? go(k_tree_join<float, 2>) : go(k_tree_join<float, 4>);
     if (type == IT_F16) return nb == 2 ? go(k_tree_join<__half, 2>) : go(k_tree_join<__half, 4>);
     return nb == 2 ? go(k_tree_join<__nv_bfloat16, 2>) : go(k_tree_join<__nv_bfloat16, 4>);
@@ -199,13 +289,18 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     TaParams p;
     char* ws = (char*)a->workspace;
     p.q = a->q; p.gate = a->gate; p.out = a->out; p.parents = a->parents; p.length = a->length; p.weights = a->weights;
-    p.part_o = (float*)(ws + pl.part_o); p.part_ml = (float2*)(ws + pl.part_ml); p.stats = a->weights ? (float2*)(ws + pl.stats) : nullptr; p.status = dev.status_dev;
-    p.q_row = a->q_row; p.q_head = a->q_head; p.g_row = a->g_row; p.g_head = a->g_head; p.o_row = a->o_row; p.o_head = a->o_head; p.w_head = a->w_head;
+    p.part_o = (float*)(ws + pl.part_o); p.part_ml = (float2*)(ws + pl.part_ml); p.stats = a->weights ? (float2*)(ws + pl.stats) : nullptr; p.scores = pl.scores ? (float*)(ws + pl.kept) : nullptr; p.status = dev.status_dev;
+    p.q_row = a->q_row; p.q_head = a->q_head; p.g_row = a->g_row; p.g_head = a->g_head; p.o_row = a->o_row; p.o_head = a->o_head; p.w_head = a->w_head; p.s_row = (long long)ta_tiles(a) * TA_KEYS;
     p.rows = a->rows; p.heads = a->heads; p.group = a->heads / a->kv_heads; p.kv_heads = a->kv_heads; p.dim = a->head_dim; p.cached = (int)a->cached; p.splits = pl.splits;
-    p.prows = a->rows * p.group; p.pad_rows = pl.pad_rows; p.joined = pl.joined; p.group_inv = (unsigned)((0x100000000ull + p.group - 1) / p.group); p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale;
+    p.prows = a->rows * p.group; p.pad_rows = pl.pad_rows; p.joined = pl.joined; p.tile_warps = 8; p.group_inv = (unsigned)((0x100000000ull + p.group - 1) / p.group); p.scale = a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale;
     const cudaStream_t st = (cudaStream_t)stream;
     if (const int r = it_tree_tc_run(p, a->type, pl.nb, pl.nr, pl.row_tiles, km, vm, st)) return r;
     if (!p.joined) if (const int r = ta_join(p, a->type, pl.nb, st)) return r;
+    if (p.scores) {
+        const int ctas = ta_weigh_ctas(p, 8);
+        if (p.joined || p.prows > TA_JOINROWS) IT_CUDA(it_launch_early(k_tree_weights, dim3(ctas, p.kv_heads), dim3(256), 0, st, 1, p));
+        return IT_OK;
+    }
     // the second walk has no runs to cut: as many product rows at once as there are, up to 64
     return p.weights ? it_tree_tc_weigh(p, a->type, pl.nb, p.prows <= 16 ? 16 : p.prows <= 32 ? 32 : 64, km, st) : IT_OK;
 }

@@ -7,9 +7,9 @@
 // What a kernel of a call gets.
 struct TaParams {
     const void *q, *gate; void* out; const int *parents, *length; float* weights;
-    float* part_o; float2* part_ml; float2* stats; int* status;
-    long long q_row, q_head, g_row, g_head, o_row, o_head, w_head;
-    int rows, heads, group, kv_heads, dim, cached, splits, prows, pad_rows, joined; unsigned group_inv; float scale;
+    float* part_o; float2* part_ml; float2* stats; float* scores; int* status;          // scores: [kv head][product row][slot] in log2 units, null if they are not kept
+    long long q_row, q_head, g_row, g_head, o_row, o_head, w_head, s_row;
+    int rows, heads, group, kv_heads, dim, cached, splits, prows, pad_rows, joined, tile_warps; unsigned group_inv; float scale;
 };
 
 // it_tree_attention_tc.cu.  nb: 64-element pieces of a head, nr: product rows of a CTA (16, 32 or 64).

@@ -348,6 +348,13 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 const float *const f = fac + wg * RW, *const bs = base_s + wg * RW;
                 float* const c = corr_s + (i & 1) * NR + wg * RW;
                 bool move = i == 0 || masked;
+                const unsigned see = masked ? (i == first_masked ? vis[0] : i == first_masked + 1 ? vis[1] : vis[2]) : 0xffffffffu;
+                if (p.scores) {                                     // for the received weights
+                    float* const s = p.scores + ((long long)g * p.prows + r0 + wg * RW) * p.s_row + (tile0 + i) * TA_KEYS + key;
+#pragma unroll
+                    for (int r = 0; r < RW; r++)
+                        if (r0 + wg * RW + r < p.prows) __stcg(s + r * p.s_row, (see >> r) & 1u ? x[r] * f[r] : -INFINITY);
+                }
                 float y[RW];
                 if (!move) {
                     float top = -INFINITY;
@@ -356,7 +363,6 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     move = group_any(wg, top > TC_TOP);             // the same answer in all four warps
                 }
                 if (move) {
-                    const unsigned see = masked ? (i == first_masked ? vis[0] : i == first_masked + 1 ? vis[1] : vis[2]) : 0xffffffffu;
 #pragma unroll
                     for (int r = 0; r < RW; r++) {
                         x[r] = (see >> r) & 1u ? x[r] * f[r] : -INFINITY;
@@ -589,7 +595,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     }
 }
 
-// ---- received weight --------------------------------------------------------------------------------------------------------
+// ---- received weight, of more product rows than k_tree_weights (it_tree_attention.cu) is for -----------------------------------
 // The scores of a 128-slot tile once more, against the finished reference and sum of every product row: a thread has a slot and adds up its columns, so that nothing crosses
 // threads but the two groups' halves.  A CTA walks tiles of a KV head; up to NR product rows are brought in once, more of them NR at a time for every tile.  The next scores are
 // formed while the last ones' exponentials are, and the next tile of K is on its way (one tile a CTA: 21 us at 8192 slots and 9 rows, most of it start-up).

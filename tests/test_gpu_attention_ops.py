@@ -290,6 +290,29 @@ def test_device_length(ops):
             assert not got[:, real + rows:].any()
 
 
+@pytest.mark.parametrize("rows,heads,kv,dim", [(1, 8, 1, 128), (4, 4, 2, 64), (3, 9, 3, 128), (9, 6, 6, 40), (8, 16, 2, 256), (13, 5, 1, 64), (13, 5, 1, 72), (16, 16, 2, 128), (43, 3, 1, 128), (64, 8, 2, 256), (37, 7, 1, 256)])
+@pytest.mark.parametrize("cached,most", [(0, 0), (120, 120), (129, 700), (2300, 2300), (9000, 9000), (700, 41000)])
+def test_received_weights_of_few_and_many_rows(ops, rows, heads, kv, dim, cached, most):
+    """Product rows and lengths on both sides of every choice; `length` below `cached`; NaN and infinities where nobody looks; what lies behind the last slot stays."""
+    q, kc, vc, g = make("f32", rows, most, heads, kv, dim, rows + cached)
+    kc[cached + rows:], vc[cached + rows:] = math.nan, math.inf
+    parents = random_parents(rows, dim)
+    par = torch.tensor(parents, dtype=torch.int32, device="cuda")
+    was = torch.rand(kv, most + rows + 5, generator=g, device="cuda")
+    out, got = torch.empty_like(q), was.clone()
+    length = torch.tensor([cached], dtype=torch.int32, device="cuda") if cached != most else None
+    ops.tree_attention(q, kc, vc, most, out, parents=par, length=length, weights=got)
+    want, tol, rec, rtol = tree_64(q, kc, vc, cached, parents, None, 0, torch.float32)
+    n = cached + rows
+    near(out, want, tol, "out")
+    near(got[:, :n], was[:, :n].double() + rec, rtol + 2 * H32 * (was[:, :n] + rec), "weights")
+    assert torch.equal(got[:, n:], was[:, n:])
+    more = was.clone()                      # a workspace for a longer cache, with what the last call left in it
+    ws = torch.full((ops.tree_attention_workspace(rows, heads, kv, dim, 2 * most + 1, weights=True),), 255, dtype=torch.uint8, device="cuda")
+    ops.tree_attention(q, kc, vc, most, out, parents=par, length=length, weights=more, workspace=ws)
+    assert torch.equal(more, got)
+
+
 def test_parents_that_are_not_smaller_rows_count_as_none(ops):
     q, kc, vc, g = make("f16", 6, 70, 4, 2, 64, 8)
     bad = [3, 1, 0, 2, 1 << 30, -9]           # forward, itself, fine, fine, far away, negative
