@@ -1,4 +1,4 @@
-// Attention of a token, a chain or a tree of drafted tokens over a KV cache that the caller owns: host side, and the kernel that joins runs of the cache.  Stands where
+// Attention of a token, a chain or a tree of drafted tokens over a KV cache that the caller owns: host side, and the kernels that join runs of the cache and form received weights.  Stands where
 // VkEngine records its attention dispatch (src/vk/mod.rs:833-840; CPU: src/cpu.rs:177-186), for any strides and lengths; sums are those of a softmax over runs of
 // the cache, not the reference's position order.
 //
@@ -11,6 +11,8 @@
 // done twice; the f16 cache is exact.  16-bit activations: p is rounded to the cache's type like the output itself, q is exact.
 // Masks: only tiles that reach behind the cached slots look at them.  A masked score is replaced, whatever it was; there a non-finite V element is
 // taken out of the product and added to the rows that do see it (0 * inf would be NaN in those that do not).
+// Received weights need the finished references and sums: the one pass leaves its scores, and a small kernel turns them into weights; for so many product rows that the scores would be larger than
+// the cache, K is walked a second time (k_tree_weights_tc).
 #include "it_tree_attention.cuh"
 #include "it_route.h"
 #include <mutex>

@@ -7,7 +7,7 @@
 //   Q               rows of 128-byte pieces, K-major; f32 activations as two sets of columns, high and low halves, added in f32 when they are read
 //   P               [slot][column], MN-major: a thread has one slot (a lane of tensor memory) and stores its columns as 16-byte pieces
 // Softmax warps (two or four groups of four; a group has its share of the columns): scores out of tensor memory, exponentials against a reference that moves only when
-// it has to (redux over the slots of a warp, an ordered atomicMax over the four), P; then the tile before: O^T out of tensor memory into f32 accumulators in registers.  Every tile's product starts from zero and is
+// it has to (its maximum over a warp's slots by halving what a lane carries, over the four warps by an ordered atomicMax), P; then the tile before: O^T out of tensor memory into f32 accumulators in registers.  Every tile's product starts from zero and is
 // added with a rounded f32 addition: chained over a long run in tensor memory the hardware's truncating accumulation loses f32's last bits (1.3e-5 of the result after 240 tiles of 64
 // slots chained in mma.sync accumulators).  Two warps copy, one issues whichever product has its inputs, the next tile's scores or this tile's O.
 // What bounds it: 64 columns of f32 activations (128 with the low halves) 2 x 1024 tensor cycles a tile of 128 slots at head dimension 256; few columns: HBM.
