@@ -277,7 +277,7 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     IT_CHECK_ARG(a->scale == a->scale && a->scale <= 3e38f && a->scale >= -3e38f, "%s: bad scale", who);
     const size_t os = it_span(T, a->o_row, H, a->o_head, D, es);
     auto same = [&](const void* x, int64_t row, int64_t head) { return x == a->out && (T < 2 || row == a->o_row) && (H < 2 || head == a->o_head); };
-    // the received weights read q again after out is written
+    // a second walk for the received weights reads q after out is written
     IT_CHECK_ARG((same(a->q, a->q_row, a->q_head) && !a->weights) || !it_overlap(a->q, it_span(T, a->q_row, H, a->q_head, D, es), a->out, os), "%s: out overlaps q", who);
     IT_CHECK_ARG(!a->gate || same(a->gate, a->g_row, a->g_head) || !it_overlap(a->gate, it_span(T, a->g_row, H, a->g_head, D, es), a->out, os), "%s: out overlaps gate", who);
     it_ops_device dev;
