@@ -402,8 +402,8 @@ typedef struct it_tree_attention_args {
 } it_tree_attention_args;
 int it_tree_attention(void* stream, const it_tree_attention_args* a);
 int it_tree_attention_workspace(const it_tree_attention_args* a, size_t* nbytes);    /* looks at sizes, and at whether weights are asked for; grows with `cached`: up to a bound
-                                                                                         * without weights, with them by 4 rows * heads bytes a slot while rows * heads / kv_heads
-                                                                                         * is at most 64 or head_dim */
+                                                                                         * without weights, with them by 4 rows * heads bytes a slot up to 256 MB, beyond that
+                                                                                         * while rows * heads / kv_heads is at most 64 or head_dim */
 
 /* Cuts a cache of n slots down to `keep` per kv head: the last `recent` slots stay, and of the others the keep - recent with the largest weight
  * (equal weights: the lower slot; NaN ranks below everything; -0 equals 0).  What stays moves to slots 0..keep-1 in its old order, in place, in k_cache, v_cache

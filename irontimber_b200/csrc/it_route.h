@@ -91,9 +91,12 @@ static inline bool it_gdn_rows_takes(int sd, int nt) { return sd == 128 && nt >=
 // of six, 30,011 slots: 231 us against 107).
 #define IT_TREE_JOIN 8                             // runs that join in a cluster, at most: the portable size
 // Whether scores are kept for the received weights, 4 bytes a product row and slot of workspace, instead of being formed again by a second walk over K: while they take no more
-// memory than the K and V that are read, or have 64 rows.
-#define IT_TREE_SCORES 256
-static inline bool it_tree_keeps_scores(long prows, int head_dim) { return prows <= 64 || (prows <= head_dim && prows <= IT_TREE_SCORES); }
+// memory than the K and V that are read (or have 64 rows), or 256 MB.  us for the call, kept / walk: 64 rows of 24 over 4 heads of 256 at 500 slots 41 / 57, at 8190 88 / 103, at 30,000
+// 210 / 256; 40 rows, bf16, 32 over 8 of 128 at 20,000 111 / 121.
+#define IT_TREE_SCORE_BYTES (256l << 20)
+static inline bool it_tree_keeps_scores(long prows, long kv_heads, int head_dim, long tiles) {
+    return prows <= (head_dim > 64 ? head_dim : 64) || prows * kv_heads * tiles <= IT_TREE_SCORE_BYTES / (4 * 128);
+}
 struct it_tree_cut { int nr, row_tiles, splits; bool joined; };
 static inline it_tree_cut it_tree_cut_by(int nr, long prows, long kv_heads, long tiles, int sm_count) {
     it_tree_cut c;

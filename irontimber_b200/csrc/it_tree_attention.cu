@@ -11,8 +11,8 @@
 // done twice; the f16 cache is exact.  16-bit activations: p is rounded to the cache's type like the output itself, q is exact.
 // Masks: only tiles that reach behind the cached slots look at them.  A masked score is replaced, whatever it was; there a non-finite V element is
 // taken out of the product and added to the rows that do see it (0 * inf would be NaN in those that do not).
-// Received weights need the finished references and sums: the one pass leaves its scores, and a small kernel turns them into weights; for so many product rows that the scores would be larger than
-// the cache, K is walked a second time (k_tree_weights_tc).
+// Received weights need the finished references and sums: the one pass leaves its scores, and a small kernel turns them into weights; where the scores would take too much
+// memory, K is walked a second time (k_tree_weights_tc).
 #include "it_tree_attention.cuh"
 #include "it_route.h"
 #include <mutex>
@@ -178,7 +178,7 @@ TaPlan ta_plan(const it_tree_attention_args* a, const it_tree_cut& c) {
     pl.stats = pl.part_ml + (!pl.joined ? up(splits * rows * 8) : 0);
     pl.kept = pl.stats + up(rows * 8);
     const size_t prows = (size_t)a->rows * (a->heads / a->kv_heads);
-    pl.scores = a->weights && it_tree_keeps_scores((long)prows, a->head_dim);
+    pl.scores = a->weights && it_tree_keeps_scores((long)prows, a->kv_heads, a->head_dim, ta_tiles(a));
     pl.total = pl.kept + (pl.scores ? prows * a->kv_heads * ta_tiles(a) * TA_KEYS * 4 : 0);
     return pl;
 }
@@ -257,6 +257,8 @@ IT_API int it_tree_attention_workspace(const it_tree_attention_args* a, size_t* 
         if (n > *nbytes) *nbytes = n;
         if (c.row_tiles == 1) break;
     }
+    const long prows = (long)a->rows * (a->heads / a->kv_heads);
+    if (a->rows && a->weights && !it_tree_keeps_scores(prows, a->kv_heads, a->head_dim, ta_tiles(a))) *nbytes += IT_TREE_SCORE_BYTES;       // a shorter cache's would be kept
     return IT_OK;
 }
 
@@ -303,6 +305,5 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
         if (p.joined || p.prows > TA_JOINROWS) IT_CUDA(it_launch_early(k_tree_weights, dim3(ctas, p.kv_heads), dim3(256), 0, st, 1, p));
         return IT_OK;
     }
-    // the second walk has no runs to cut: as many product rows at once as there are, up to 64
-    return p.weights ? it_tree_tc_weigh(p, a->type, pl.nb, p.prows <= 16 ? 16 : p.prows <= 32 ? 32 : 64, km, st) : IT_OK;
+    return p.weights ? it_tree_tc_weigh(p, a->type, pl.nb, km, st) : IT_OK;
 }

@@ -15,7 +15,7 @@ struct TaParams {
 // it_tree_attention_tc.cu.  nb: 64-element pieces of a head, nr: product rows of a CTA (16, 32 or 64).
 int it_tree_tc_prepare();
 int it_tree_tc_run(const TaParams& p, int type, int nb, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st);
-int it_tree_tc_weigh(const TaParams& p, int type, int nb, int nr, const CUtensorMap& km, cudaStream_t st);
+int it_tree_tc_weigh(const TaParams& p, int type, int nb, const CUtensorMap& km, cudaStream_t st);
 
 namespace {
 

@@ -595,11 +595,11 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
     }
 }
 
-// ---- received weight, of more product rows than k_tree_weights (it_tree_attention.cu) is for -----------------------------------
+// ---- received weight, where the scores are not kept -----------------------------------------------------------------------------
 // The scores of a 128-slot tile once more, against the finished reference and sum of every product row: a thread has a slot and adds up its columns, so that nothing crosses
-// threads but the two groups' halves.  A CTA walks tiles of a KV head; up to NR product rows are brought in once, more of them NR at a time for every tile.  The next scores are
+// threads but the two groups' halves.  A CTA walks tiles of a KV head; product rows are brought in NR at a time for every tile.  The next scores are
 // formed while the last ones' exponentials are, and the next tile of K is on its way (one tile a CTA: 21 us at 8192 slots and 9 rows, most of it start-up).
-constexpr int TW_THREADS = 256;
+constexpr int TW_THREADS = 256, TW_ROWS = 64;
 template <bool SPLIT, int NB, int NR> struct TcWeights {
     using A = TcTree<SPLIT, NB, NR>;
     static constexpr int Q = 0, K = A::QB, ANC = K + 2 * A::SLOT, JUMP = ANC + TA_MAXROWS * TA_WORDS * 4, ROW = JUMP + TA_MAXROWS * 4, HALF = ROW + 3 * 4 * NR * 4, BARS = HALF + 2 * TA_KEYS * 4, TMEM = BARS + 32,
@@ -692,7 +692,7 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
             const bool last = i + 1 == steps;
             if (last && tid == 0 && j + 2 < nt && ok) load(j + 2);    // every product with this tile is done
             if (!last || j + 1 < nt) {
-                if (steps > 1) bring(last ? 0 : i + 1, q + 1);        // the products of step q are done with Q
+                bring(last ? 0 : i + 1, q + 1);                       // the products of step q are done with Q
                 fence_before();
                 __syncthreads();                                      // everyone has read the scores of step q - 1
                 issue(last ? j + 1 : j, q + 1);
@@ -708,7 +708,7 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
                 for (int r = 0; r < RW; r++) { asm volatile("" : "+f"(y[r])); x[r] += y[r]; }
             } else tm_wait(x);
             fence_before();
-            const float* const rw = row + (steps > 1 ? q % 3 : 0) * 4 * NR + wg * RW;
+            const float* const rw = row + q % 3 * 4 * NR + wg * RW;
             if (!masked) {
 #pragma unroll
                 for (int r = 0; r < RW; r++) sum = fmaf(ex2(fmaf(x[r], rw[r], -rw[NR + r])), rw[2 * NR + r], sum);
@@ -748,13 +748,14 @@ template <class T, bool SPLIT, int NB, int NR> int prepare_shape() {
     IT_CUDA(cudaFuncGetAttributes(&at, k_tree_attention_tc<T, SPLIT, NB, NR>));
     using L = TcTree<SPLIT, NB, NR>;
     if (at.numRegs < L::REGS) return it_fail(IT_ESTATE, "it_tree_attention: built with %d registers a thread", at.numRegs);
-    IT_CUDA(cudaFuncSetAttribute(k_tree_weights_tc<T, SPLIT, NB, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcWeights<SPLIT, NB, NR>::TOTAL));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB> int prepare_dim() {
     if (const int r = prepare_shape<T, SPLIT, NB, 16>()) return r;
     if (const int r = prepare_shape<T, SPLIT, NB, 32>()) return r;
-    return prepare_shape<T, SPLIT, NB, 64>();
+    if (const int r = prepare_shape<T, SPLIT, NB, 64>()) return r;
+    IT_CUDA(cudaFuncSetAttribute(k_tree_weights_tc<T, SPLIT, NB, TW_ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcWeights<SPLIT, NB, TW_ROWS>::TOTAL));
+    return IT_OK;
 }
 template <class T, bool SPLIT> int prepare_type() { const int r = prepare_dim<T, SPLIT, 2>(); return r ? r : prepare_dim<T, SPLIT, 4>(); }
 
@@ -762,17 +763,14 @@ template <class T, bool SPLIT, int NB, int NR> int run_shape(const TaParams& p, 
     IT_CUDA(it_launch_early(k_tree_attention_tc<T, SPLIT, NB, NR>, dim3(p.splits, p.kv_heads, row_tiles), dim3(TcTree<SPLIT, NB, NR>::THREADS), TcTree<SPLIT, NB, NR>::TOTAL, st, p.joined ? p.splits : 1, km, vm, p));
     return IT_OK;
 }
-template <class T, bool SPLIT, int NB, int NR> int weigh_shape(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
+template <class T, bool SPLIT, int NB> int weigh_dim(const TaParams& p, const CUtensorMap& km, cudaStream_t st) {
     // one wave of CTAs, as many tiles for each
     const int tiles = (p.cached + p.rows + TA_KEYS - 1) / TA_KEYS, most = p.kv_heads < TA_MAXSPLITS ? TA_MAXSPLITS / p.kv_heads : 1, rounds = (tiles + most - 1) / most;
-    IT_CUDA(it_launch_early(k_tree_weights_tc<T, SPLIT, NB, NR>, dim3((tiles + rounds - 1) / rounds, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, NR>::TOTAL, st, 1, km, p));
+    IT_CUDA(it_launch_early(k_tree_weights_tc<T, SPLIT, NB, TW_ROWS>, dim3((tiles + rounds - 1) / rounds, p.kv_heads), dim3(TW_THREADS), TcWeights<SPLIT, NB, TW_ROWS>::TOTAL, st, 1, km, p));
     return IT_OK;
 }
 template <class T, bool SPLIT, int NB> int run_dim(const TaParams& p, int nr, int row_tiles, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
     return nr == 16 ? run_shape<T, SPLIT, NB, 16>(p, row_tiles, km, vm, st) : nr == 32 ? run_shape<T, SPLIT, NB, 32>(p, row_tiles, km, vm, st) : run_shape<T, SPLIT, NB, 64>(p, row_tiles, km, vm, st);
-}
-template <class T, bool SPLIT, int NB> int weigh_dim(const TaParams& p, int nr, const CUtensorMap& km, cudaStream_t st) {
-    return nr == 16 ? weigh_shape<T, SPLIT, NB, 16>(p, km, st) : nr == 32 ? weigh_shape<T, SPLIT, NB, 32>(p, km, st) : weigh_shape<T, SPLIT, NB, 64>(p, km, st);
 }
 
 }  // namespace
@@ -787,8 +785,8 @@ int it_tree_tc_run(const TaParams& p, int type, int nb, int nr, int row_tiles, c
     if (type == IT_F16) return nb <= 2 ? run_dim<__half, false, 2>(p, nr, row_tiles, km, vm, st) : run_dim<__half, false, 4>(p, nr, row_tiles, km, vm, st);
     return nb <= 2 ? run_dim<__nv_bfloat16, false, 2>(p, nr, row_tiles, km, vm, st) : run_dim<__nv_bfloat16, false, 4>(p, nr, row_tiles, km, vm, st);
 }
-int it_tree_tc_weigh(const TaParams& p, int type, int nb, int nr, const CUtensorMap& km, cudaStream_t st) {
-    if (type == IT_F32) return nb <= 2 ? weigh_dim<__half, true, 2>(p, nr, km, st) : weigh_dim<__half, true, 4>(p, nr, km, st);
-    if (type == IT_F16) return nb <= 2 ? weigh_dim<__half, false, 2>(p, nr, km, st) : weigh_dim<__half, false, 4>(p, nr, km, st);
-    return nb <= 2 ? weigh_dim<__nv_bfloat16, false, 2>(p, nr, km, st) : weigh_dim<__nv_bfloat16, false, 4>(p, nr, km, st);
+int it_tree_tc_weigh(const TaParams& p, int type, int nb, const CUtensorMap& km, cudaStream_t st) {
+    if (type == IT_F32) return nb <= 2 ? weigh_dim<__half, true, 2>(p, km, st) : weigh_dim<__half, true, 4>(p, km, st);
+    if (type == IT_F16) return nb <= 2 ? weigh_dim<__half, false, 2>(p, km, st) : weigh_dim<__half, false, 4>(p, km, st);
+    return nb <= 2 ? weigh_dim<__nv_bfloat16, false, 2>(p, km, st) : weigh_dim<__nv_bfloat16, false, 4>(p, km, st);
 }

@@ -162,10 +162,11 @@ def test_workspace_goes_by_sizes_alone(lib):
     assert lib.it_tree_attention_workspace(C.byref(tree_args(rows=0)), C.byref(n)) == 0 and n.value == 0
     # runs of a cache are at most one wave of CTAs: never more than this, however long it is
     assert tree_attention_workspace(256, 24, 4, 256, (1 << 30) - 1) < 64 << 20 and tree_attention_workspace(1, 1, 1, 256, (1 << 30) - 1) < 4 << 20
-    # scores for the received weights: 4 bytes a product row and slot, in whole tiles, while the product rows are at most 64 or the head dimension
-    for rows, heads, kv, dim, cached, kept in ((1, 6, 1, 64, 1000, True), (64, 1, 1, 64, 1000, True), (65, 1, 1, 64, 1000, False), (128, 2, 2, 128, 5000, True), (129, 2, 2, 128, 5000, False), (256, 4, 4, 256, 100000, True)):
+    # scores for the received weights: 4 bytes a product row and slot, in whole tiles, up to 256 MB or while the product rows are at most 64 or the head dimension
+    for rows, heads, kv, dim, cached, kept in ((1, 6, 1, 64, 1000, True), (65, 1, 1, 64, 1000, True), (64, 64, 64, 64, 100000, True), (65, 64, 64, 64, 100000, False), (128, 32, 32, 128, 50000, True), (129, 32, 32, 128, 50000, False),
+                                                (65, 64, 64, 64, 16064, False), (65, 64, 64, 64, 16000, True), (256, 4, 4, 256, 100000, True)):
         plain, more = tree_attention_workspace(rows, heads, kv, dim, cached), tree_attention_workspace(rows, heads, kv, dim, cached, weights=True)
-        assert more - plain == (4 * rows * heads * ((cached + rows + 127) // 128 * 128) if kept else 0)
+        assert more - plain == (4 * rows * heads * ((cached + rows + 127) // 128 * 128) if kept else 256 << 20)
         assert tree_attention_workspace(rows, heads, kv, dim, cached // 3, weights=True) <= more
     assert lib.it_cache_evict_workspace(C.byref(evict_args(workspace=None, weights=None)), C.byref(n)) == 0 and n.value >= 800
     assert lib.it_cache_evict_workspace(C.byref(evict_args(keep=0, recent=0)), C.byref(n)) == 0 and n.value == 0

@@ -313,6 +313,25 @@ def test_received_weights_of_few_and_many_rows(ops, rows, heads, kv, dim, cached
     assert torch.equal(more, got)
 
 
+@pytest.mark.parametrize("kind,rows,heads,kv,dim,cached", [("f32", 130, 64, 2, 16, 8200), ("f32", 66, 66, 1, 72, 15600), ("bf16", 256, 40, 2, 136, 6800), ("f16", 256, 32, 4, 64, 8300)])
+def test_received_weights_whose_scores_are_not_kept(ops, kind, rows, heads, kv, dim, cached):
+    """More than 256 MB of scores: K is read again."""
+    assert 4 * rows * heads * cached > 1 << 28 and rows * heads // kv > max(64, dim)
+    q, kc, vc, g = make(kind, rows, cached, heads, kv, dim, rows)
+    parents = random_parents(rows, dim)
+    par = torch.tensor(parents, dtype=torch.int32, device="cuda")
+    was = torch.rand(kv, cached + rows + 5, generator=g, device="cuda")
+    for real in (cached, 700):
+        k2, v2 = kc.clone(), vc.clone()
+        k2[real + rows:], v2[real + rows:] = math.nan, math.inf
+        out, got = torch.empty_like(q), was.clone()
+        ops.tree_attention(q, k2, v2, cached, out, parents=par, length=torch.tensor([real], dtype=torch.int32, device="cuda"), weights=got)
+        want, tol, rec, rtol = tree_64(q, k2, v2, real, parents, None, 0, ACT[kind])
+        near(out, want, tol, "out")
+        near(got[:, :real + rows], was[:, :real + rows].double() + rec, rtol + 2 * H32 * (was[:, :real + rows] + rec), "weights")
+        assert torch.equal(got[:, real + rows:], was[:, real + rows:])
+
+
 def test_parents_that_are_not_smaller_rows_count_as_none(ops):
     q, kc, vc, g = make("f16", 6, 70, 4, 2, 64, 8)
     bad = [3, 1, 0, 2, 1 << 30, -9]           # forward, itself, fine, fine, far away, negative
