@@ -194,7 +194,7 @@ def tree_attention(q, k_cache, v_cache, cached, out, parents=None, gate=None, sc
 
     parents: int32 [row], the row that a row continues or -1 for the cache; None: a chain.  scale 0: head_dim^-1/2.  length: int32 tensor, the number of cached
     slots (at most `cached`), read on the device.  weights: f32 [kv head, slot], to which the softmax weight that every slot received is added.
-    workspace: a uint8 tensor of tree_attention_workspace() bytes; None: one from torch's allocator."""
+    workspace: a uint8 tensor of tree_attention_workspace() bytes (asked with weights=True when weights are given); None: one from torch's allocator."""
     shape = rows, heads, dim = _rows(q, "q")
     act, index = q.dtype, q.get_device()
     (slots, kv, d), ct, kc, vc = _caches(k_cache, v_cache, index)

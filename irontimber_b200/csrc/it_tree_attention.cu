@@ -217,7 +217,7 @@ int ta_prepare(int device) {
 }
 
 // CTAs of `warps` warps that form received weights.  All warps of one share a tile, or, where there are many tiles, as many as have four rows each (one row at 30,000 slots: 33.5 us for the call
-// with a tile a CTA, 29.3).
+// with a tile a CTA and a kernel more, 29.3).
 int ta_weigh_ctas(TaParams& p, int warps) {
     const int tiles = (p.cached + p.rows + TA_KEYS - 1) / TA_KEYS;
     p.tile_warps = warps;
