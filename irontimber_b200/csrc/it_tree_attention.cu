@@ -8,7 +8,7 @@
 // The cache is cut into runs of 128-slot tiles, one per CTA (k_tree_attention_tc, it_tree_attention_tc.cu), so that a single token's few product rows still use every SM, and
 // k_tree_join puts the runs' sums together; a cache of one tile is finished by its CTA.
 // f32 activations: q (scaled per row by a power of two to the top of f16's range) and p are each the sum of two f16 values, 22 bits, and every product is
-// done twice; the f16 cache is exact.  16-bit activations: p is rounded to the cache's type like the output itself, q is exact.
+// done twice; the f16 cache is exact.  16-bit activations: q is exact, p is two values of the cache's type (22 bits, bf16 16), so that a result is rounded once, when it is stored.
 // Masks: only tiles that reach behind the cached slots look at them.  A masked score is replaced, whatever it was; there a non-finite V element is
 // taken out of the product and added to the rows that do see it (0 * inf would be NaN in those that do not).
 // Received weights need the finished references and sums: the one pass leaves its scores, and a small kernel turns them into weights; where the scores would take too much

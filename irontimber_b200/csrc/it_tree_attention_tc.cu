@@ -5,7 +5,7 @@
 // so that a decoded token's six rows cost 32 columns and not 128 rows, and everything comes in the layout that it has:
 //   K and V tiles   128 slots as boxes of 64 elements of a tensor map, 128-byte swizzle: K is read K-major, V (as V^T) MN-major
 //   Q               rows of 128-byte pieces, K-major; f32 activations as two sets of columns, high and low halves, added in f32 when they are read
-//   P               [slot][column], MN-major: a thread has one slot (a lane of tensor memory) and stores its columns as 16-byte pieces
+//   P               [slot][column], MN-major: a thread has one slot (a lane of tensor memory) and stores its columns as 16-byte pieces; high and low halves, two sets of columns
 // Softmax warps (two or four groups of four; a group has its share of the columns): scores out of tensor memory, exponentials against a reference that moves only when
 // it has to (its maximum over a warp's slots by halving what a lane carries, over the four warps by an ordered atomicMax), P; then the tile before: O^T out of tensor memory into f32 accumulators in registers.  Every tile's product starts from zero and is
 // added with a rounded f32 addition: chained over a long run in tensor memory the hardware's truncating accumulation loses f32's last bits (1.3e-5 of the result after 240 tiles of 64
@@ -21,7 +21,11 @@ constexpr int TC_JOIN = IT_TREE_JOIN;                            // runs that jo
 constexpr float TC_SHIFT = 6.f, TC_TOP = 15.f;              // p is 2^6 at the reference and may grow to 2^15 before the reference moves
 
 template <bool SPLIT, int NB, int NR> struct TcTree {
-    static constexpr int NC = NR * (SPLIT ? 2 : 1), NCB = NC > 64 ? 2 : 1;                    // columns of a product, 64-column blocks of P
+    static constexpr int NC = NR * (SPLIT ? 2 : 1);                                           // columns of a tile's scores
+    // Columns of P and of O^T: high and low halves whatever the activations.  p rounded once to the cache's type would cost a result over many slots as much as its own last rounding (bf16, one row at
+    // 131,071 slots: 0.0022 of the result against 0.0016).  With both, us: 32 over 8 heads of 128, bf16, 12 rows at 8190 slots 19.5 for 18.6, f16, 64 rows 42.9 for 41.7; 24 over 4 of 256, bf16, 64 rows at
+    // 30,011 122 for 111; 16 and 32 product rows up to 0.2 more.
+    static constexpr int NP = 2 * NR, NCB = NP > 64 ? 2 : 1;                                  // NCB: 64-column blocks of P
     static constexpr int HD = 64 * NB, MT = NB / 2;                                           // M tiles of O^T
     // Accumulators that a score is spread over (f32 activations, where tensor memory has the columns): the hardware truncates at every step, and a chain of 16 of them
     // cost more than half of the result's error at 16 and 32 rows (1.1e-6 of the result after 512 slots).
@@ -37,8 +41,8 @@ template <bool SPLIT, int NB, int NR> struct TcTree {
     static constexpr int Q = 0, P = QB, KR = P + PB, VR = KR + KS * SLOT, SMALL = VR + VS * SLOT, TOTAL = SMALL + TC_SMALL;
     // offsets from SMALL
     static constexpr int BARS = 0, TMEM = 512, FLAG = 528, MAXES = 576, BASE = 1088, CORR = 1344, FAC = 2112, TROW = 2368;
-    static constexpr int TCOLS = 2 * SC + MT * NC, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
-    static_assert(VS >= 1 && NR % 16 == 0 && NC <= 128 && NR <= 64 && NC % 16 == 0 && RW % 8 == 0, "");
+    static constexpr int TCOLS = 2 * SC + MT * NP, ALLOC = TCOLS <= 64 ? 64 : TCOLS <= 128 ? 128 : TCOLS <= 256 ? 256 : 512;
+    static_assert(VS >= 1 && NR % 16 == 0 && NP <= 128 && TCOLS <= 512 && NR <= 64 && NC % 16 == 0 && RW % 8 == 0, "");
     static_assert((2 * KS * NB + 2 * VS * MT + 5 + MT) * 8 <= TMEM, "");
     static_assert(SOFT_REGS * SOFT + OTHER_REGS * 128 <= REGS * THREADS, "");
     static_assert(PB >= TA_MAXROWS * TA_WORDS * 4 + TA_MAXROWS * 4, "the ancestors are worked out in P's place");
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(TcTree<SPLIT, NB, NR>::THREADS, 1)
 k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TaParams p) {
     using L = TcTree<SPLIT, NB, NR>;
     using TA = typename std::conditional<SPLIT, float, T>::type;
-    constexpr int NC = L::NC, RW = L::RW, HD = L::HD, KS = L::KS, VS = L::VS, WGS = L::WGS, MT = L::MT, W0 = 4 * WGS;       // W0: the first warp behind the softmax warps
+    constexpr int NC = L::NC, NP = L::NP, RW = L::RW, HD = L::HD, KS = L::KS, VS = L::VS, WGS = L::WGS, MT = L::MT, W0 = 4 * WGS;       // W0: the first warp behind the softmax warps
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, g = blockIdx.y, r0 = blockIdx.z * NR;
@@ -304,14 +308,12 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 constexpr int CH = RW < 16 ? RW : 16;
 #pragma unroll
                 for (int k = 0; k < RW; k += CH) {
-                    float u[CH], v[SPLIT ? CH : 1];
-                    tm_ld(u, oaddr + m * NC + k);
-                    if constexpr (SPLIT) tm_ld(v, oaddr + m * NC + NR + k);
+                    float u[CH], v[CH];
+                    tm_ld(u, oaddr + m * NP + k);
+                    tm_ld(v, oaddr + m * NP + NR + k);
                     tm_wait(u);
-                    if constexpr (SPLIT) {
 #pragma unroll
-                        for (int e = 0; e < CH; e++) { asm volatile("" : "+f"(v[e])); u[e] += v[e]; }
-                    }
+                    for (int e = 0; e < CH; e++) { asm volatile("" : "+f"(v[e])); u[e] += v[e]; }
 #pragma unroll
                     for (int e = 0; e < CH; e++) acc[m][k + e] = fmaf(acc[m][k + e], c[k + e], u[e]);
                 }
@@ -320,7 +322,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
         };
 #pragma unroll 1
         for (int i = 0; i <= n; i++) {                              // softmax of tile i, O^T of tile i - 1, P of tile i
-            unsigned hi[RW / 2], lo[SPLIT ? RW / 2 : 1];
+            unsigned hi[RW / 2], lo[RW / 2];
             const bool masked = i >= first_masked;
             if (i < n) {
                 const int buf = i & 1;
@@ -388,7 +390,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     const float a = ex2(y[r]), b = ex2(y[r + 1]);
                     l[r] += a; l[r + 1] += b;
                     hi[r / 2] = Ta16<T>::pack(a, b);
-                    if constexpr (SPLIT) { const float2 h = Ta16<T>::unpack(hi[r / 2]); lo[r / 2] = Ta16<T>::pack(a - h.x, b - h.y); }
+                    const float2 h = Ta16<T>::unpack(hi[r / 2]);
+                    lo[r / 2] = Ta16<T>::pack(a - h.x, b - h.y);
                 }
             }
             if (i > 0) collect(i - 1);                               // frees O^T and P
@@ -398,8 +401,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
             for (int k = 0; k < RW / 8; k++) {
                 const int ch = wg * (RW / 8) + k, cl = ch + NR / 8;       // 16-byte pieces of the high and the low columns
                 *reinterpret_cast<uint4*>(prow + ((ch ^ (key & 7)) << 4)) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-                if constexpr (SPLIT)
-                    *reinterpret_cast<uint4*>(prow + (cl >> 3) * L::BOX + (((cl & 7) ^ (key & 7)) << 4)) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+                *reinterpret_cast<uint4*>(prow + (cl >> 3) * L::BOX + (((cl & 7) ^ (key & 7)) << 4)) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
             }
             if (masked) {
                 // V elements that are not finite leave the product and go to the rows that see their slot
@@ -559,7 +561,7 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll 1
                         for (int k = 0; k < TA_KEYS / 16; k += 4) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++) mma_f16(otm + om * NC, vd + (unsigned)(j * 2048 >> 4), pb + (unsigned)(j * 2048 >> 4), idesc<T>(NC, true), k + j > 0);          // 16 slots a step
+                            for (int j = 0; j < 4; j++) mma_f16(otm + om * NP, vd + (unsigned)(j * 2048 >> 4), pb + (unsigned)(j * 2048 >> 4), idesc<T>(NP, true), k + j > 0);          // 16 slots a step
                             vd += (unsigned)(4 * 2048 >> 4); pb += (unsigned)(4 * 2048 >> 4);
                         }
                         commit_to(ofull + 8 * om); commit_to(vempty + 8 * va);
