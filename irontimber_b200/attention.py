@@ -246,10 +246,13 @@ def _weights(w, kv, n, index):
 def _workspace(nbytes, index, stream):
     if index < 0:
         raise ValueError("tensors are not on a CUDA device")
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=index)
-    if stream is not None:                   # torch hands the memory out again in the order of the current stream
-        workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream, device=index))
-    return workspace
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=index)
+    # Torch hands memory out, and takes it back, in the order of the stream that is current: a block that was just freed on another one may still be written by what is queued there.
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=index) if stream else torch.cuda.default_stream(index)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=index)
 
 
 def _check_workspace(w, index):

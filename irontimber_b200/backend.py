@@ -291,7 +291,8 @@ class CudaBackend:
         import torch
         if not self._workspaces or self._workspaces[-1].numel() < nbytes:
             had = self._workspaces[-1].numel() if self._workspaces else 0
-            self._workspaces.append(torch.empty(max(nbytes, min(2 * had, 1 << 26), 256), dtype=torch.uint8, device=f"cuda:{self.device}"))
+            with torch.cuda.stream(self.torch_stream):       # in the order of the stream that uses it, whatever the current one is
+                self._workspaces.append(torch.empty(max(nbytes, min(2 * had, 1 << 26), 256), dtype=torch.uint8, device=f"cuda:{self.device}"))
         return self._workspaces[-1]
 
     def read_u32(self, off):

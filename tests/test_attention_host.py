@@ -1,0 +1,51 @@
+"""What attention.py and CudaBackend do on the host around a launch, without a GPU: whose memory a workspace is, how much is kept, and what is refused."""
+import contextlib
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Streams:
+    """Torch's streams and allocator as far as a workspace needs them: blocks belong to the stream that is current when they are asked for."""
+
+    def __init__(self, monkeypatch):
+        self.now, self.blocks = "current", []
+        monkeypatch.setattr(torch.cuda, "stream", self.stream)
+        monkeypatch.setattr(torch.cuda, "ExternalStream", lambda ptr, device=None: f"stream {ptr} of {device}")
+        monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: f"default of {device}")
+        monkeypatch.setattr(torch, "empty", self.empty)
+
+    @contextlib.contextmanager
+    def stream(self, s):
+        was, self.now = self.now, s
+        yield
+        self.now = was
+
+    def empty(self, n, dtype=None, device=None):
+        assert dtype is torch.uint8
+        block = types.SimpleNamespace(owner=self.now, numel=lambda: n, device=device, record_stream=lambda s: None)
+        self.blocks.append(block)
+        return block
+
+
+@pytest.mark.parametrize("stream,owner", [(None, "current"), ("another", "another"), (77, "stream 77 of 3"), (0, "default of 3")])
+def test_a_workspace_comes_from_the_pool_of_the_stream_that_uses_it(monkeypatch, stream, owner):
+    """Memory of another stream's pool may be a block that was just freed there and that queued kernels still write."""
+    from irontimber_b200 import attention
+    s = Streams(monkeypatch)
+    assert attention._workspace(1000, 3, stream).owner == owner and s.now == "current"
+
+
+def backend():
+    """A CudaBackend without a device."""
+    from irontimber_b200.backend import CudaBackend
+    be = CudaBackend.__new__(CudaBackend)
+    be.device, be.ctx, be._torch_stream, be._workspaces, be.arena_floats = 0, None, "the backend's", [], 1 << 20
+    return be
+
+
+def test_a_backends_workspace_comes_from_its_streams_pool(monkeypatch):
+    s = Streams(monkeypatch)
+    assert backend()._workspace(1000).owner == "the backend's" and s.now == "current"

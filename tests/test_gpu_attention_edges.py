@@ -25,3 +25,28 @@ def test_results_of_16_bit_activations_are_rounded_once(ops, kind, rows, cached,
     once = float((want.to(q.dtype).double() - want).norm())
     left = 1e-5 + half_step(q.dtype) ** 2 + (math.sqrt(cached + rows) * 2.0 ** -31 if kind == "f16" else 0)
     assert float((out.double() - want).norm()) <= once + 2 * left * float(want.norm())
+
+
+def test_workspaces_of_other_streams_are_not_used(ops):
+    """Calls that allocate, on the current stream and on others in turn, behind work that keeps the current stream busy while its blocks are freed."""
+    q, kc, vc, g = make("f32", 12, 3000, 24, 4, 256, 20)
+    par = torch.tensor(random_parents(12, 5), dtype=torch.int32, device="cuda")
+    want, w0 = torch.empty_like(q), torch.zeros(4, 3100, device="cuda")
+    ops.tree_attention(q, kc, vc, 3000, want, parents=par, weights=w0)
+    other = torch.cuda.Stream()
+    a, b = torch.randn(4096, 4096, device="cuda"), torch.empty(4096, 4096, device="cuda")
+    nbytes = ops.tree_attention_workspace(12, 24, 4, 256, 4095, weights=True)
+    outs, ws = [torch.empty_like(q) for _ in range(24)], [torch.zeros(4, 3100, device="cuda") for _ in range(24)]
+    torch.cuda.synchronize()
+    for i, (o, w) in enumerate(zip(outs, ws)):
+        for _ in range(3):
+            torch.mm(a, a, out=b)
+        torch.empty(nbytes, dtype=torch.uint8, device="cuda").fill_(255)                # freed with its write still queued
+        for s in (other, other.cuda_stream) if i % 2 else (None,):
+            ops.tree_attention(q, kc, vc, 3000, o, parents=par, weights=w, stream=s)
+        if i % 2:
+            with torch.cuda.stream(other):
+                w.mul_(0.5)                                                            # two equal calls have added to it
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    assert all(torch.equal(w, w0) for w in ws)
