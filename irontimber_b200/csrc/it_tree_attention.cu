@@ -66,8 +66,10 @@ template <int WARPS, bool JOIN> __device__ __forceinline__ void ta_weigh(const T
     }
     float a[4] = { 0.f, 0.f, 0.f, 0.f };
     auto add = [&](const float4& v, float2 st) {
-        const float inv = st.y == 0.f ? 0.f : 1.f / st.y;
-        a[0] = fmaf(ex2(v.x - st.x), inv, a[0]); a[1] = fmaf(ex2(v.y - st.x), inv, a[1]); a[2] = fmaf(ex2(v.z - st.x), inv, a[2]); a[3] = fmaf(ex2(v.w - st.x), inv, a[3]);
+        const float inv = st.y == 0.f ? 0.f : 1.f / st.y, s[4] = { v.x, v.y, v.z, v.w };
+        // a masked slot's score is -inf: it gets nothing, be the row's sum NaN (0 * NaN)
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[i] = s[i] == -INFINITY ? a[i] : fmaf(ex2(s[i] - st.x), inv, a[i]);
     };
 #pragma unroll
     for (int k = 0; k < AHEAD; k++) if (first + k * groups < rows) add(x[k], JOIN ? stat[first + k * groups] : e[k]);

@@ -50,3 +50,26 @@ def test_workspaces_of_other_streams_are_not_used(ops):
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
     assert all(torch.equal(w, w0) for w in ws)
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim,cached,real", [
+    (4, 2, 2, 64, 100, 100), (20, 6, 2, 128, 100, 100), (64, 8, 2, 256, 2000, 2000), (7, 1, 1, 64, 30000, 30000), (12, 24, 4, 256, 2091, 1900), (130, 64, 2, 16, 8200, 8200), (130, 64, 2, 16, 8200, 700)])
+def test_a_row_that_is_not_a_number_weighs_only_what_it_sees(ops, rows, heads, kv, dim, cached, real):
+    """A NaN or infinite key of a tree row makes that row's weights NaN, for the slots that it sees.  Those of its siblings, which nobody but they see, are what they were: with the weights formed
+    by their own launch, beside the joining, and in a second walk over the keys."""
+    q, kc, vc, g = make("f32", rows, cached, heads, kv, dim, rows + real)
+    parents = [-1] * rows
+    par = torch.tensor(parents, dtype=torch.int32, device="cuda")
+    length = None if real == cached else torch.tensor([real], dtype=torch.int32, device="cuda")
+    out, clean = torch.empty_like(q), torch.zeros(kv, cached + rows, device="cuda")
+    ops.tree_attention(q, kc, vc, cached, out, parents=par, weights=clean, length=length)
+    others = [real + t for t in range(rows) if t != 1]
+    for bad in (math.nan, math.inf):
+        k2 = kc.clone()
+        k2[real + 1] = bad
+        got = torch.zeros_like(clean)
+        ops.tree_attention(q, k2, vc, cached, out, parents=par, weights=got, length=length)
+        assert torch.equal(got[:, others], clean[:, others])
+        if math.isnan(bad):
+            assert got[:, real + 1].isnan().all() and got[:, :real].isnan().all()
+        assert not got[:, real + rows:].any()
