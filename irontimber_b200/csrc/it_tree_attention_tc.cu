@@ -713,14 +713,17 @@ k_tree_weights_tc(const __grid_constant__ CUtensorMap kmap, const __grid_constan
             const float* const rw = row + q % 3 * 4 * NR + wg * RW;
             if (!masked) {
 #pragma unroll
-                for (int r = 0; r < RW; r++) sum = fmaf(ex2(fmaf(x[r], rw[r], -rw[NR + r])), rw[2 * NR + r], sum);
+                for (int r = 0; r < RW; r++) {                        // rows behind the last are zeros: 0 * inf of a key is NaN, and does not count
+                    const float inv = rw[2 * NR + r];
+                    sum = inv == 0.f ? sum : fmaf(ex2(fmaf(x[r], rw[r], -rw[NR + r])), inv, sum);
+                }
             } else {
-                // a masked score does not count, whatever it is; the sum of a row behind the last is 0 and its statistics are 0
+                // a masked score does not count, whatever it is, nor does a row behind the last
                 const int t0 = tile * TA_KEYS + key;
 #pragma unroll
                 for (int r = 0; r < RW; r++) {
-                    const float e = ex2(fmaf(x[r], rw[r], -rw[NR + r])) * rw[2 * NR + r];
-                    if (ta_sees(p, anc, reinterpret_cast<const int*>(rw)[3 * NR + r], t0, cached)) sum += e;
+                    const float inv = rw[2 * NR + r], e = ex2(fmaf(x[r], rw[r], -rw[NR + r])) * inv;
+                    if (inv != 0.f && ta_sees(p, anc, reinterpret_cast<const int*>(rw)[3 * NR + r], t0, cached)) sum += e;
                 }
             }
         }

@@ -73,3 +73,19 @@ def test_a_row_that_is_not_a_number_weighs_only_what_it_sees(ops, rows, heads, k
         if math.isnan(bad):
             assert got[:, real + 1].isnan().all() and got[:, :real].isnan().all()
         assert not got[:, real + rows:].any()
+
+
+@pytest.mark.parametrize("cached,rows", [(6900, 255), (2000, 9)])
+def test_a_key_of_minus_infinity_gets_no_weight(ops, cached, rows):
+    """Every row scores it -inf, in a whole tile and in one that reaches behind the cached slots; the product tile's rows behind the last are zeros, and 0 * inf is not a number."""
+    heads, kv, dim = 40, 2, 136
+    assert rows * heads // kv % 64 and (4 * rows * heads * cached > 1 << 28) == (rows == 255)
+    q, kc, vc, g = make("bf16", rows, cached, heads, kv, dim, rows)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    par = torch.tensor(random_parents(rows, dim), dtype=torch.int32, device="cuda")
+    out, got = torch.empty_like(q), torch.zeros(kv, cached + rows, device="cuda")
+    for at in (5, cached - 1):
+        kc[at, :, 0] = -math.inf
+    ops.tree_attention(q, kc, vc, cached, out, parents=par, weights=got)
+    assert torch.isfinite(out).all() and torch.isfinite(got).all()
+    assert not got[:, 5].any() and not got[:, cached - 1].any() and (got[:, 6:cached - 1] > 0).any(1).all()
