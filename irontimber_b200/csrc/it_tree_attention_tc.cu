@@ -404,7 +404,14 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 *reinterpret_cast<uint4*>(prow + (cl >> 3) * L::BOX + (((cl & 7) ^ (key & 7)) << 4)) = make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
             }
             if (masked) {
-                // V elements that are not finite leave the product and go to the rows that see their slot
+                // V elements that are not finite leave the product and go to the rows that see their slot; in front of this tile's correction, which therefore must not be 0 (0 * inf)
+                float* const c = corr_s + (i & 1) * NR + wg * RW;
+#pragma unroll
+                for (int r = 0; r < RW; r++)
+                    if (c[r] == 0.f) {
+#pragma unroll
+                        for (int m = 0; m < MT; m++) acc[m][r] = 0.f;
+                    }
                 const int j0 = (tile0 + i) * TA_KEYS, from = max(cached - j0, 0), to = min(TA_KEYS, p.cached + p.rows - j0);
                 bool any[MT];
 #pragma unroll
@@ -426,7 +433,8 @@ k_tree_attention_tc(const __grid_constant__ CUtensorMap kmap, const __grid_const
                         for (int r = 0; r < RW; r++) if ((rows >> r) & 1u) acc[m][r] += bad;
                     }
                 }
-                groups_sync<WGS>();                         // all groups have looked at the elements that one of them clears
+                groups_sync<WGS>();                         // all groups have looked at the elements that one of them clears, and at the corrections
+                if (lane < RW && c[lane] == 0.f) c[lane] = 1.f;          // (the four warps write the same)
 #pragma unroll
                 for (int m = 0; m < MT; m++)
                     if (any[m] && wg == 0) {

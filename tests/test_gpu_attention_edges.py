@@ -89,3 +89,30 @@ def test_a_key_of_minus_infinity_gets_no_weight(ops, cached, rows):
     ops.tree_attention(q, kc, vc, cached, out, parents=par, weights=got)
     assert torch.isfinite(out).all() and torch.isfinite(got).all()
     assert not got[:, 5].any() and not got[:, cached - 1].any() and (got[:, 6:cached - 1] > 0).any(1).all()
+
+
+@pytest.mark.parametrize("rows,cached,heads,kv,dim,kind", [
+    (5, 100, 6, 2, 128, "f32"), (5, 100, 6, 2, 128, "f16"), (1, 0, 2, 1, 64, "bf16"), (9, 128, 4, 2, 256, "f32"), (40, 120, 2, 1, 256, "bf16"), (64, 0, 8, 2, 128, "f32"), (64, 1000, 4, 1, 256, "f16"), (200, 300, 2, 2, 64, "f32"),
+    (3, 128 * 300 - 1, 4, 4, 64, "f32")])
+def test_an_infinite_value_of_a_row_reaches_those_that_see_it_as_it_is(ops, rows, cached, heads, kv, dim, kind):
+    """In the first tile that a run has and in later ones, and for rows that have seen nothing before; the sign is the value's.  Elements beside it are what they were."""
+    q, kc, vc, g = make(kind, rows, cached, heads, kv, dim, rows + cached)
+    parents = random_parents(rows, 3)
+    par = torch.tensor(parents, dtype=torch.int32, device="cuda")
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    ops.tree_attention(q, kc, vc, cached, clean, parents=par)
+    for at in {0, rows // 2, rows - 1}:
+        sees = []
+        for t in range(rows):
+            j = t
+            while j > at:
+                j = parents[j]
+            sees.append(j == at)
+        for bad in (math.inf, -math.inf):
+            v2 = vc.clone()
+            v2[cached + at, :, 3] = bad
+            ops.tree_attention(q, kc, v2, cached, out, parents=par)
+            seen = torch.tensor(sees, device="cuda")
+            assert (out[seen][..., 3] == bad).all()
+            assert torch.equal(out[~seen], clean[~seen])
+            assert torch.equal(out[..., :3], clean[..., :3]) and torch.equal(out[..., 4:], clean[..., 4:])
