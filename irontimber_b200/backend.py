@@ -288,11 +288,12 @@ class CudaBackend:
         attention.cache_evict(k_cache, v_cache, weights, n, keep, recent, kept, stream=self.torch_stream, **options)
 
     def _workspace(self, nbytes):
+        """At least nbytes.  One that has to grow at least doubles, so that all that are kept for recorded graphs have at most four times the bytes of the largest request."""
         import torch
         if not self._workspaces or self._workspaces[-1].numel() < nbytes:
             had = self._workspaces[-1].numel() if self._workspaces else 0
             with torch.cuda.stream(self.torch_stream):       # in the order of the stream that uses it, whatever the current one is
-                self._workspaces.append(torch.empty(max(nbytes, min(2 * had, 1 << 26), 256), dtype=torch.uint8, device=f"cuda:{self.device}"))
+                self._workspaces.append(torch.empty(max(nbytes, 2 * had, 256), dtype=torch.uint8, device=f"cuda:{self.device}"))
         return self._workspaces[-1]
 
     def read_u32(self, off):

@@ -49,3 +49,15 @@ def backend():
 def test_a_backends_workspace_comes_from_its_streams_pool(monkeypatch):
     s = Streams(monkeypatch)
     assert backend()._workspace(1000).owner == "the backend's" and s.now == "current"
+
+
+def test_what_a_backend_keeps_is_bounded_by_the_largest_request(monkeypatch):
+    """A cache that grows by views, or calls of more and more rows, ask for a little more each time; earlier workspaces stay, since recorded graphs may know them."""
+    from irontimber_b200 import attention
+    for requests in ([attention.tree_attention_workspace(64, 24, 4, 256, n, weights=True) for n in range(1000, 131072, 128)],
+                     [attention.tree_attention_workspace(r, 24, 4, 256, 131072, weights=True) for r in range(1, 257)], range(1, 200000, 999), [10, 10, 5, 10]):
+        s, be = Streams(monkeypatch), backend()
+        for n in requests:
+            assert be._workspace(n).numel() >= n
+        assert sum(w.numel() for w in be._workspaces) <= 4 * max(max(requests), 256)
+        assert len(be._workspaces) <= 30 and len(s.blocks) == len(be._workspaces)
