@@ -112,6 +112,7 @@ SIGNATURES = {
 }
 
 _lib = None
+RECORDING = set()          # streams that a CudaBackend is recording: memory that a call allocates for itself there would be handed on while the graph still uses it
 
 
 class IronTimberError(RuntimeError):

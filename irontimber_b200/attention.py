@@ -5,6 +5,9 @@ Tensors are torch CUDA tensors of one device; work is launched on `stream` (torc
 Activations are f32 over an f16 cache, or f16 / bf16 for both.  Heads are contiguous, everything else may have strides: a cache tensor is
 [slot, kv head, element] whatever its memory order (`cache.transpose(0, 1)` of a [kv head, slot, element] one).  `CudaBackend` has the same calls on its own
 stream.  All arithmetic runs in libirontimber_cuda.so; this file only marshals arguments.
+
+In a graph: torch.cuda.graph gives a call that allocates its workspace memory of the graph's own; any other way of recording needs workspace=, memory that lives as long as the graph and that nothing
+uses while it runs.
 """
 import ctypes as C
 import functools
@@ -246,6 +249,8 @@ def _weights(w, kv, n, index):
 def _workspace(nbytes, index, stream):
     if index < 0:
         raise ValueError("tensors are not on a CUDA device")
+    if _lib.RECORDING and (stream if isinstance(stream, int) else stream.cuda_stream if stream is not None else torch.cuda.current_stream(index).cuda_stream) in _lib.RECORDING:
+        raise ValueError("a call that a CudaBackend records needs workspace=: one from torch's allocator would be handed on while the graph still uses it")
     if stream is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=index)
     # Torch hands memory out, and takes it back, in the order of the stream that is current: a block that was just freed on another one may still be written by what is queued there.

@@ -101,6 +101,11 @@ class CudaBackend:
 
     def close(self):
         if self.ctx:
+            if _lib.RECORDING and self.stream in _lib.RECORDING:          # one that was given up
+                try:
+                    self.graph_destroy(self.capture_end())
+                except _lib.IronTimberError:
+                    pass
             if self._workspaces:               # torch's allocator hands them on without waiting for this stream
                 self.sync()
                 self._workspaces = []
@@ -135,8 +140,10 @@ class CudaBackend:
     # ---- graphs (one recorded command sequence, replayed with one launch) -------------------------
     def capture_begin(self):
         _lib.check(self.L.it_capture_begin(self.ctx))
+        _lib.RECORDING.add(self.stream)
 
     def capture_end(self):
+        _lib.RECORDING.discard(self.stream)
         h = C.c_void_p()
         _lib.check(self.L.it_capture_end(self.ctx, C.byref(h)))
         return h
@@ -274,7 +281,8 @@ class CudaBackend:
 
     def tree_attention(self, q, k_cache, v_cache, cached, out, **options):
         """attention.tree_attention on this backend's stream (attention dispatch, src/vk/mod.rs:833-840).  The workspace is the backend's own: one stream
-        orders its uses, those of recorded graphs too, and a larger one does not replace one that a recorded graph knows."""
+        orders its uses, those of graphs that the backend records and launches too, and a larger one does not replace one that a recorded graph knows.  A call is recorded after one that
+        needs as much (the same sizes, weights or not) has been made, so that nothing is allocated meanwhile; a graph that is launched on another stream than the backend's gets workspace=."""
         from . import attention
         if options.get("workspace") is None:
             options["workspace"] = self._workspace(attention.tree_attention_workspace(q.shape[0], q.shape[1], k_cache.shape[1], q.shape[2], min(k_cache.shape[0], (1 << 30) - 1), q.dtype, options.get("weights") is not None))
@@ -292,6 +300,8 @@ class CudaBackend:
         import torch
         if not self._workspaces or self._workspaces[-1].numel() < nbytes:
             had = self._workspaces[-1].numel() if self._workspaces else 0
+            if _lib.RECORDING and self.stream in _lib.RECORDING:
+                raise ValueError(f"a recorded call needs a workspace of {nbytes} bytes, and earlier calls {had}: make the call once before it is recorded, or give workspace=")
             with torch.cuda.stream(self.torch_stream):       # in the order of the stream that uses it, whatever the current one is
                 self._workspaces.append(torch.empty(max(nbytes, 2 * had, 256), dtype=torch.uint8, device=f"cuda:{self.device}"))
         return self._workspaces[-1]

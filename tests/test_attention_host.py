@@ -61,3 +61,38 @@ def test_what_a_backend_keeps_is_bounded_by_the_largest_request(monkeypatch):
             assert be._workspace(n).numel() >= n
         assert sum(w.numel() for w in be._workspaces) <= 4 * max(max(requests), 256)
         assert len(be._workspaces) <= 30 and len(s.blocks) == len(be._workspaces)
+
+
+class Recorder:
+    """The library's recording calls."""
+
+    @staticmethod
+    def it_capture_begin(ctx):
+        return 0
+
+    it_capture_end = staticmethod(lambda ctx, out: 0)
+    it_ctx_stream = staticmethod(lambda ctx: 4711)
+    it_ctx_destroy = it_sync = it_graph_destroy = staticmethod(lambda ctx: 0)
+
+
+def test_a_recorded_call_does_not_allocate(monkeypatch):
+    """The backend's own workspace has to be there; one from torch's allocator would be freed, and handed on, with the graph still writing to it."""
+    from irontimber_b200 import _lib, attention
+    s, be = Streams(monkeypatch), backend()
+    be.L, be.ctx = Recorder, 1
+    be._workspace(5000)
+    mine = types.SimpleNamespace(cuda_stream=4711)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index: mine)
+    be.capture_begin()
+    assert be._workspace(5000) is s.blocks[0] and be._workspace(10) is s.blocks[0]
+    with pytest.raises(ValueError, match="before it is recorded"):
+        be._workspace(5001)
+    for stream in (mine, 4711, None):
+        with pytest.raises(ValueError, match="needs workspace="):
+            attention._workspace(100, 0, stream)
+    attention._workspace(100, 0, 4712)
+    be.capture_end()
+    assert be._workspace(5001) is s.blocks[-1] and attention._workspace(100, 0, 4711) is s.blocks[-1]
+    be.capture_begin()
+    be.close()
+    assert not _lib.RECORDING

@@ -116,3 +116,45 @@ def test_an_infinite_value_of_a_row_reaches_those_that_see_it_as_it_is(ops, rows
             assert (out[seen][..., 3] == bad).all()
             assert torch.equal(out[~seen], clean[~seen])
             assert torch.equal(out[..., :3], clean[..., :3]) and torch.equal(out[..., 4:], clean[..., 4:])
+
+
+def test_a_backend_records_with_its_own_workspace_only(ops):
+    """Refused while recording: a call that would need a larger workspace, and one that would take it from torch's allocator.  The recording goes on, and what it holds is launched beside larger calls."""
+    from irontimber_b200.backend import CudaBackend
+    be = CudaBackend(0, arena_floats=1 << 12)
+    try:
+        with torch.cuda.stream(be.torch_stream):
+            q, kc, vc, g = make("f32", 3, 5000, 8, 2, 128, 21)
+            big = torch.randn(200, 8, 128, device="cuda")
+            want, out, more = torch.empty_like(q), torch.zeros_like(q), torch.empty_like(big)
+            w = torch.zeros(2, 5003, device="cuda")
+            be.tree_attention(q, kc, vc, 5000, want)
+            be.capture_begin()
+            be.tree_attention(q, kc, vc, 5000, out)
+            with pytest.raises(ValueError, match="before it is recorded"):
+                be.tree_attention(big, kc, vc, 4800, more)
+            with pytest.raises(ValueError, match="needs workspace="):
+                ops.tree_attention(q, kc, vc, 5000, want)
+            gr = be.capture_end()
+            be.tree_attention(big, kc, vc, 4800, more)
+            be.tree_attention(q, kc, vc, 5000, want.clone(), weights=w)
+            be.graph_launch(gr)
+            be.tree_attention(big, kc, vc, 4800, more)
+            be.sync()
+            assert torch.equal(out, want) and be.L.it_graph_kernel_nodes(gr) == 2
+            be.graph_destroy(gr)
+    finally:
+        be.close()
+
+
+def test_a_backend_is_closed_in_a_recording(ops):
+    """As a `finally` does after a refusal: the recording is given up, nothing is raised, and the next backend works."""
+    from irontimber_b200.backend import CudaBackend
+    for _ in range(2):
+        be = CudaBackend(0, arena_floats=1 << 12)
+        q, kc, vc, g = make("f32", 3, 500, 8, 2, 128, 22)
+        torch.cuda.synchronize()
+        be.tree_attention(q, kc, vc, 500, torch.empty_like(q))
+        be.capture_begin()
+        be.tree_attention(q, kc, vc, 500, torch.empty_like(q))
+        be.close()
