@@ -338,7 +338,9 @@ int it_argmax_static(void* stream, const float* logits_dev, size_t n, uint32_t* 
  * aligned to 4 elements, cache pointers to 16 bytes and cache strides to 8 elements, norm weights to 16 bytes.  At most 1024 query heads share a kv head.  A cache is [slot][kv head][head_dim] or [kv head][slot][head_dim] or
  * any other pair of strides; k and v may lie in one buffer.  All may be recorded in a CUDA graph once one call of that entry point on that device
  * has been made outside of recording.  A call of no rows (keep 0) looks at no pointer and does nothing.  Sums, norms, softmax statistics and accumulators are f32 (angles: 64-bit fractions of a turn); in
- * the products q (f32) and the softmax's values are two 16-bit halves each (22 bits; bf16: 16), added in f32, and a result is rounded to its type once. */
+ * the products q (f32) and the softmax's values are two 16-bit halves each (22 bits; bf16: 16), added in f32, and a result is rounded to its type once.  A wait inside a kernel that
+ * ran out (none should; about a second) is reported once, as IT_ETIMEOUT, by the next call of the three on the device: that attention's outputs are NaN; an eviction's K and V are moved in
+ * part, with nothing in them that says so, and have to be filled again. */
 enum { IT_F32 = 0, IT_F16 = 1, IT_BF16 = 2 };
 enum { IT_ROPE_HALF = 0, IT_ROPE_INTERLEAVED = 1 };                                     /* pair i: elements (i, i + n_rot/2), or (2i, 2i + 1) */
 enum { IT_ROPE_SCALE_NONE = 0, IT_ROPE_SCALE_LINEAR = 1, IT_ROPE_SCALE_NTK = 2, IT_ROPE_SCALE_YARN = 3 };

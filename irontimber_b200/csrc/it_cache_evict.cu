@@ -12,6 +12,7 @@
 // and never before their place, so those are rows of at most two earlier blocks (the select kernel notes how many kept slots lie before every 64th).  A block reads its
 // rows into shared memory, says so, waits for those two, and writes.  Blocks are numbered as they start, so whom a block waits for has started before it.
 #include "it_ops.cuh"
+#include "it_ops_sites.h"
 #include "it_pipe.cuh"
 #include <cooperative_groups.h>
 #include <mutex>
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) k_evict_move(const __grid_con
             while (true) {
                 asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(flags + q) : "memory");
                 if (seen) break;
-                if (clock64() - t0 > WAIT_CLOCKS) { atomicExch(p.status, 71); ok = 0; break; }
+                if (clock64() - t0 > WAIT_CLOCKS) { atomicExch(p.status, IT_SITE_EVICT_MOVE); ok = 0; break; }
             }
             if (!ok) break;
         }

@@ -1,5 +1,6 @@
 // Device facts of the operators that take a stream instead of a context.
 #include "it_ops.cuh"
+#include "it_ops_sites.h"
 #include <mutex>
 
 int it_ops_current(void* stream, const char* who, it_ops_device* out) {
@@ -28,6 +29,6 @@ int it_ops_current(void* stream, const char* who, it_ops_device* out) {
     *out = known[dev];
     // A wait that ran out in an earlier call: said once, by the next call.
     volatile int* status = out->status_host;
-    if (*status) { const int site = *status; *status = 0; return it_fail(IT_ETIMEOUT, "%s: a wait of an earlier call on this device ran out (site %d); its outputs are NaN", who, site); }
+    if (*status) { const int site = *status; *status = 0; return it_fail(IT_ETIMEOUT, "%s: a wait of an earlier call on this device ran out (site %d); %s", who, site, it_ops_after_timeout(site)); }
     return IT_OK;
 }

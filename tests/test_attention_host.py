@@ -96,3 +96,21 @@ def test_a_recorded_call_does_not_allocate(monkeypatch):
     be.capture_begin()
     be.close()
     assert not _lib.RECORDING
+
+
+def test_what_a_wait_that_ran_out_leaves_behind(tmp_path):
+    """An attention's outputs are NaN.  An eviction's caches are not: the next call's message must not say so, nor that they are as they were."""
+    import ctypes
+    import os
+    import re
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "irontimber_b200", "csrc")
+    sites = [int(n) for n in re.findall(r"atomicExch\(p?\.?\w*status, (\d+)\)|abort_flag, p\.status, (\d+)\)", open(os.path.join(csrc, "it_tree_attention_tc.cu")).read()) for n in n if n]
+    src = open(os.path.join(csrc, "it_cache_evict.cu")).read()
+    assert "atomicExch(p.status, IT_SITE_EVICT_MOVE)" in src and src.count("p.status,") == 1 and len(sites) >= 8
+    (tmp_path / "t.cpp").write_text('#include "it_ops_sites.h"\nextern "C" const char* text(int site) { return it_ops_after_timeout(site); }\nextern "C" int evict() { return IT_SITE_EVICT_MOVE; }\n')
+    subprocess.run(["g++", "-Wall", "-Werror", "-shared", "-fPIC", "-I", csrc, str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t.so")], check=True)
+    lib = ctypes.CDLL(str(tmp_path / "t.so"))
+    lib.text.restype = ctypes.c_char_p
+    assert all(s != lib.evict() and b"NaN" in lib.text(s) for s in sites)
+    assert b"NaN" not in lib.text(lib.evict()) and b"moved in part" in lib.text(lib.evict())
