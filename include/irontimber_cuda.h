@@ -362,7 +362,7 @@ int it_rope_read(const it_rope* r, double* freq, double* mscale);   /* n_rot / 2
  * norm(x) = x / sqrt(mean(x^2) + eps) * weight, per head, skipped where the weight pointer is NULL; rope NULL: no rotation.  The position of row t
  * is positions[t] (device), or pos0 + t (+ *base) when positions is NULL.  base (device, may be NULL): one i32 added to slots and default
  * positions, so that a recorded graph can be replayed at other lengths; rows whose slot then falls outside [0, slots) are not stored.
- * q may be NULL (k and v only) and k, v may be NULL together (q only).  q_out is q itself (same strides) or does not overlap q, k or v.
+ * q may be NULL (k and v only) and k, v may be NULL together (q only).  q_out is q itself (same strides) or does not overlap q, k or v; it does not overlap the caches.
  * A head's positions beyond 2^31 do not exist; negative positions rotate backwards. */
 typedef struct it_norm_rope_args {
     int32_t type, cache_type, rows, heads, kv_heads, head_dim;
@@ -387,7 +387,8 @@ int it_norm_rope(void* stream, const it_norm_rope_args* a);
  * (NaN, infinities, slots behind the last) does not reach the result.  `length` (device i32, may be NULL): the number of cached slots, clamped to
  * [0, cached], for recorded graphs.  weights (f32, [kv head][slot], slots contiguous, may be NULL): weights[g][slot] += the softmax weight
  * that the slot received from all rows and all query heads of kv head g; slots that no row sees are left alone.
- * slots: how many the cache has, >= cached + rows.  out may be q or gate itself (same strides).
+ * slots: how many the cache has, >= cached + rows.  out may be gate itself, and without weights q itself (same strides; forming the weights may read q once more); otherwise out, weights and the
+ * workspace overlap neither one another nor anything that the call reads.
  * workspace: 256-byte aligned device memory of it_tree_attention_workspace() bytes (0: may be NULL), free for other use once the call's work is done;
  * calls that may overlap need one each.  Results do not depend on it, on the stream, or on chance: the same inputs give the same bits. */
 typedef struct it_tree_attention_args {
@@ -411,7 +412,7 @@ int it_tree_attention_workspace(const it_tree_attention_args* a, size_t* nbytes)
 /* Cuts a cache of n slots down to `keep` per kv head: the last `recent` slots stay, and of the others the keep - recent with the largest weight
  * (equal weights: the lower slot; NaN ranks below everything; -0 equals 0).  What stays moves to slots 0..keep-1 in its old order, in place, in k_cache, v_cache
  * and weights (each may be NULL except weights); kept[g][i] (i32, kept_head apart, may be NULL) is the slot that slot i of head g held before.  Slots from keep on are left
- * as they were.  0 <= recent <= keep <= n <= slots, n <= 524,288.  Works on 16-bit caches of any head_dim that is a multiple of 8 up to 256.
+ * as they were.  Weights, kept and the workspace overlap neither one another nor a cache.  0 <= recent <= keep <= n <= slots, n <= 524,288.  Works on 16-bit caches of any head_dim that is a multiple of 8 up to 256.
  * workspace as above, it_cache_evict_workspace() bytes. */
 typedef struct it_cache_evict_args {
     int32_t kv_heads, head_dim;

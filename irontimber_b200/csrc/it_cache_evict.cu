@@ -343,6 +343,11 @@ IT_API int it_cache_evict(void* stream, const it_cache_evict_args* a) {
     IT_CHECK_ARG(!a->kept || (it_aligned(a->kept, 4) && (G == 1 || a->kept_head >= a->keep)), "%s: kept: a head's slots do not overlap the next one's", who);
     const EvPlan pl = ev_plan(a);
     IT_CHECK_ARG(a->workspace && it_aligned(a->workspace, 256) && a->workspace_bytes >= pl.total, "%s: a workspace of %zu bytes, 256-byte aligned, is needed", who, pl.total);
+    const it_stretch all[] = { { "the workspace", a->workspace, pl.total }, { "weights", a->weights, ((size_t)(G - 1) * (size_t)a->w_head + (size_t)a->n) * 4 },
+                               { "kept", a->kept, ((size_t)(G - 1) * (size_t)a->kept_head + (size_t)a->keep) * 4 }, { "k_cache", a->k_cache, it_span(a->n, a->kc_slot, G, a->kc_head, D, 2) },
+                               { "v_cache", a->v_cache, it_span(a->n, a->vc_slot, G, a->vc_head, D, 2) } };         // (k and v may lie in one buffer)
+    for (int i = 0; i < 3; i++)
+        if (const char* x = it_overlaps(all[i], all + i + 1, 4 - i)) return it_fail(IT_EINVAL, "%s: %s overlaps %s", who, all[i].name, x);
     it_ops_device dev;
     if (const int r = it_ops_current(stream, who, &dev)) return r;
     if (const int r = ev_prepare(dev.device)) return r;

@@ -208,6 +208,8 @@ IT_API int it_norm_rope(void* stream, const it_norm_rope_args* a) {
                      "%s: k or v: pointers and strides are multiples of 4 elements, strides hold what lies between", who);
         IT_CHECK_ARG(it_aligned(a->k_cache, 16) && it_aligned(a->v_cache, 16) && a->slots >= 1 && a->slots <= 0x7fffffffll && it_strides_ok(a->slots, a->kc_slot, G, a->kc_head, D, 8) &&
                      it_strides_ok(a->slots, a->vc_slot, G, a->vc_head, D, 8), "%s: caches: 16-byte aligned, strides are multiples of 8 elements and hold what lies between", who);
+        const it_stretch caches[] = { { "k_cache", a->k_cache, it_span(a->slots, a->kc_slot, G, a->kc_head, D, 2) }, { "v_cache", a->v_cache, it_span(a->slots, a->vc_slot, G, a->vc_head, D, 2) } };
+        if (const char* x = a->q ? it_overlaps({ "q_out", a->q_out, it_span(T, a->qo_row, H, a->qo_head, D, es) }, caches, 2) : nullptr) return it_fail(IT_EINVAL, "%s: q_out overlaps %s", who, x);
         IT_CHECK_ARG(a->slot0 >= 0 && a->slot0 <= a->slots && (a->base || a->slot0 + T <= a->slots), "%s: rows at slots %lld .. of %lld", who, (long long)a->slot0, (long long)a->slots);
     }
     IT_CHECK_ARG(it_aligned(a->positions, 4) && it_aligned(a->base, 4) && it_aligned(a->q_norm, 16) && it_aligned(a->k_norm, 16), "%s: a pointer is not aligned to its type (norm weights: 16 bytes)", who);

@@ -18,6 +18,12 @@ static inline bool it_overlap(const void* a, size_t an, const void* b, size_t bn
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return x < y + bn && y < x + an;
 }
+// A stretch of memory that a call reads or writes, and the first of `others` (n of them) that shares a byte with it; null if none does.
+struct it_stretch { const char* name; const void* at; size_t bytes; };
+static inline const char* it_overlaps(const it_stretch& a, const it_stretch* others, int n) {
+    for (int i = 0; i < n; i++) if (a.at && others[i].at && a.bytes && others[i].bytes && it_overlap(a.at, a.bytes, others[i].at, others[i].bytes)) return others[i].name;
+    return nullptr;
+}
 // Bytes from the first to behind the last element of a [n0][n1][d] array with these strides.
 static inline size_t it_span(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t d, size_t size) {
     return n0 > 0 && n1 > 0 ? ((size_t)((n0 - 1) * s0 + (n1 - 1) * s1) + (size_t)d) * size : 0;

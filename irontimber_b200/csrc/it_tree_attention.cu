@@ -284,10 +284,16 @@ IT_API int it_tree_attention(void* stream, const it_tree_attention_args* a) {
     // a second walk for the received weights reads q after out is written
     IT_CHECK_ARG((same(a->q, a->q_row, a->q_head) && !a->weights) || !it_overlap(a->q, it_span(T, a->q_row, H, a->q_head, D, es), a->out, os), "%s: out overlaps q", who);
     IT_CHECK_ARG(!a->gate || same(a->gate, a->g_row, a->g_head) || !it_overlap(a->gate, it_span(T, a->g_row, H, a->g_head, D, es), a->out, os), "%s: out overlaps gate", who);
+    const TaPlan pl = ta_plan(a, it_tree_cut_of((long)a->rows * (a->heads / a->kv_heads), a->kv_heads, a->head_dim, ta_tiles(a), TA_MAXSPLITS));
+    // what a call writes is none of what it reads or writes elsewhere (out may be q or gate, see above)
+    const it_stretch all[] = { { "out", a->out, os }, { "weights", a->weights, ((size_t)(G - 1) * (size_t)a->w_head + (size_t)(a->cached + T)) * 4 }, { "the workspace", a->workspace, pl.total },
+                               { "k_cache", a->k_cache, it_span(a->cached + T, a->kc_slot, G, a->kc_head, D, 2) }, { "v_cache", a->v_cache, it_span(a->cached + T, a->vc_slot, G, a->vc_head, D, 2) },
+                               { "q", a->q, it_span(T, a->q_row, H, a->q_head, D, es) }, { "gate", a->gate, it_span(T, a->g_row, H, a->g_head, D, es) } };
+    for (int i = 0; i < 3; i++)
+        if (const char* x = it_overlaps(all[i], all + i + 1, i == 0 ? 4 : 6 - i)) return it_fail(IT_EINVAL, "%s: %s overlaps %s", who, all[i].name, x);
     it_ops_device dev;
     if (const int r = it_ops_current(stream, who, &dev)) return r;
     if (const int r = ta_prepare(dev.device)) return r;
-    const TaPlan pl = ta_plan(a, it_tree_cut_of((long)a->rows * (a->heads / a->kv_heads), a->kv_heads, a->head_dim, ta_tiles(a), TA_MAXSPLITS));
     IT_CHECK_ARG(a->workspace && it_aligned(a->workspace, 256) && a->workspace_bytes >= pl.total, "%s: a workspace of %zu bytes, 256-byte aligned, is needed", who, pl.total);
     CUtensorMap km, vm;
     if (const int r = ta_map(&km, a->k_cache, a->cache_type, a->head_dim, a->cached + T, a->kc_slot, a->kv_heads, a->kc_head)) return r;

@@ -114,3 +114,45 @@ def test_what_a_wait_that_ran_out_leaves_behind(tmp_path):
     lib.text.restype = ctypes.c_char_p
     assert all(s != lib.evict() and b"NaN" in lib.text(s) for s in sites)
     assert b"NaN" not in lib.text(lib.evict()) and b"moved in part" in lib.text(lib.evict())
+
+
+from tests.test_attention_ops import A, evict_args, lib, norm_rope_args, refused, tree_args  # noqa: E402,F401
+
+
+@pytest.mark.parametrize("change,part", [
+    (dict(q_out=5 * A), "q_out overlaps k_cache"), (dict(q_out=6 * A + 512), "q_out overlaps v_cache"), (dict(q_out=5 * A - 64), "q_out overlaps k_cache")])
+def test_norm_rope_does_not_write_what_it_writes_elsewhere(lib, change, part):
+    refused(lib, lib.it_norm_rope, norm_rope_args(**change), part)
+
+
+W = dict(weights=9 * A, w_head=300)
+
+
+@pytest.mark.parametrize("change,part", [
+    (dict(out=5 * A), "out overlaps k_cache"), (dict(out=6 * A + 204 * 128 * 2 + 192), "out overlaps v_cache"), (dict(out=9 * A + 4 * 300 + 16, **W), "out overlaps weights"), (dict(out=16 * A), "out overlaps the workspace"), (dict(out=16 * A + 512, **W), "out overlaps the workspace"),
+    (dict(W, weights=16 * A), "weights overlaps the workspace"), (dict(W, weights=5 * A + 4), "weights overlaps k_cache"), (dict(W, weights=A), "weights overlaps q"),
+    (dict(gate=11 * A, g_row=384, g_head=64, weights=11 * A + 4, w_head=300), "weights overlaps gate"), (dict(workspace=A + 256), "the workspace overlaps q"), (dict(workspace=5 * A), "the workspace overlaps k_cache"),
+    (dict(workspace=6 * A), "the workspace overlaps v_cache"), (dict(gate=16 * A, g_row=384, g_head=64), "the workspace overlaps gate")])
+def test_tree_attention_does_not_write_what_it_reads(lib, change, part):
+    refused(lib, lib.it_tree_attention, tree_args(**change), part)
+
+
+@pytest.mark.parametrize("change,part", [
+    (dict(workspace=7 * A), "the workspace overlaps weights"), (dict(workspace=8 * A), "the workspace overlaps kept"), (dict(workspace=5 * A), "the workspace overlaps k_cache"), (dict(kept=7 * A + 4 * 300), "weights overlaps kept"),
+    (dict(weights=6 * A), "weights overlaps v_cache"), (dict(kept=5 * A + 256), "kept overlaps k_cache")])
+def test_cache_evict_does_not_write_what_it_reads(lib, change, part):
+    refused(lib, lib.it_cache_evict, evict_args(**change), part)
+
+
+def test_memory_next_to_one_another_is_not_refused(lib):
+    if torch.cuda.is_available():
+        pytest.skip("addresses here are stand-ins")
+    import ctypes as C
+    n = C.c_size_t()
+    assert lib.it_tree_attention_workspace(C.byref(tree_args(**W)), C.byref(n)) == 0
+    for args in (tree_args(out=5 * A - 5 * 384 * 4), tree_args(out=5 * A + 205 * 128 * 2), tree_args(out=9 * A + 4 * (300 + 208), **W), tree_args(out=16 * A - 5 * 384 * 4, **W),
+                 tree_args(v_cache=5 * A + 128, kc_slot=256, vc_slot=256),                              # k and v of a slot side by side
+                 tree_args(gate=4 * A, g_row=384, g_head=64, **W)):                                     # out in gate's place
+        assert lib.it_tree_attention(None, C.byref(args)) == -2, lib.it_last_error()                    # as far as the device
+    assert lib.it_norm_rope(None, C.byref(norm_rope_args(q_out=5 * A - 5 * 384 * 4))) == -2
+    assert lib.it_cache_evict(None, C.byref(evict_args(kept=7 * A + 4 * (300 + 200)))) == -2
