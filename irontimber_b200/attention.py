@@ -99,6 +99,8 @@ _F16, _BF16, _F32, _I32T = torch.float16, torch.bfloat16, torch.float32, torch.i
 
 def _three(x, name, shape, dtype, index):
     """Address and outer strides of a [a, b, element] tensor of this shape with contiguous elements."""
+    if x is None:
+        raise ValueError(f"{name} is missing")
     st = x.stride()
     if x.shape != shape or x.dtype is not dtype or x.get_device() != index or st[2] != 1:
         _refuse_three(x, name, shape, dtype, index)
@@ -128,6 +130,8 @@ def _flat(x, name, n, dtype, index):
 
 def _caches(k, v, index):
     """Shape, type and the addresses and strides of a pair of caches."""
+    if k is None:
+        raise ValueError("k_cache is missing")
     shape, dtype = k.shape, k.dtype
     if dtype is not _F16 and dtype is not _BF16:
         raise TypeError(f"a cache is float16 or bfloat16, not {dtype}")
@@ -140,6 +144,8 @@ def _caches(k, v, index):
 
 
 def _rows(x, name):
+    if x is None:
+        raise ValueError(f"{name} is missing")
     shape = x.shape
     if len(shape) != 3:
         raise ValueError(f"{name} has the shape {tuple(shape)}, not three dimensions")
@@ -167,7 +173,9 @@ def norm_rope(rope, q, k, v, q_out, k_cache, v_cache, slot0, positions, q_norm=N
     q, q_out: [row, head, element] (q_out may be q); k, v: [row, kv head, element]; q_norm, k_norm: f32 weights of a head, or None for no norm; rope None: no
     rotation.  positions: int32 tensor [row], or the position of row 0.  base: int32 tensor whose value is added to slots (and to positions that
     are a number), read on the device.  q and q_out, or k, v and the caches, may be None."""
-    some, name = (q, "q") if q is not None else (k, "k")
+    some, name = (q, "q") if q is not None else (k, "k") if k is not None else (None, "q or k")
+    if rope is not None and rope.handle is None:
+        raise ValueError("rope is closed")
     shape = rows, heads, dim = _rows(some, name)
     act, index = some.dtype, some.get_device()
     t = ct = TYPES.get(act, -1)
@@ -220,6 +228,8 @@ def cache_evict(k_cache, v_cache, weights, n, keep, recent, kept=None, workspace
     """Cuts a cache of n slots to `keep` a KV head: the last `recent`, and of the others those with the largest weight (f32 [kv head, slot]; ties: the
     lower slot).  They move to the front in their order, in place, in both caches and the weights; kept (int32 [kv head, keep]) gets the slots they had.
     workspace: a uint8 tensor of cache_evict_workspace() bytes; None: one from torch's allocator."""
+    if weights is None:
+        raise ValueError("weights is missing")
     index = weights.get_device()
     (slots, kv, dim), _, kc, vc = _caches(k_cache, v_cache, index)
     wp, wh = _weights(weights, kv, n, index)

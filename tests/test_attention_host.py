@@ -156,3 +156,25 @@ def test_memory_next_to_one_another_is_not_refused(lib):
         assert lib.it_tree_attention(None, C.byref(args)) == -2, lib.it_last_error()                    # as far as the device
     assert lib.it_norm_rope(None, C.byref(norm_rope_args(q_out=5 * A - 5 * 384 * 4))) == -2
     assert lib.it_cache_evict(None, C.byref(evict_args(kept=7 * A + 4 * (300 + 200)))) == -2
+
+
+def test_missing_tensors_and_closed_ropes_are_refused(lib):
+    from irontimber_b200 import attention
+    q, kc = torch.zeros(3, 2, 64), torch.zeros(50, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="q or k is missing"):
+        attention.norm_rope(None, None, None, None, None, None, None, 0, 0)
+    with pytest.raises(ValueError, match="q_out is missing"):
+        attention.norm_rope(None, q, None, None, None, None, None, 0, 0)
+    with pytest.raises(ValueError, match="v is missing"):
+        attention.norm_rope(None, None, q, None, None, kc, kc.clone(), 0, 0)
+    with pytest.raises(ValueError, match="v_cache is missing"):
+        attention.norm_rope(None, None, q, q, None, kc, None, 0, 0)
+    rope = attention.Rope(64)
+    rope.close()
+    with pytest.raises(ValueError, match="rope is closed"):
+        attention.norm_rope(rope, q, None, None, q.clone(), None, None, 0, 0)
+    for args, part in (((None, kc, kc, 10, q), "q is missing"), ((q, None, kc, 10, q), "k_cache is missing"), ((q, kc, None, 10, q), "v_cache is missing"), ((q, kc, kc.clone(), 10, None), "out is missing")):
+        with pytest.raises(ValueError, match=part):
+            attention.tree_attention(*args)
+    with pytest.raises(ValueError, match="weights is missing"):
+        attention.cache_evict(kc, kc.clone(), None, 40, 20, 3)
