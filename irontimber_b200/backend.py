@@ -9,6 +9,7 @@ Hadamard is fused with q8k quantisation and `mv` consumes the quantised rows.
 Everything here is ctypes plumbing; all arithmetic runs in libirontimber_cuda.so on the GPU.
 """
 import ctypes as C
+import math
 
 import numpy as np
 
@@ -262,7 +263,7 @@ class CudaBackend:
     def view(self, off, *shape):
         """Arena elements off .. as a torch tensor of this shape (f32), without a copy; valid until close()."""
         import torch
-        if off % 4 or off + int(np.prod(shape)) > self.arena_floats:
+        if off < 0 or off % 4 or any(n < 0 for n in shape) or off + math.prod(shape) > self.arena_floats:
             raise ValueError(f"elements {off} .. of a shape {shape} in an arena of {self.arena_floats}; offsets are multiples of 4")
         return torch.as_tensor(_Floats(self.arena_ptr + 4 * off, shape), device=f"cuda:{self.device}")
 

@@ -178,3 +178,10 @@ def test_missing_tensors_and_closed_ropes_are_refused(lib):
             attention.tree_attention(*args)
     with pytest.raises(ValueError, match="weights is missing"):
         attention.cache_evict(kc, kc.clone(), None, 40, 20, 3)
+
+
+@pytest.mark.parametrize("off,shape", [(-4, (4,)), (-8, (2, 2)), (2, (4,)), (0, ((1 << 20) + 1,)), ((1 << 20) - 4, (5,)), (0, (-1, 8)), (0, (-2, -2)), (0, (1 << 32, 1 << 32)), (0, (1 << 62, 4))])
+def test_a_view_stays_in_the_arena(off, shape):
+    """In front of it, behind it, sizes below zero and sizes whose product does not fit 64 bits."""
+    with pytest.raises(ValueError, match="in an arena of"):
+        backend().view(off, *shape)
