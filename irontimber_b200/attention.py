@@ -99,9 +99,10 @@ _F16, _BF16, _F32, _I32T = torch.float16, torch.bfloat16, torch.float32, torch.i
 
 def _three(x, name, shape, dtype, index):
     """Address and outer strides of a [a, b, element] tensor of this shape with contiguous elements."""
-    if x is None:
-        raise ValueError(f"{name} is missing")
-    st = x.stride()
+    try:
+        st = x.stride()
+    except AttributeError:
+        raise ValueError(f"{name} is missing") from None
     if x.shape != shape or x.dtype is not dtype or x.get_device() != index or st[2] != 1:
         _refuse_three(x, name, shape, dtype, index)
     return x.data_ptr(), st[0], st[1]
@@ -130,9 +131,10 @@ def _flat(x, name, n, dtype, index):
 
 def _caches(k, v, index):
     """Shape, type and the addresses and strides of a pair of caches."""
-    if k is None:
-        raise ValueError("k_cache is missing")
-    shape, dtype = k.shape, k.dtype
+    try:
+        shape, dtype = k.shape, k.dtype
+    except AttributeError:
+        raise ValueError("k_cache is missing") from None
     if dtype is not _F16 and dtype is not _BF16:
         raise TypeError(f"a cache is float16 or bfloat16, not {dtype}")
     st = k.stride()
@@ -144,9 +146,10 @@ def _caches(k, v, index):
 
 
 def _rows(x, name):
-    if x is None:
-        raise ValueError(f"{name} is missing")
-    shape = x.shape
+    try:
+        shape = x.shape
+    except AttributeError:
+        raise ValueError(f"{name} is missing") from None
     if len(shape) != 3:
         raise ValueError(f"{name} has the shape {tuple(shape)}, not three dimensions")
     return shape
