@@ -384,7 +384,7 @@ int it_norm_rope(void* stream, const it_norm_rope_args* a);
  * Row t sees slot cached + j when j == t or j is an ancestor of t: parents[t] (device, i32) is the row it continues, or -1 for one that
  * continues the cache; a parent that is not a smaller row counts as -1.  parents NULL: a chain, row t sees rows 0..t.
  * out[t][h] = softmax(scale * q.k) v (* sigmoid(gate[t][h]) when gate is given); scale 0 means head_dim^-1/2.  What masked slots hold
- * (NaN, infinities, slots behind the last) does not reach the result.  `length` (device i32, may be NULL): the number of cached slots, clamped to
+ * (NaN, infinities, slots behind the last) does not reach the result; infinities that a row sees make it infinite or NaN.  `length` (device i32, may be NULL): the number of cached slots, clamped to
  * [0, cached], for recorded graphs.  weights (f32, [kv head][slot], slots contiguous, may be NULL): weights[g][slot] += the softmax weight
  * that the slot received from all rows and all query heads of kv head g; slots that no row sees are left alone.
  * slots: how many the cache has, >= cached + rows.  out may be gate itself, and without weights q itself (same strides; forming the weights may read q once more); otherwise out, weights and the
