@@ -26,7 +26,7 @@ static inline const char* it_overlaps(const it_stretch& a, const it_stretch* oth
 }
 // Bytes from the first to behind the last element of a [n0][n1][d] array with these strides.
 static inline size_t it_span(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t d, size_t size) {
-    return n0 > 0 && n1 > 0 ? ((size_t)((n0 - 1) * s0 + (n1 - 1) * s1) + (size_t)d) * size : 0;
+    return n0 > 0 && n1 > 0 ? ((size_t)(n0 - 1) * (size_t)s0 + (size_t)(n1 - 1) * (size_t)s1 + (size_t)d) * size : 0;
 }
 // Strides of a [n0][n1][d] array that nothing overlaps itself with: the smaller one holds a head, the larger one all of the other axis.
 static inline bool it_strides_ok(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t d, int64_t unit) {

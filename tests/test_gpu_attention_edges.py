@@ -158,3 +158,62 @@ def test_a_backend_is_closed_in_a_recording(ops):
         be.capture_begin()
         be.tree_attention(q, kc, vc, 500, torch.empty_like(q))
         be.close()
+
+
+def test_evictions_are_recorded_and_run_beside_one_another(ops):
+    """One recorded eviction replayed on other contents, and evictions of two caches on two streams at once, each with a workspace of its own."""
+    from tests.test_gpu_attention_ops import evict_plain
+    g = gen(23)
+    n, keep, recent, kv, dim = 9000, 5000, 70, 2, 64
+    state = [[randn(g, n, kv, dim).half(), randn(g, n, kv, dim).half(), torch.rand(kv, n, generator=g, device="cuda")] for _ in range(2)]
+    kept = [torch.empty(kv, keep, dtype=torch.int32, device="cuda") for _ in range(2)]
+    first = [[x.clone() for x in s] for s in state]
+    ops.cache_evict(*state[0], n, keep, recent, kept[0])                # outside of recording
+
+    def check(i, was):
+        for h in range(kv):
+            at = torch.tensor(evict_plain(was[2][h].cpu(), n, keep, recent), dtype=torch.long, device="cuda")
+            assert torch.equal(kept[i][h].long(), at)
+            assert all(torch.equal(state[i][k][:keep, h], was[k][at, h]) and torch.equal(state[i][k][keep:], was[k][keep:]) for k in (0, 1))
+            assert torch.equal(state[i][2][h, :keep], was[2][h, at])
+
+    check(0, first[0])
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        ops.cache_evict(*state[0], n, keep, recent, kept[0])
+    for turn in range(4):
+        was = [randn(g, n, kv, dim).half(), randn(g, n, kv, dim).half(), torch.rand(kv, n, generator=g, device="cuda")]
+        for x, y in zip(state[0], was):
+            x.copy_(y)
+        gr.replay()
+        check(0, was)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(8):
+        for i in (0, 1):
+            for x, y in zip(state[i], first[i]):
+                x.copy_(y)
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            ops.cache_evict(*state[i], n, keep, recent, kept[i], stream=streams[i])
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            check(i, first[i])
+
+
+def test_a_recorded_call_with_weights_adds_them_at_every_replay(ops):
+    """Kept scores (by their own launch and beside the joining) and the second walk, at a length that moves between replays."""
+    for kind, rows, heads, kv, dim, most in (("f32", 1, 6, 1, 64, 3000), ("f32", 20, 24, 4, 256, 2091), ("bf16", 256, 40, 2, 136, 6800)):
+        q, kc, vc, g = make(kind, rows, most, heads, kv, dim, 24)
+        par = torch.tensor(random_parents(rows, 1), dtype=torch.int32, device="cuda")
+        n = torch.tensor([most], dtype=torch.int32, device="cuda")
+        out, got, want, ref = torch.empty_like(q), torch.zeros(kv, most + rows, device="cuda"), torch.empty_like(q), torch.zeros(kv, most + rows, device="cuda")
+        ops.tree_attention(q, kc, vc, most, want, parents=par, length=n, weights=ref)
+        ref.zero_()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            ops.tree_attention(q, kc, vc, most, out, parents=par, length=n, weights=got)
+        for real in (most, 0, 127, most - 1, 128):
+            n.fill_(real)
+            gr.replay()
+            ops.tree_attention(q, kc, vc, most, want, parents=par, length=n, weights=ref)
+            assert torch.equal(out, want) and torch.equal(got, ref)
